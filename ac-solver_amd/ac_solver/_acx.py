@@ -18,7 +18,7 @@ LIB_PATH = os.environ.get("ACX_LIB", os.path.join(os.path.dirname(_HERE), "lib",
 # return codes / flags (mirror include/acx.h)
 OK, E_INVAL, E_NODEVICE, E_NOMEM, E_ROWERR, E_CAPACITY = 0, -1, -2, -3, -4, -5
 F_CYCLICAL, F_NO_SIMPLIFY, F_NO_MOVE, F_BYTES = 1, 2, 4, 8
-U8, I32, I64, I8, F32 = 0, 1, 2, 3, 4
+U8, I32, I64, I8, F32, BF16, F16 = range(7)
 ENV_RECORD_ACTIONS = 1
 SEARCH_BFS, SEARCH_GREEDY = 0, 1
 ERR_ASSERT, ERR_INDEX, ERR_VALUE, ERR_UNPACKABLE = 1, 2, 3, 250
@@ -152,6 +152,10 @@ SIGNATURES = {
     "acx_get_option": (C.c_int64, [C.c_int]),
     "acx_policy_sample": (C.c_int, [_vp, C.c_int, C.c_int64, C.c_int, _vp, _vp, C.c_int, C.c_uint64, _vp, _vp, _vp, _vp]),
     "acx_policy_packed_bytes": (C.c_int64, [C.c_int]),
+    "acx_scan_bounds_bytes": (C.c_int64, [C.c_int64] * 3),
+    "acx_scan_workspace_bytes": (C.c_int64, [C.c_int64] * 3 + [C.c_int]),
+    "acx_scan_forward": (C.c_int, [_vp, C.c_int64, C.c_int64, _vp, C.c_int64, C.c_int64, C.c_int, _vp, _vp] + [C.c_int64] * 3 + [_vp, _vp, _vp, _vp, C.c_int64, _vp]),
+    "acx_scan_backward": (C.c_int, [_vp, C.c_int64, C.c_int64] * 3 + [C.c_int, _vp, _vp, _vp] + [C.c_int64] * 3 + [_vp, C.c_int64, C.c_int64] * 2 + [_vp, _vp, C.c_int64, _vp]),
     "acx_search_minima_enable": (C.c_int, [C.c_int]),
     "acx_search_last_minima": (C.c_int, [_i32p, C.c_int64, _i64p]),
     "acx_search_digest_enable": (C.c_int, [C.c_int]),

@@ -1,0 +1,101 @@
+"""The gated recurrence of the recurrent agent over a rollout [steps, environments, features], with its gradient: `acx_scan_forward` /
+`acx_scan_backward` (csrc/acx_scan.hip).  The reference's agent has no memory (ac_solver/agents/ppo_agent.py:11-109)."""
+import torch
+
+from ac_solver import _acx
+from ac_solver.agents import _tensors as T
+
+
+def _operands(candidate, gate, reset, state):
+    candidate = T.activation(candidate, "candidate")
+    if candidate.dim() != 3:
+        raise ValueError(f"candidate has to be [steps, rows, features], not {tuple(candidate.shape)}")
+    gate = T.activation(gate, "gate", like=candidate, shape=candidate.shape)
+    steps, rows, width = candidate.shape
+    if steps < 1:
+        raise ValueError("a scan needs at least one step")
+    if reset is not None:
+        if isinstance(reset, torch.Tensor) and reset.dtype == torch.bool:
+            reset = reset.view(torch.uint8)
+        reset = T.plain(reset, "reset", (steps, rows), candidate.device, torch.uint8)
+    if state is not None:
+        state = T.plain(state, "state", (rows, width), candidate.device)
+    T.require_gpu(candidate)
+    return candidate, gate, reset, state
+
+
+def gated_scan_forward(candidate, gate, reset=None, state=None, save=True):
+    """The forward pass alone -> (hidden, last_state, bounds); `bounds` is what `gated_scan_backward` needs besides the operands, None
+    without `save`."""
+    candidate, gate, reset, state = _operands(candidate, gate, reset, state)
+    steps, rows, width = candidate.shape
+    dev = candidate.device
+    hidden = torch.empty((steps, rows, width), dtype=candidate.dtype, device=dev)
+    last = torch.empty((rows, width), dtype=torch.float32, device=dev)
+    bounds = torch.empty(_acx.lib.acx_scan_bounds_bytes(steps, rows, width) // 4, dtype=torch.float32, device=dev) if save else None
+    code = T.DTYPES[candidate.dtype]
+    work = T.scratch(_acx.lib.acx_scan_workspace_bytes(steps, rows, width, code), dev)
+    with T.on_device_of(candidate):
+        _acx.check(_acx.lib.acx_scan_forward(candidate.data_ptr(), candidate.stride(0), candidate.stride(1), gate.data_ptr(), gate.stride(0), gate.stride(1), code,
+                                             T.ptr(reset), T.ptr(state), steps, rows, width, hidden.data_ptr(), last.data_ptr(), T.ptr(bounds), T.ptr(work),
+                                             0 if work is None else work.numel(), T.stream_of(candidate)), "acx_scan_forward")
+    return hidden, last, bounds
+
+
+def gated_scan_backward(d_hidden, d_last, candidate, gate, reset, bounds, want_state=True, out=None):
+    """Gradients of candidate, gate and initial state from those of hidden and last state (`d_last` may be None).  `out`: two tensors
+    [steps, rows, features] to write the first two into (slices of a projection's gradient, say).  -> (d_candidate, d_gate, d_state or None)"""
+    candidate, gate, reset, _ = _operands(candidate, gate, reset, None)
+    steps, rows, width = candidate.shape
+    dev = candidate.device
+    d_hidden = T.activation(d_hidden, "d_hidden", like=candidate, shape=candidate.shape)
+    d_last = None if d_last is None else T.plain(d_last, "d_last", (rows, width), dev)
+    bounds = T.plain(bounds, "bounds", (_acx.lib.acx_scan_bounds_bytes(steps, rows, width) // 4,), dev)
+    if out is None:
+        dc, dz = (torch.empty((steps, rows, width), dtype=candidate.dtype, device=dev) for _ in range(2))
+    else:
+        dc, dz = out
+        for t, name in ((dc, "out[0]"), (dz, "out[1]")):
+            if T.activation(t, name, like=candidate, shape=candidate.shape) is not t:
+                raise ValueError(f"{name} has to have a contiguous last axis")
+    d_state = torch.empty((rows, width), dtype=torch.float32, device=dev) if want_state else None
+    code = T.DTYPES[candidate.dtype]
+    work = T.scratch(_acx.lib.acx_scan_workspace_bytes(steps, rows, width, code), dev)
+    with T.on_device_of(candidate):
+        _acx.check(_acx.lib.acx_scan_backward(candidate.data_ptr(), candidate.stride(0), candidate.stride(1), gate.data_ptr(), gate.stride(0), gate.stride(1),
+                                              d_hidden.data_ptr(), d_hidden.stride(0), d_hidden.stride(1), code, T.ptr(reset), bounds.data_ptr(), T.ptr(d_last), steps, rows,
+                                              width, dc.data_ptr(), dc.stride(0), dc.stride(1), dz.data_ptr(), dz.stride(0), dz.stride(1), T.ptr(d_state), T.ptr(work),
+                                              0 if work is None else work.numel(), T.stream_of(candidate)), "acx_scan_backward")
+    return dc, dz, d_state
+
+
+class _GatedScan(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, candidate, gate, reset, state):
+        hidden, last, bounds = gated_scan_forward(candidate, gate, reset, state, save=any(ctx.needs_input_grad))
+        ctx.save_for_backward(candidate, gate, reset, bounds)
+        ctx.set_materialize_grads(False)
+        return hidden, last
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, d_hidden, d_last):
+        candidate, gate, reset, bounds = ctx.saved_tensors
+        if d_hidden is None:
+            if d_last is None:
+                return None, None, None, None
+            d_hidden = torch.zeros((), dtype=candidate.dtype, device=candidate.device).expand(candidate.shape)
+        dc, dz, d_state = gated_scan_backward(d_hidden, d_last, candidate, gate, reset, bounds, ctx.needs_input_grad[3])
+        return dc if ctx.needs_input_grad[0] else None, dz if ctx.needs_input_grad[1] else None, None, d_state
+
+
+def gated_scan(candidate, gate, reset=None, state=None):
+    """Along the steps t of candidate, gate [steps, rows, features] (float32, bfloat16 or float16; slices of a projection as they are):
+
+        f = sigmoid(gate[t]);  h[t] = f * h[t - 1] + (1 - f) * candidate[t]
+
+    with h[t - 1] replaced by zero where `reset` [steps, rows] (bool) says that an episode starts at step t, and h[-1] = `state`
+    [rows, features] float32, or zero.  The recurrence runs in float32 whatever the type of the activations.
+    -> (hidden [steps, rows, features] of the activations' type, last state [rows, features] float32); both differentiable (once) with
+    respect to candidate, gate and state."""
+    return _GatedScan.apply(candidate, gate, reset, state)

@@ -1,0 +1,92 @@
+// acx_elem.h -- element types and wave helpers of the recurrent agent's operators (acx_scan.hip, acx_block.hip, acx_act8.hip).
+#pragma once
+#include "acx_common.h"
+
+namespace acx {
+namespace elem {
+
+// Activations are float, bfloat16 or float16; every computation on them is in float32.  A rounding to 16 bits is the hardware's, to
+// nearest even, and happens once, at the store.
+typedef __bf16 bf16_t;
+typedef _Float16 f16_t;
+
+// V elements of E behind a pointer that is aligned for E alone: a strided slice, or a row of odd width, may start anywhere, and global
+// memory takes 16-byte accesses at any address on this chip (a misaligned one costs a second cache line at most)
+template <class E, int V> struct Vec {
+    typedef E type __attribute__((ext_vector_type(V), aligned(sizeof(E))));
+};
+template <class E> struct Vec<E, 1> {
+    typedef E type;
+};
+
+template <class E, int V> __device__ __forceinline__ void load(const E* p, float (&out)[V]) {
+    if constexpr (V == 1) {
+        out[0] = (float)*p;
+    } else {
+        const typename Vec<E, V>::type v = *(const typename Vec<E, V>::type*)p;
+#pragma unroll
+        for (int i = 0; i < V; i++) out[i] = (float)v[i];
+    }
+}
+template <class E, int V> __device__ __forceinline__ void store(E* p, const float (&in)[V]) {
+    if constexpr (V == 1) {
+        *p = (E)in[0];
+    } else {
+        typename Vec<E, V>::type v;
+#pragma unroll
+        for (int i = 0; i < V; i++) v[i] = (E)in[i];
+        *(typename Vec<E, V>::type*)p = v;
+    }
+}
+// the first `valid` of V elements (the end of a row); the others read as zero and are not touched
+template <class E, int V> __device__ __forceinline__ void load_some(const E* p, int valid, float (&out)[V]) {
+    if (valid >= V) {
+        load<E, V>(p, out);
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; i++) out[i] = i < valid ? (float)p[i] : 0.0f;
+    }
+}
+template <class E, int V> __device__ __forceinline__ void store_some(E* p, int valid, const float (&in)[V]) {
+    if (valid >= V) {
+        store<E, V>(p, in);
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; i++)
+            if (i < valid) p[i] = (E)in[i];
+    }
+}
+
+// sigmoid of z and of -z from one exponential: e = exp(-|z|), the smaller of the two is e / (1 + e), and the larger 1 minus it, which
+// loses nothing (the smaller one as 1 - sigmoid would).  exp(-|z|) = 2^t (1 + l ln 2) with t = -|z| log2 e rounded and l what the rounding
+// and the constant left out: the error of t alone would grow to |z| 2^-24.  PRECISE false leaves l out: for 16-bit results.
+// NaN comes out as NaN, +-infinity as 0 and 1.
+template <bool PRECISE> __device__ __forceinline__ float small_sigmoid(float z) {
+    constexpr float kLog2e = 1.44269502162933349609375f, kLog2eLow = 1.92596299e-8f, kLn2 = 0.693147182464599609375f;
+    const float a = -__builtin_fabsf(z);
+    const float t = a * kLog2e;
+    float e = __builtin_amdgcn_exp2f(t);
+    if constexpr (PRECISE) {
+        const float l = __builtin_fmaf(a, kLog2eLow, __builtin_fmaf(a, kLog2e, -t));
+        // (at infinity l is NaN and e is 0: the comparison keeps the 0, and a NaN of z is in e already)
+        e = t < -126.0f ? e : __builtin_fmaf(e * l, kLn2, e);
+    }
+    return e * __builtin_amdgcn_rcpf(1.0f + e);
+}
+// sigmoid(z) and 1 - sigmoid(z) from small_sigmoid(z)
+__device__ __forceinline__ float keep_of(float z, float s) { return z < 0.0f ? s : 1.0f - s; }
+__device__ __forceinline__ float take_of(float z, float s) { return z < 0.0f ? 1.0f - s : s; }
+
+// run fn.template operator()<E>() for the element type of an ACX_* code; false for any other code
+template <class F> static inline bool with_element(int dtype, F&& fn) {
+    switch (dtype) {
+        case ACX_F32: fn((float*)nullptr); return true;
+        case ACX_BF16: fn((bf16_t*)nullptr); return true;
+        case ACX_F16: fn((f16_t*)nullptr); return true;
+        default: return false;
+    }
+}
+static inline int element_bytes(int dtype) { return dtype == ACX_F32 ? 4 : 2; }
+
+}  // namespace elem
+}  // namespace acx

@@ -31,7 +31,7 @@
 extern "C" {
 #endif
 
-#define ACX_VERSION 600  /* history: INTEGRATION.md, "ACX_VERSION history" */
+#define ACX_VERSION 700  /* history: INTEGRATION.md, "ACX_VERSION history" */
 
 /* return codes */
 #define ACX_OK 0
@@ -47,12 +47,14 @@ extern "C" {
 #define ACX_F_NO_MOVE 4     /* simplify_presentation only (ACX_F_BYTES only) */
 #define ACX_F_BYTES 8       /* byte-exact kernel: any int8 letters, invalid rows, L <= 128 */
 
-/* dtypes of action / observation buffers */
+/* dtypes of action / observation buffers and of activations */
 #define ACX_U8 0
 #define ACX_I32 1
 #define ACX_I64 2
 #define ACX_I8 3
 #define ACX_F32 4
+#define ACX_BF16 5
+#define ACX_F16 6
 
 int acx_version(void);
 const char *acx_last_error(void);
@@ -343,6 +345,26 @@ int acx_shard_check_owners(acx_shard *h, int64_t *n_bad, void *stream);
 int acx_policy_sample(const void *d_obs, int obs_dtype, int64_t n_env, int in_dim, const void *d_actor, const void *d_critic,
                       int n_actions, uint64_t seed, int64_t *d_action, float *d_logprob, float *d_value, void *stream);
 int64_t acx_policy_packed_bytes(int in_dim);
+
+/* ---- recurrent agent: gated recurrence over a rollout (csrc/acx_scan.hip) -----------------------------------------------------
+ * No counterpart in the reference, whose agent has no memory (agents/ppo_agent.py:11-109).  For every row n < N and feature d < D, along
+ * the steps t < T:
+ *     f = sigmoid(gate[t]),  h[t] = f * (d_reset[t, n] ? 0 : h[t - 1]) + (1 - f) * candidate[t],   h[-1] = d_state (NULL: 0)
+ * `dtype` (ACX_F32 / ACX_BF16 / ACX_F16) is the type of candidate, gate, hidden and their gradients; states are float32.  A tensor of
+ * activations is given with the strides of its steps and rows in elements (features contiguous, any alignment of the type itself);
+ * d_hidden is contiguous [T, N, D], d_reset [T, N] bytes (nullable), d_state and d_last [N, D] (different buffers).
+ * d_bounds (nullable: no gradient wanted; acx_scan_bounds_bytes) takes what acx_scan_backward needs besides the operands.
+ * d_work: acx_scan_workspace_bytes of scratch for the duration of the call's kernels, not shared with another call in flight.
+ * acx_scan_backward: gradients of candidate, gate and state (nullable) from those of hidden and last (nullable). */
+int64_t acx_scan_bounds_bytes(int64_t T, int64_t N, int64_t D);
+int64_t acx_scan_workspace_bytes(int64_t T, int64_t N, int64_t D, int dtype);
+int acx_scan_forward(const void *d_candidate, int64_t c_step, int64_t c_row, const void *d_gate, int64_t z_step, int64_t z_row, int dtype,
+                     const uint8_t *d_reset, const float *d_state, int64_t T, int64_t N, int64_t D, void *d_hidden, float *d_last,
+                     float *d_bounds, void *d_work, int64_t work_bytes, void *stream);
+int acx_scan_backward(const void *d_candidate, int64_t c_step, int64_t c_row, const void *d_gate, int64_t z_step, int64_t z_row,
+                      const void *d_hidden_grad, int64_t g_step, int64_t g_row, int dtype, const uint8_t *d_reset, const float *d_bounds,
+                      const float *d_last_grad, int64_t T, int64_t N, int64_t D, void *d_candidate_grad, int64_t dc_step, int64_t dc_row,
+                      void *d_gate_grad, int64_t dz_step, int64_t dz_row, float *d_state_grad, void *d_work, int64_t work_bytes, void *stream);
 
 /* ---- neighbourhood sizes ------------------------------------------------------------
  * Replaces `neibourhood` of the reference's C++ side program (barcode_analysis/5_steps_neibourhoods/neibourhoods.cpp:18-54,

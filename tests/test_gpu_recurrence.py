@@ -1,0 +1,257 @@
+"""gated_scan (csrc/acx_scan.hip): the recurrence and its gradient against the definition in float64, at the lengths, widths, strides and
+resets where a segment, a wave's share or a chunk of the steps ends; its refusals are in test_recurrence_cpu.py."""
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+DTYPES = ("float32", "bfloat16", "float16")
+
+
+def inputs(T, N, D, dtype, seed, reset=True, state=True, layout="contiguous"):
+    import torch
+
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    dt = getattr(torch, dtype)
+
+    def make(scale, shift=0.0):
+        x = torch.randn((T, N, D), device="cuda", generator=g) * scale + shift
+        return x.to(dt)
+
+    c, z, dh = make(1.0), make(1.5, 2.0), make(0.5)
+    if layout == "slices":  # slices of one projection, as the agent has them
+        p = torch.empty((T, N, 3 * D + 1), device="cuda", dtype=dt)
+        p[..., :D], p[..., D:2 * D] = c, z
+        c, z = p[..., :D], p[..., D:2 * D]
+    elif layout == "rows first":  # [rows, steps, features] in memory
+        c, z, dh = (x.transpose(0, 1).contiguous().transpose(0, 1) for x in (c, z, dh))
+    r = (torch.rand((T, N), device="cuda", generator=g) < 0.1) if reset else None
+    s = torch.randn((N, D), device="cuda", generator=g) if state else None
+    dl = torch.randn((N, D), device="cuda", generator=g) * 0.5 if state else None
+    return c, z, r, s, dh, dl
+
+
+def definition(c, z, r, s, dh, dl):
+    """hidden, last, gradients in float64, step by step"""
+    import torch
+
+    c, z, dh = c.double(), z.double(), dh.double()
+    T = c.shape[0]
+    f, k = torch.sigmoid(z), torch.sigmoid(-z)
+    h = torch.zeros_like(c[0]) if s is None else s.double()
+    hs, before = [], []
+    for t in range(T):
+        if r is not None:
+            h = h.masked_fill(r[t, :, None], 0.0)
+        before.append(h)
+        h = f[t] * h + k[t] * c[t]
+        hs.append(h)
+    x = torch.zeros_like(c[0]) if dl is None else dl.double()
+    dc, dz = [None] * T, [None] * T
+    for t in range(T - 1, -1, -1):
+        G = dh[t] + x
+        dc[t] = k[t] * G
+        dz[t] = f[t] * k[t] * (before[t] - c[t]) * G
+        x = f[t] * G
+        if r is not None:
+            x = x.masked_fill(r[t, :, None], 0.0)
+    return torch.stack(hs), h, torch.stack(dc), torch.stack(dz), x
+
+
+def assert_close(got, want, dtype, what, top=None):
+    """Tolerance: one rounding to the output's type, |want| eps / 2, plus the float32 arithmetic in front of it.  That arithmetic adds up at most
+    sum of f^j ~ 1 / (1 - f) terms that matter, with a relative error of a few 2^-24 each, of values no larger than the largest one: 64 * 2^-24
+    of the largest magnitude of the tensor covers forty operations on each of the terms that have not decayed."""
+    import torch
+
+    top = float(want.abs().max()) if top is None else top
+    eps = torch.finfo(getattr(torch, dtype)).eps / 2
+    err = (got.double() - want).abs()
+    tiny = torch.finfo(getattr(torch, dtype)).smallest_normal * eps if dtype == "float16" else 0.0
+    lim = want.abs() * eps * (1 + 2 ** -7) + top * 64 * 2.0 ** -24 + tiny
+    bad = err > lim
+    assert not bool(bad.any()), f"{what}: {int(bad.sum())} of {err.numel()} off, worst {float((err - lim).max())} beyond the tolerance"
+
+
+def check(T, N, D, dtype, seed=0, **kw):
+    import torch
+
+    from ac_solver.agents.recurrence import gated_scan
+
+    c, z, r, s, dh, dl = inputs(T, N, D, dtype, seed, **kw)
+    print(f"T {T} N {N} D {D} {dtype} {kw}", flush=True)
+    leaves = [t.detach().requires_grad_() for t in ([c, z] if s is None else [c, z, s])]
+    hidden, last = gated_scan(leaves[0], leaves[1], reset=r, state=leaves[2] if s is not None else None)
+    assert hidden.dtype == c.dtype and last.dtype == torch.float32 and hidden.is_contiguous()
+    outs, gouts = ([hidden, last], [dh, dl]) if s is not None else ([hidden], [dh])
+    grads = torch.autograd.grad(outs, leaves, gouts)
+    want = definition(c, z, r, s, dh, dl)
+    assert_close(hidden, want[0], dtype, "hidden")
+    assert_close(last, want[1], "float32", "last")
+    gtop = float(want[2].abs().max()) + float(dh.abs().max()) * 4  # (G itself, before the factor 1 - f, can be larger than dc)
+    assert_close(grads[0], want[2], dtype, "d candidate", gtop)
+    assert_close(grads[1], want[3], dtype, "d gate", gtop * 4)
+    if s is not None:
+        assert_close(grads[2], want[4], "float32", "d state", gtop)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("T", [1, 2, 15, 16, 17, 63, 64, 65, 255, 257, 600])
+def test_lengths(T, dtype):
+    check(T, 3, 70, dtype)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("N,D", [(1, 1), (1, 2), (5, 1), (3, 33), (2, 64), (1, 129), (7, 130), (2, 1031)])
+def test_widths(N, D, dtype):
+    check(37, N, D, dtype, reset=N % 2 == 1, state=D % 2 == 0)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("layout", ["slices", "rows first"])
+@pytest.mark.parametrize("D", [50, 63])
+def test_strides(D, layout, dtype):
+    check(70, 9, D, dtype, layout=layout)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_one_wave_over_all_steps(dtype):
+    check(50, 1030, 256, dtype)  # channels enough for W = 1 (2048 groups and more)
+    check(35, 520, 130, dtype, state=False)
+
+
+@pytest.mark.parametrize("T", [4096, 5003])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_chunks_of_a_long_sequence(T, dtype):
+    check(T, 2, 66, dtype)
+    check(T, 1, 1, dtype, reset=False)
+
+
+def test_resets_cut_infinities_and_nans_off():
+    """what an episode left behind, infinite or NaN, does not reach the next one; gradients of the steps before are those of a cut"""
+    import torch
+
+    from ac_solver.agents.recurrence import gated_scan
+
+    for T in (40, 4100):  # within one launch; through the composed chunks
+        c, z, _, s, dh, dl = inputs(T, 2, 64, "float32", 3)
+        r = torch.zeros((T, 2), dtype=torch.bool, device="cuda")
+        r[T // 2] = True
+        s[0], s[1] = float("inf"), float("nan")
+        c[3, 0] = float("nan")
+        hidden, last = gated_scan(c, z, reset=r, state=s)
+        assert not torch.isfinite(hidden[0]).any()
+        fresh, fresh_last = gated_scan(c[T // 2:], z[T // 2:])
+        assert torch.isfinite(hidden[T // 2:]).all() and torch.isfinite(last).all()
+        # (cut into other segments: other roundings)
+        assert float((hidden[T // 2:] - fresh).abs().max()) < 64 * 2.0 ** -24 * float(fresh.abs().max())
+        assert float((last - fresh_last).abs().max()) < 64 * 2.0 ** -24 * float(fresh.abs().max())
+
+
+def test_gates_at_the_ends_of_their_range():
+    """z = +-infinity, +-200, 0: f is exactly 1, 0 and 1 / 2, and 1 - f keeps its accuracy where f rounds to 1"""
+    import torch
+
+    from ac_solver.agents.recurrence import gated_scan
+
+    z = torch.tensor([float("inf"), -float("inf"), 200.0, -200.0, 0.0, -0.0, 20.0, -20.0], device="cuda").view(1, 1, -1)
+    c = torch.full_like(z, 3.0)
+    s = torch.full((1, 8), 5.0, device="cuda")
+    hidden, _ = gated_scan(c, z, state=s)
+    want = (torch.sigmoid(z.double()) * 5 + torch.sigmoid(-z.double()) * 3)[0]
+    assert float((hidden[0].double() - want).abs().max()) <= 5 * 2.0 ** -22
+    hidden, _ = gated_scan(c, z)  # state 0: h = (1 - f) c alone
+    want = torch.sigmoid(-z.double()) * 3
+    ok = (hidden.double() - want).abs() <= want * 8 * 2.0 ** -24 + 1e-37
+    assert bool(ok.all()), (hidden, want)
+
+
+def test_gradient_against_differences():
+    """central differences of the kernel's own forward pass in float32: step 2^-6 on values of order one leaves h^2 / 6 f''' ~ 1e-4 and
+    rounding 2^-24 / 2^-6 * |sum|"""
+    import torch
+
+    from ac_solver.agents.recurrence import gated_scan
+
+    c, z, r, s, dh, dl = inputs(20, 2, 5, "float32", 11)
+    leaves = [t.detach().clone().requires_grad_() for t in (c, z, s)]
+
+    def loss(c, z, s):
+        h, last = gated_scan(c, z, reset=r, state=s)
+        return (h.double() * dh.double()).sum() + (last.double() * dl.double()).sum()
+
+    grads = torch.autograd.grad(loss(*leaves), leaves)
+    g = torch.Generator(device="cuda").manual_seed(5)
+    for k in range(3):
+        for _ in range(6):
+            e = torch.zeros_like(leaves[k])
+            i = int(torch.randint(0, e.numel(), (1,), device="cuda", generator=g))
+            e.view(-1)[i] = 2.0 ** -6
+            args = [t.detach() for t in leaves]
+            up, down = list(args), list(args)
+            up[k], down[k] = args[k] + e, args[k] - e
+            num = float((loss(*up) - loss(*down)) / 2 ** -5)
+            assert abs(num - float(grads[k].view(-1)[i])) < 2e-3
+
+
+def test_only_what_is_asked_for_is_differentiated():
+    import torch
+
+    from ac_solver.agents.recurrence import gated_scan
+
+    c, z, r, s, dh, dl = inputs(18, 2, 8, "float32", 2)
+    want = definition(c, z, r, s, torch.zeros_like(dh), dl)
+    c2 = c.clone().requires_grad_()
+    _, last = gated_scan(c2, z, reset=r, state=s)  # only the last state is used
+    (g,) = torch.autograd.grad(last, [c2], dl)
+    assert_close(g, want[2], "float32", "d candidate of the last state", 4.0)
+    hidden, _ = gated_scan(c2, z, reset=r, state=s)
+    (g,) = torch.autograd.grad(hidden.sum(), [c2])  # an expanded gradient: no strides at all
+    want = definition(c, z, r, s, torch.ones_like(dh), None)
+    assert_close(g, want[2], "float32", "d candidate of a sum", 40.0)
+    with torch.no_grad():
+        assert not gated_scan(c2, z)[0].requires_grad
+
+
+def test_other_streams_and_repeated_calls_agree():
+    import torch
+
+    from ac_solver.agents.recurrence import gated_scan_backward, gated_scan_forward
+
+    c, z, r, s, dh, dl = inputs(4100, 2, 66, "bfloat16", 8)
+    first = gated_scan_forward(c, z, r, s)
+    grads = gated_scan_backward(dh, dl, c, z, r, first[2])
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    for _ in range(3):
+        with torch.cuda.stream(side):
+            again = gated_scan_forward(c, z, r, s)
+            g2 = gated_scan_backward(dh, dl, c, z, r, again[2])
+        here = gated_scan_forward(c, z, r, s)
+        side.synchronize()
+        for a, b, d in zip(first + grads, again + g2, here):
+            assert torch.equal(a, b)
+        assert all(torch.equal(a, b) for a, b in zip(first, here))
+
+
+def test_a_captured_pass_replays():
+    """forward and backward captured into one graph, replayed on new inputs with eager calls between the replays"""
+    import torch
+
+    from ac_solver.agents.recurrence import gated_scan_backward, gated_scan_forward
+
+    c, z, r, s, dh, dl = inputs(4100, 2, 66, "float32", 8)
+    gated_scan_forward(c, z, r, s)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        hidden, last, bounds = gated_scan_forward(c, z, r, s)
+        grads = gated_scan_backward(dh, dl, c, z, r, bounds)
+    for seed in (1, 2, 3):
+        for dst, src in zip((c, z, r, s, dh, dl), inputs(4100, 2, 66, "float32", seed)):
+            dst.copy_(src)
+        graph.replay()
+        torch.cuda.synchronize()
+        want = gated_scan_forward(c, z, r, s)
+        wg = gated_scan_backward(dh, dl, c, z, r, want[2])
+        for a, b in zip((hidden, last, bounds) + grads, want + wg):
+            assert torch.equal(a, b)
