@@ -4,6 +4,7 @@ import torch
 
 from ac_solver import _acx
 from ac_solver.agents import _tensors as T
+from ac_solver.agents.block_norm import MAX_WIDTH
 
 
 def _operands(candidate, gate, reset, state):
@@ -99,3 +100,45 @@ def gated_scan(candidate, gate, reset=None, state=None):
     -> (hidden [steps, rows, features] of the activations' type, last state [rows, features] float32); both differentiable (once) with
     respect to candidate, gate and state."""
     return _GatedScan.apply(candidate, gate, reset, state)
+
+
+def recurrent_step(x, projected, state, weight, scale=None, next_weight=None, reset=None, next_state=None, eps=1e-6):
+    """A whole block for ONE step of the environments in one launch (rollouts; no gradient): with candidate, gate, output gate = the
+    three thirds of projected [rows, 3 width],
+
+        h = gated_scan of one step from `state` [rows, width] float32 (zero where `reset` [rows] (bool) says that an episode starts)
+        new, u = block_output(x, h, output gate, weight, scale, next_weight, eps)
+
+    x and projected of one type (float32, bfloat16 or float16); h stays float32.  `next_state`: where the new state goes, `state` itself for
+    in place; None: a new tensor.  -> (new, u, next_state); u is None without `next_weight`."""
+    x = T.activation(x, "x")
+    if x.dim() != 2:
+        raise ValueError(f"x has to be [rows, features], not {tuple(x.shape)}")
+    rows, width = x.shape
+    if width > MAX_WIDTH:
+        raise ValueError(f"rows of up to {MAX_WIDTH} features are handled, not {width}")
+    if not eps >= 0.0:
+        raise ValueError(f"eps has to be a number of at least 0, not {eps}")
+    dev = x.device
+    projected = T.activation(projected, "projected", like=x, shape=(rows, 3 * width))
+    state = T.plain(state, "state", (rows, width), dev)
+    weight = T.plain(weight, "weight", (width,), dev)
+    scale = None if scale is None else T.plain(scale, "scale", (width,), dev)
+    next_weight = None if next_weight is None else T.plain(next_weight, "next_weight", (width,), dev)
+    if reset is not None:
+        if isinstance(reset, torch.Tensor) and reset.dtype == torch.bool:
+            reset = reset.view(torch.uint8)
+        reset = T.plain(reset, "reset", (rows,), dev, torch.uint8)
+    if next_state is not None and T.plain(next_state, "next_state", (rows, width), dev) is not next_state:
+        raise ValueError("next_state has to be contiguous")
+    T.require_gpu(x)
+    if next_state is None:
+        next_state = torch.empty_like(state)
+    new = torch.empty((rows, width), dtype=x.dtype, device=dev)
+    u = None if next_weight is None else torch.empty((rows, width), dtype=x.dtype, device=dev)
+    if rows and width:
+        with T.on_device_of(x):
+            _acx.check(_acx.lib.acx_block_step(x.data_ptr(), x.stride(0), projected.data_ptr(), projected.stride(0), T.DTYPES[x.dtype], T.ptr(reset), state.data_ptr(),
+                                               weight.data_ptr(), T.ptr(scale), T.ptr(next_weight), eps, rows, width, next_state.data_ptr(), new.data_ptr(), T.ptr(u),
+                                               T.stream_of(x)), "acx_block_step")
+    return new, u, next_state

@@ -366,6 +366,30 @@ int acx_scan_backward(const void *d_candidate, int64_t c_step, int64_t c_row, co
                       const float *d_last_grad, int64_t T, int64_t N, int64_t D, void *d_candidate_grad, int64_t dc_step, int64_t dc_row,
                       void *d_gate_grad, int64_t dz_step, int64_t dz_row, float *d_state_grad, void *d_work, int64_t work_bytes, void *stream);
 
+/* ---- recurrent agent: the end of a block (csrc/acx_block.hip) -------------------------------------------------------------------
+ * For each of M rows of D <= 8192 features (rms(v) = v / sqrt(mean(v^2) + eps)):
+ *     new = x + scale * silu(gate) * rms(y) * weight,   u = rms(new) * next_weight
+ * acx_block_forward: d_gate NULL: without the gate, d_scale NULL: 1, d_next_weight NULL: no u; d_y NULL: u = rms(x) * next_weight alone
+ * (d_new is not written).  Activations of type `dtype` with a stride between rows in elements, d_new and d_u contiguous; weights float32.
+ * d_stats (nullable: no gradient wanted): [M, 2] floats for acx_block_backward.
+ * acx_block_backward: gradients from those of new and u (each nullable: zero); d_weight_grads [3, D] takes those of weight, scale and
+ * next_weight, summed over the rows in a fixed order; d_work: acx_block_workspace_bytes for the duration of the call's kernels.
+ * acx_block_step: one step of the recurrence (acx_scan_forward) and the end of its block in one launch, no gradient: a row of d_projected
+ * holds candidate, gate of the recurrence and output gate, D each; y is the new state, which goes to d_next_state [M, D] (d_state
+ * itself: in place). */
+int64_t acx_block_workspace_bytes(int64_t M, int64_t D, int dtype);
+int acx_block_forward(const void *d_x, int64_t x_row, const void *d_y, int64_t y_row, const void *d_gate, int64_t g_row, int dtype,
+                      const float *d_weight, const float *d_scale, const float *d_next_weight, float eps, int64_t M, int64_t D, void *d_new,
+                      void *d_u, float *d_stats, void *stream);
+int acx_block_backward(const void *d_x, int64_t x_row, const void *d_y, int64_t y_row, const void *d_gate, int64_t g_row,
+                       const void *d_new_grad, int64_t dn_row, const void *d_u_grad, int64_t du_row, int dtype, const float *d_weight,
+                       const float *d_scale, const float *d_next_weight, const float *d_stats, int64_t M, int64_t D, void *d_x_grad,
+                       void *d_y_grad, void *d_gate_grad, int64_t dg_row, float *d_weight_grads, void *d_work, int64_t work_bytes,
+                       void *stream);
+int acx_block_step(const void *d_x, int64_t x_row, const void *d_projected, int64_t p_row, int dtype, const uint8_t *d_reset,
+                   const float *d_state, const float *d_weight, const float *d_scale, const float *d_next_weight, float eps, int64_t M,
+                   int64_t D, float *d_next_state, void *d_new, void *d_u, void *stream);
+
 /* ---- neighbourhood sizes ------------------------------------------------------------
  * Replaces `neibourhood` of the reference's C++ side program (barcode_analysis/5_steps_neibourhoods/neibourhoods.cpp:18-54,
  * moves and word arithmetic AC_UTILS_no_hash.cpp:83-211): number of distinct SORTED pairs of freely reduced relators

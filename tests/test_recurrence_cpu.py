@@ -49,3 +49,49 @@ def test_scan_buffer_sizes():
     assert _acx.lib.acx_scan_bounds_bytes(1, 2, 4) == 32 and _acx.lib.acx_scan_bounds_bytes(17, 2, 4) == 64 and _acx.lib.acx_scan_bounds_bytes(16, 0, 4) == 0
     assert _acx.lib.acx_scan_workspace_bytes(1, 1, 1, _acx.F32) == 0 and _acx.lib.acx_scan_workspace_bytes(1 << 16, 1, 256, _acx.BF16) > 0
     assert _acx.lib.acx_scan_workspace_bytes(32, 131072, 256, _acx.F32) == 0
+
+
+def test_the_block_end_refuses_what_it_cannot_read():
+    from ac_solver.agents import block_norm as B
+
+    x, w = torch.zeros(5, 8), torch.ones(8)
+    with pytest.raises(ValueError, match="GPU"):
+        B.block_output(x, x, x, w, w, w)
+    with pytest.raises(ValueError, match="GPU"):
+        B.block_input(x, w)
+    with pytest.raises(ValueError, match="8192"):
+        B.block_input(torch.zeros(1, 8193), torch.zeros(8193))
+    with pytest.raises(ValueError, match="y has the shape"):
+        B.block_output(x, x[:4], x, w)
+    with pytest.raises(ValueError, match="gate is"):
+        B.block_output(x, x, x.half(), w)
+    with pytest.raises(TypeError, match="weight"):
+        B.block_output(x, x, x, w.half())
+    with pytest.raises(ValueError, match="scale has the shape"):
+        B.block_output(x, x, x, w, w[:3])
+    with pytest.raises(TypeError, match="weight has to be a tensor"):
+        B.block_output(x, x, x, None)
+    with pytest.raises(ValueError, match="eps"):
+        B.block_input(x, w, eps=-1.0)
+    with pytest.raises(ValueError, match="eps"):
+        B.block_input(x, w, eps=float("nan"))
+    with pytest.raises(TypeError, match="float32, bfloat16 or float16"):
+        B.block_input(x.to(torch.int8), w)
+
+
+def test_a_step_refuses_what_it_cannot_read():
+    x, p, h, w = torch.zeros(5, 8), torch.zeros(5, 24), torch.zeros(5, 8), torch.ones(8)
+    with pytest.raises(ValueError, match="GPU"):
+        R.recurrent_step(x, p, h, w, w, w, reset=torch.zeros(5, dtype=torch.bool), next_state=h)
+    with pytest.raises(ValueError, match="projected has the shape"):
+        R.recurrent_step(x, p[:, :16], h, w)
+    with pytest.raises(ValueError, match="rows, features"):
+        R.recurrent_step(x[0], p, h, w)
+    with pytest.raises(TypeError, match="state"):
+        R.recurrent_step(x.half(), p.half(), h.half(), w)
+    with pytest.raises(ValueError, match="next_state has to be contiguous"):
+        R.recurrent_step(x, p, h, w, next_state=torch.zeros(8, 5).t())
+    with pytest.raises(TypeError, match="reset"):
+        R.recurrent_step(x, p, h, w, reset=torch.zeros(5))
+    with pytest.raises(ValueError, match="8192"):
+        R.recurrent_step(torch.zeros(1, 8193), torch.zeros(1, 3 * 8193), torch.zeros(1, 8193), torch.zeros(8193))
