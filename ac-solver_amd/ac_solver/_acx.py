@@ -160,6 +160,10 @@ SIGNATURES = {
     "acx_block_forward": (C.c_int, [_vp, C.c_int64] * 3 + [C.c_int, _vp, _vp, _vp, C.c_float, C.c_int64, C.c_int64, _vp, _vp, _vp, _vp]),
     "acx_block_backward": (C.c_int, [_vp, C.c_int64] * 5 + [C.c_int, _vp, _vp, _vp, _vp, C.c_int64, C.c_int64, _vp, _vp, _vp, C.c_int64, _vp, _vp, C.c_int64, _vp]),
     "acx_block_step": (C.c_int, [_vp, C.c_int64] * 2 + [C.c_int, _vp, _vp, _vp, _vp, _vp, C.c_float, C.c_int64, C.c_int64, _vp, _vp, _vp, _vp]),
+    "acx_act8_pack": (C.c_int, [_vp, C.c_int64, C.c_int, C.c_int64, C.c_int64, _vp, _vp, _vp]),
+    "acx_act8_unpack": (C.c_int, [_vp, _vp, C.c_int64, C.c_int64, _vp, C.c_int, _vp]),
+    "acx_act8_workspace_bytes": (C.c_int64, [C.c_int64] * 3),
+    "acx_act8_weight_grad": (C.c_int, [_vp, C.c_int64, C.c_int, _vp, _vp] + [C.c_int64] * 3 + [_vp, _vp, _vp, C.c_int64, _vp]),
     "acx_search_minima_enable": (C.c_int, [C.c_int]),
     "acx_search_last_minima": (C.c_int, [_i32p, C.c_int64, _i64p]),
     "acx_search_digest_enable": (C.c_int, [C.c_int]),

@@ -1,0 +1,403 @@
+// acx_act8.hip -- activations kept in 8 bits for the backward pass, and the weight gradient that reads them.
+//
+//   checkpoint of x [M, K]:  blocks of 32 features of a row share a power of two 2^e, the smallest for which the block's largest magnitude
+//   rounds to at most 127 (never below 2^-126);  q = rint(x 2^-e) as int8, ties to even;  e + 127 as one byte.  1.03 bytes a value.
+//   weight gradient:  dW [O, I] = sum over m of dy[m, o] (q[m, i] 2^e[m, i / 32]),   db[o] = sum over m of dy[m, o]
+//
+// A power of two as the scale makes q 2^e EXACT in bfloat16 (7 bits of magnitude, bfloat16's own exponent range): the product runs on the bf16
+// matrix instructions without rounding the checkpoint again.  dy is brought there without rounding either: a float32 is the sum of three
+// bfloat16 (8 + 8 + 8 bits, each the truncated rest of the last), a float16 of two, a bfloat16 of one; the accumulators are float32.  So dW has
+// the accuracy of a float32 product, at one to three times the matrix work of a bf16 one and 1 byte instead of 4 read per x.
+// A block with an infinity or a NaN is marked with the exponent byte 255 and restores to NaN: it is not hidden.
+#include <type_traits>
+
+#include "acx_elem.h"
+
+namespace acx {
+namespace act8 {
+using namespace elem;
+
+constexpr int kBlock = 32;
+
+__device__ __forceinline__ float exponent_factor(uint32_t e) { return __builtin_bit_cast(float, e == 255 ? 0x7FC00000u : e << 23); }
+
+template <int N> struct Bytes;
+template <> struct Bytes<4> {
+    typedef uint32_t type __attribute__((aligned(1)));
+};
+template <> struct Bytes<8> {
+    typedef uint64_t type __attribute__((aligned(1)));
+};
+
+// V features a lane, 32 / V lanes a block
+template <class E, int V> __global__ void __launch_bounds__(256) k_pack8(const E* __restrict__ x, int64_t x_sn, int64_t M, int K, int lpr, int8_t* __restrict__ q, uint8_t* __restrict__ exps) {
+    const int64_t l = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    const int64_t row = l / lpr;
+    const int j = (int)(l - row * lpr), d = j * V, valid = row < M ? K - d : 0;
+    float v[V];
+    load_some<E, V>(x + row * x_sn + d, valid, v);
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < V; i++) {
+        const uint32_t b = __builtin_bit_cast(uint32_t, v[i]) & 0x7FFFFFFFu;
+        top = b > top ? b : top;  // (as bits: an infinity is above every number, a NaN above that)
+    }
+#pragma unroll
+    for (int m = 1; m < kBlock / V; m *= 2) {
+        const uint32_t o = __shfl_xor((int)top, m);
+        top = o > top ? o : top;
+    }
+    // the exponent field, one more where the mantissa is 1.9921875 or above (it would round to 128), minus 6
+    const int field = (int)((top + 0x10000u) >> 23) - 6;
+    const uint32_t e = top >= 0x7F800000u ? 255u : field < 1 ? 1u : (uint32_t)field;
+    const float inv = e == 255 ? 0.0f : __builtin_bit_cast(float, (254u - e) << 23);
+    uint64_t bytes = 0;
+#pragma unroll
+    for (int i = 0; i < V; i++) {
+        const int n = e == 255 ? 0 : (int)__builtin_rintf(v[i] * inv);
+        bytes |= (uint64_t)(uint8_t)n << (8 * i);
+    }
+    int8_t* out = q + row * K + d;
+    if (valid >= V) {
+        *(typename Bytes<V>::type*)out = (typename Bytes<V>::type)bytes;
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; i++)
+            if (i < valid) out[i] = (int8_t)(bytes >> (8 * i));
+    }
+    if (valid > 0 && j % (kBlock / V) == 0) exps[row * ((K + kBlock - 1) / kBlock) + d / kBlock] = (uint8_t)e;
+}
+
+template <class E, int V> __global__ void __launch_bounds__(256) k_unpack8(const int8_t* __restrict__ q, const uint8_t* __restrict__ exps, int64_t M, int K, int lpr, E* __restrict__ out) {
+    const int64_t l = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    const int64_t row = l / lpr;
+    if (row >= M) return;
+    const int j = (int)(l - row * lpr), d = j * V, valid = K - d;
+    const float factor = exponent_factor(exps[row * ((K + kBlock - 1) / kBlock) + d / kBlock]);
+    const int8_t* p = q + row * K + d;
+    float v[V];
+    if (valid >= V) {
+        const uint64_t bytes = *(const typename Bytes<V>::type*)p;
+#pragma unroll
+        for (int i = 0; i < V; i++) v[i] = (float)(int8_t)(bytes >> (8 * i)) * factor;
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; i++) v[i] = i < valid ? (float)p[i] * factor : 0.0f;
+    }
+    store_some<E, V>(out + row * K + d, valid, v);
+}
+
+// ---- weight gradient ----------------------------------------------------------------------------------------------------------------
+// A workgroup owns a TO x TI tile of dW and a share of the rows, kRows at a time: dy and q of these rows go from memory through registers
+// (the next rows' while the current ones are multiplied) into LDS as the 16-byte operands of v_mfma_f32_32x32x16_bf16, 8 rows of one column
+// each.  Columns are stored in the order in which the threads bring them (column c of a vector of V stands at (c % V) TO / V + c / V): a
+// wave's stores and its operand loads are both contiguous, and the order is undone when dW is written.
+constexpr int kRows = 64;
+
+typedef __bf16 frag __attribute__((ext_vector_type(8)));
+typedef float acc16 __attribute__((ext_vector_type(16)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+struct Args {
+    const void* dy;
+    int64_t dy_sn;
+    const int8_t* q;
+    const uint8_t* exps;
+    int64_t M, share;  // rows of a workgroup's share (a multiple of kRows)
+    int O, I, nb;
+    float *dw, *db;    // [shares, O, I], [shares, O] (db nullable)
+};
+
+__device__ __forceinline__ uint32_t bits_of(float v) { return __builtin_bit_cast(uint32_t, v); }
+// the high halves of two floats, side by side
+__device__ __forceinline__ uint32_t high_halves(float lo, float hi) { return __builtin_amdgcn_perm(bits_of(hi), bits_of(lo), 0x07060302u); }
+__device__ __forceinline__ float truncated(float v) { return __builtin_bit_cast(float, bits_of(v) & 0xFFFF0000u); }
+
+template <class E> struct Pieces { static constexpr int n = 3; };
+template <> struct Pieces<bf16_t> { static constexpr int n = 1; };
+template <> struct Pieces<f16_t> { static constexpr int n = 2; };
+
+template <class E, int TO, int TI, int NT> __global__ void __launch_bounds__(NT) k_weight_grad8(const Args p) {
+    constexpr int kP = Pieces<E>::n, VO = sizeof(E) == 4 ? 4 : 4, VI = 4, kChunks = kRows / 8;
+    constexpr int kWaves = NT / 64;
+    constexpr int kWO = TO / 64 < 1 ? 1 : (TO == 256 ? 4 : (NT == 256 ? 2 : 1)), kWI = kWaves / kWO;  // waves over the tile
+    constexpr int kFO = TO / kWO / 32, kFI = TI / kWI / 32;                                           // 32 x 32 products of a wave
+    static_assert(kFO >= 1 && kFI >= 1 && kWO * kWI == kWaves, "tile");
+    constexpr int kItemsA = kChunks * (TO / VO), kItemsB = kChunks * (TI / VI);
+    constexpr int kPerA = (kItemsA + NT - 1) / NT, kPerB = (kItemsB + NT - 1) / NT;
+    extern __shared__ u32x4 s_mem[];
+    u32x4* sA = s_mem;                          // [piece][chunk][TO]
+    u32x4* sB = s_mem + kP * kChunks * TO;      // [chunk][TI]
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int o0 = blockIdx.x * TO, i0 = blockIdx.y * TI;
+    const int64_t begin = (int64_t)blockIdx.z * p.share, end = begin + p.share < p.M ? begin + p.share : p.M;
+    float a[kPerA][8][VO];
+    uint32_t b[kPerB][8], be[kPerB][8];
+    float bias[kPerA][VO] = {};
+    auto fetch = [&](int64_t m0) {
+#pragma unroll
+        for (int k = 0; k < kPerA; k++) {
+            const int item = tid + k * NT, chunk = item / (TO / VO), o = o0 + item % (TO / VO) * VO;
+            const bool on = item < kItemsA;
+#pragma unroll
+            for (int r = 0; r < 8; r++) {
+                const int64_t m = m0 + chunk * 8 + r;
+                load_some<E, VO>((const E*)p.dy + m * p.dy_sn + o, on && m < end ? p.O - o : 0, a[k][r]);
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < kPerB; k++) {
+            const int item = tid + k * NT, chunk = item / (TI / VI), i = i0 + item % (TI / VI) * VI;
+            const bool on = item < kItemsB;
+#pragma unroll
+            for (int r = 0; r < 8; r++) {
+                const int64_t m = m0 + chunk * 8 + r;
+                const int valid = on && m < end ? p.I - i : 0;
+                const int8_t* src = p.q + m * p.I + i;
+                b[k][r] = 0;
+                if (valid >= VI) {
+                    b[k][r] = *(const typename Bytes<4>::type*)src;
+                } else {
+#pragma unroll
+                    for (int v = 0; v < VI; v++)
+                        if (v < valid) b[k][r] |= (uint32_t)(uint8_t)src[v] << (8 * v);
+                }
+                be[k][r] = valid > 0 ? p.exps[m * p.nb + i / kBlock] : 0;
+            }
+        }
+    };
+    auto stage = [&]() {
+#pragma unroll
+        for (int k = 0; k < kPerA; k++) {
+            const int item = tid + k * NT, chunk = item / (TO / VO), g = item % (TO / VO);
+            if (item < kItemsA) {
+#pragma unroll
+                for (int v = 0; v < VO; v++) {
+#pragma unroll
+                    for (int r = 0; r < 8; r++) bias[k][v] += a[k][r][v];
+#pragma unroll
+                    for (int piece = 0; piece < kP; piece++) {
+                        u32x4 w;
+#pragma unroll
+                        for (int r = 0; r < 4; r++) {
+                            float &lo = a[k][2 * r][v], &hi = a[k][2 * r + 1][v];
+                            w[r] = high_halves(lo, hi);
+                            if (piece + 1 < kP) {  // (an infinity is its own first piece: nothing is left)
+                                const float tl = truncated(lo), th = truncated(hi);
+                                lo = tl == lo ? 0.0f : lo - tl;
+                                hi = th == hi ? 0.0f : hi - th;
+                            }
+                        }
+                        sA[(piece * kChunks + chunk) * TO + v * (TO / VO) + g] = w;
+                    }
+                }
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < kPerB; k++) {
+            const int item = tid + k * NT, chunk = item / (TI / VI), g = item % (TI / VI);
+            if (item < kItemsB) {
+                float f[8];
+#pragma unroll
+                for (int r = 0; r < 8; r++) f[r] = exponent_factor(be[k][r]);
+#pragma unroll
+                for (int v = 0; v < VI; v++) {
+                    u32x4 w;
+#pragma unroll
+                    for (int r = 0; r < 4; r++)
+                        w[r] = high_halves((float)(int8_t)(b[k][2 * r] >> (8 * v)) * f[2 * r], (float)(int8_t)(b[k][2 * r + 1] >> (8 * v)) * f[2 * r + 1]);
+                    sB[chunk * TI + v * (TI / VI) + g] = w;
+                }
+            }
+        }
+    };
+    const int wo = wave % kWO, wi = wave / kWO;
+    acc16 acc[kFO][kFI];
+#pragma unroll
+    for (int x = 0; x < kFO; x++)
+#pragma unroll
+        for (int y = 0; y < kFI; y++)
+#pragma unroll
+            for (int r = 0; r < 16; r++) acc[x][y][r] = 0.0f;
+    fetch(begin);
+    for (int64_t m0 = begin; m0 < end; m0 += kRows) {
+        __syncthreads();  // (the operands of the last rows have been read)
+        stage();
+        __syncthreads();
+        if (m0 + kRows < end) fetch(m0 + kRows);
+#pragma unroll
+        for (int ks = 0; ks < kRows / 16; ks++) {
+            const int chunk = 2 * ks + (lane >> 5), col = lane & 31;
+            frag fb[kFI];
+#pragma unroll
+            for (int y = 0; y < kFI; y++) fb[y] = __builtin_bit_cast(frag, sB[chunk * TI + (wi * kFI + y) * 32 + col]);
+#pragma unroll
+            for (int piece = kP - 1; piece >= 0; piece--) {
+#pragma unroll
+                for (int x = 0; x < kFO; x++) {
+                    const frag fa = __builtin_bit_cast(frag, sA[(piece * kChunks + chunk) * TO + (wo * kFO + x) * 32 + col]);
+#pragma unroll
+                    for (int y = 0; y < kFI; y++) acc[x][y] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fa, fb[y], acc[x][y], 0, 0, 0);
+                }
+            }
+        }
+    }
+    float* dw = p.dw + (int64_t)blockIdx.z * p.O * p.I;
+#pragma unroll
+    for (int x = 0; x < kFO; x++)
+#pragma unroll
+        for (int y = 0; y < kFI; y++) {
+            const int ui = (wi * kFI + y) * 32 + (lane & 31), i = i0 + ui % (TI / VI) * VI + ui / (TI / VI);
+#pragma unroll
+            for (int r = 0; r < 16; r++) {
+                const int uo = (wo * kFO + x) * 32 + (r & 3) + 8 * (r >> 2) + 4 * (lane >> 5), o = o0 + uo % (TO / VO) * VO + uo / (TO / VO);
+                if (o < p.O && i < p.I) dw[(int64_t)o * p.I + i] = acc[x][y][r];
+            }
+        }
+    if (p.db && blockIdx.y == 0) {
+        float* s = (float*)s_mem;  // [chunk][TO]
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < kPerA; k++) {
+            const int item = tid + k * NT, chunk = item / (TO / VO), g = item % (TO / VO);
+            if (item < kItemsA) {
+#pragma unroll
+                for (int v = 0; v < VO; v++) s[chunk * TO + g * VO + v] = bias[k][v];
+            }
+        }
+        __syncthreads();
+        for (int o = tid; o < TO && o0 + o < p.O; o += NT) {
+            float v = 0.0f;
+#pragma unroll
+            for (int c = 0; c < kChunks; c++) v += s[c * TO + o];
+            p.db[(int64_t)blockIdx.z * p.O + o0 + o] = v;
+        }
+    }
+}
+
+// out[c] = sum over the shares, in their order; dW and db in one launch
+__global__ void __launch_bounds__(256) k_join_shares(const float* __restrict__ dw, const float* __restrict__ db, int n, int64_t size, int O, float* __restrict__ out, float* __restrict__ out_db) {
+    const int64_t c = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    const bool bias = c >= size;
+    if (c >= size + (db ? O : 0)) return;
+    const float* src = bias ? db + (c - size) : dw + c;
+    const int64_t step = bias ? O : size;
+    float a[8] = {};
+    int k = 0;
+    for (; k + 8 <= n; k += 8) {
+#pragma unroll
+        for (int i = 0; i < 8; i++) a[i] += src[(k + i) * step];
+    }
+    for (; k < n; k++) a[k & 7] += src[k * step];
+    const float v = ((a[0] + a[1]) + (a[2] + a[3])) + ((a[4] + a[5]) + (a[6] + a[7]));
+    if (bias) out_db[c - size] = v;
+    else out[c] = v;
+}
+
+struct Plan {
+    int to, ti;
+    int64_t go, gi, shares, share;
+};
+static Plan plan_of(int64_t M, int64_t O, int64_t I) {
+    Plan p;
+    p.to = O <= 64 ? 64 : 256;
+    p.ti = I <= 64 ? 64 : 256;
+    p.go = (O + p.to - 1) / p.to;
+    p.gi = (I + p.ti - 1) / p.ti;
+    int64_t want = 256 / (p.go * p.gi);
+    if (want < 1) want = 1;
+    const int64_t steps = (M + kRows - 1) / kRows;
+    const int64_t per = (steps + want - 1) / want;
+    p.share = (per < 4 ? 4 : per) * kRows;
+    p.shares = (M + p.share - 1) / p.share;
+    return p;
+}
+static int64_t work_floats(const Plan& p, int64_t O, int64_t I) { return p.shares > 1 ? p.shares * O * (I + 1) : 0; }
+
+template <class E, int TO, int TI, int NT> static hipError_t launch(const Args& a, const Plan& p, hipStream_t st) {
+    const size_t lds = (size_t)(Pieces<E>::n * TO + TI) * (kRows / 8) * 16;
+    const hipError_t e = hipFuncSetAttribute((const void*)k_weight_grad8<E, TO, TI, NT>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+    if (e != hipSuccess) return e;
+    hipLaunchKernelGGL((k_weight_grad8<E, TO, TI, NT>), dim3((unsigned)p.go, (unsigned)p.gi, (unsigned)p.shares), dim3(NT), lds, st, a);
+    return hipGetLastError();
+}
+
+static int check_rows(int64_t M, int64_t K, int dtype, const char* who) {
+    if (dtype != ACX_F32 && dtype != ACX_BF16 && dtype != ACX_F16) return fail(ACX_E_INVAL, "%s: activations are ACX_F32, ACX_BF16 or ACX_F16", who);
+    if (M < 0 || K < 0 || K > (1 << 20) || M > ((int64_t)1 << 38)) return fail(ACX_E_INVAL, "%s: bad sizes", who);
+    return ACX_OK;
+}
+
+}  // namespace act8
+}  // namespace acx
+
+using namespace acx;
+
+extern "C" int acx_act8_pack(const void* d_x, int64_t x_row, int dtype, int64_t M, int64_t K, int8_t* d_q, uint8_t* d_exponent, void* stream) {
+    if (!have_device()) return ACX_E_NODEVICE;
+    const int rc = act8::check_rows(M, K, dtype, "acx_act8_pack");
+    if (rc) return rc;
+    if (M == 0 || K == 0) return ACX_OK;
+    if (!d_x || !d_q || !d_exponent) return fail(ACX_E_INVAL, "acx_act8_pack: null pointer");
+    const int64_t nb = (K + act8::kBlock - 1) / act8::kBlock, lpr = nb * (dtype == ACX_F32 ? 8 : 4), grid = (M * lpr + 255) / 256;
+    if (grid >= ((int64_t)1 << 31)) return fail(ACX_E_INVAL, "acx_act8_pack: too many values");
+    elem::with_element(dtype, [&](auto* e) {
+        using E = std::remove_pointer_t<decltype(e)>;
+        hipLaunchKernelGGL((act8::k_pack8<E, sizeof(E) == 4 ? 4 : 8>), dim3((unsigned)grid), dim3(256), 0, (hipStream_t)stream, (const E*)d_x, x_row, M, (int)K, (int)lpr, d_q, d_exponent);
+    });
+    ACX_HIP_TRY(hipGetLastError());
+    return ACX_OK;
+}
+extern "C" int acx_act8_unpack(const int8_t* d_q, const uint8_t* d_exponent, int64_t M, int64_t K, void* d_x, int dtype, void* stream) {
+    if (!have_device()) return ACX_E_NODEVICE;
+    const int rc = act8::check_rows(M, K, dtype, "acx_act8_unpack");
+    if (rc) return rc;
+    if (M == 0 || K == 0) return ACX_OK;
+    if (!d_x || !d_q || !d_exponent) return fail(ACX_E_INVAL, "acx_act8_unpack: null pointer");
+    const int v = dtype == ACX_F32 ? 4 : 8;
+    const int64_t lpr = (K + v - 1) / v, grid = (M * lpr + 255) / 256;
+    if (grid >= ((int64_t)1 << 31)) return fail(ACX_E_INVAL, "acx_act8_unpack: too many values");
+    elem::with_element(dtype, [&](auto* e) {
+        using E = std::remove_pointer_t<decltype(e)>;
+        hipLaunchKernelGGL((act8::k_unpack8<E, sizeof(E) == 4 ? 4 : 8>), dim3((unsigned)grid), dim3(256), 0, (hipStream_t)stream, d_q, d_exponent, M, (int)K, (int)lpr, (E*)d_x);
+    });
+    ACX_HIP_TRY(hipGetLastError());
+    return ACX_OK;
+}
+extern "C" int64_t acx_act8_workspace_bytes(int64_t M, int64_t O, int64_t I) {
+    if (M <= 0 || O <= 0 || I <= 0) return 0;
+    return act8::work_floats(act8::plan_of(M, O, I), O, I) * 4;
+}
+extern "C" int acx_act8_weight_grad(const void* d_out_grad, int64_t o_row, int dtype, const int8_t* d_q, const uint8_t* d_exponent, int64_t M, int64_t O, int64_t I, float* d_weight_grad,
+                                    float* d_bias_grad, void* d_work, int64_t work_bytes, void* stream) {
+    if (!have_device()) return ACX_E_NODEVICE;
+    int rc = act8::check_rows(M, O, dtype, "acx_act8_weight_grad");
+    if (!rc) rc = act8::check_rows(M, I, dtype, "acx_act8_weight_grad");
+    if (rc) return rc;
+    if (O == 0 || I == 0 || M == 0) return fail(ACX_E_INVAL, "acx_act8_weight_grad: no rows, outputs or inputs");
+    if (O > (1 << 16) || I > (1 << 16)) return fail(ACX_E_INVAL, "acx_act8_weight_grad: up to 65536 outputs and inputs");
+    if (!d_out_grad || !d_q || !d_exponent || !d_weight_grad) return fail(ACX_E_INVAL, "acx_act8_weight_grad: null pointer");
+    const act8::Plan p = act8::plan_of(M, O, I);
+    const int64_t need = act8::work_floats(p, O, I) * 4;
+    if (need && (!d_work || work_bytes < need)) return fail(ACX_E_CAPACITY, "acx_act8_weight_grad: a workspace of %lld bytes is needed (acx_act8_workspace_bytes)", (long long)need);
+    act8::Args a = {};
+    a.dy = d_out_grad, a.dy_sn = o_row, a.q = d_q, a.exps = d_exponent, a.M = M, a.share = p.share, a.O = (int)O, a.I = (int)I, a.nb = (int)((I + act8::kBlock - 1) / act8::kBlock);
+    a.dw = need ? (float*)d_work : d_weight_grad;
+    a.db = !d_bias_grad ? nullptr : need ? (float*)d_work + p.shares * O * I : d_bias_grad;
+    hipError_t err = hipSuccess;
+    elem::with_element(dtype, [&](auto* e) {
+        using E = std::remove_pointer_t<decltype(e)>;
+        const hipStream_t st = (hipStream_t)stream;
+        if (p.to == 64 && p.ti == 64) err = act8::launch<E, 64, 64, 256>(a, p, st);
+        else if (p.to == 64) err = act8::launch<E, 64, 256, 512>(a, p, st);
+        else if (p.ti == 64) err = act8::launch<E, 256, 64, 512>(a, p, st);
+        else err = act8::launch<E, 256, 256, 512>(a, p, st);
+    });
+    ACX_HIP_TRY(err);
+    if (need) {
+        const int64_t columns = O * I + (d_bias_grad ? O : 0);
+        hipLaunchKernelGGL(act8::k_join_shares, dim3((unsigned)((columns + 255) / 256)), dim3(256), 0, (hipStream_t)stream, a.dw, a.db, (int)p.shares, O * I, (int)O, d_weight_grad, d_bias_grad);
+        ACX_HIP_TRY(hipGetLastError());
+    }
+    return ACX_OK;
+}

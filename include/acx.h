@@ -390,6 +390,18 @@ int acx_block_step(const void *d_x, int64_t x_row, const void *d_projected, int6
                    const float *d_state, const float *d_weight, const float *d_scale, const float *d_next_weight, float eps, int64_t M,
                    int64_t D, float *d_next_state, void *d_new, void *d_u, void *stream);
 
+/* ---- activations kept in 8 bits (csrc/acx_act8.hip) -----------------------------------------------------------------------------
+ * A checkpoint of M rows of K values: int8 q [M, K] and one exponent byte per 32 neighbouring values of a row [M, ceil(K / 32)]; the
+ * value it stands for is q * 2^(exponent - 127).  The exponent is the smallest for which the block's largest magnitude rounds to at most
+ * 127 (at least 1); 255 marks a block that held an infinity or a NaN, and stands for NaN.  x has a stride between rows in elements.
+ * acx_act8_weight_grad: d_weight_grad [O, I] = d_out_grad^T (q 2^e) and d_bias_grad [O] (nullable) = column sums of d_out_grad, float32, for
+ * d_out_grad [M, O] of type dtype; M, O, I >= 1, O and I <= 65536; d_work: acx_act8_workspace_bytes for the duration of the call's kernels. */
+int acx_act8_pack(const void *d_x, int64_t x_row, int dtype, int64_t M, int64_t K, int8_t *d_q, uint8_t *d_exponent, void *stream);
+int acx_act8_unpack(const int8_t *d_q, const uint8_t *d_exponent, int64_t M, int64_t K, void *d_x, int dtype, void *stream);
+int64_t acx_act8_workspace_bytes(int64_t M, int64_t O, int64_t I);
+int acx_act8_weight_grad(const void *d_out_grad, int64_t o_row, int dtype, const int8_t *d_q, const uint8_t *d_exponent, int64_t M,
+                         int64_t O, int64_t I, float *d_weight_grad, float *d_bias_grad, void *d_work, int64_t work_bytes, void *stream);
+
 /* ---- neighbourhood sizes ------------------------------------------------------------
  * Replaces `neibourhood` of the reference's C++ side program (barcode_analysis/5_steps_neibourhoods/neibourhoods.cpp:18-54,
  * moves and word arithmetic AC_UTILS_no_hash.cpp:83-211): number of distinct SORTED pairs of freely reduced relators

@@ -1,0 +1,242 @@
+"""pack8 / unpack8 / weight_grad8 / linear8 / checkpoint8 (csrc/acx_act8.hip): the format bit by bit against its definition, the weight
+gradient against a float64 product of the values that the checkpoint stands for."""
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+DTYPES = ("float32", "bfloat16", "float16")
+
+
+def definition(x):
+    """q, exponent by the definition, in float64 on the host"""
+    import numpy as np
+
+    x = x.detach().double().cpu().numpy()
+    M, K = x.shape
+    q, e = np.zeros((M, K), np.int8), np.zeros((M, -(-K // 32)), np.uint8)
+    for b in range(e.shape[1]):
+        part = x[:, 32 * b:32 * b + 32]
+        top = np.abs(part).max(1)
+        ok = np.isfinite(top)
+        n = np.full(M, -126)
+        for _ in range(300):  # (the smallest exponent, found by trying)
+            with np.errstate(all="ignore"):
+                n = np.where(ok & (np.rint(top * 2.0 ** -n) > 127), n + 1, n)
+        e[:, b] = np.where(ok, n + 127, 255)
+        with np.errstate(all="ignore"):
+            q[:, 32 * b:32 * b + 32] = np.where(ok[:, None], np.rint(part * 2.0 ** -n[:, None].astype(float)), 0)
+    return q, e
+
+
+def values(M, K, dtype, seed):
+    import torch
+
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    x = torch.randn((M, K), device="cuda", generator=g) * torch.exp(3 * torch.randn((M, 1), device="cuda", generator=g))
+    return x.to(getattr(torch, dtype))
+
+
+def check_format(x):
+    import numpy as np
+    import torch
+
+    from ac_solver.agents.activation8 import pack8, unpack8
+
+    q, e = pack8(x)
+    wq, we = definition(x)
+    assert np.array_equal(e.cpu().numpy(), we) and np.array_equal(q.cpu().numpy(), wq)
+    factor = np.repeat(np.where(we == 255, np.nan, 2.0 ** (we.astype(float) - 127)), 32, axis=1)[:, :wq.shape[1]]
+    for dt in DTYPES:
+        back = unpack8(q, e, getattr(torch, dt))
+        want = torch.from_numpy(wq.astype(float) * factor).to(getattr(torch, dt)) if dt != "float16" else torch.from_numpy((wq * factor).astype(np.float32)).to(torch.float16)
+        assert torch.equal(torch.nan_to_num(back.cpu(), 7.0), torch.nan_to_num(want, 7.0)), dt
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("K", [1, 2, 3, 4, 5, 7, 8, 9, 31, 32, 33, 50, 64, 72, 255, 256, 1031])
+def test_format(K, dtype):
+    print(K, dtype, flush=True)
+    check_format(values(37, K, dtype, K))
+
+
+def test_format_at_the_edges():
+    """the magnitudes where the exponent changes, ties, zeros, subnormals, the largest number, infinities and NaNs"""
+    import torch
+
+    f = lambda *v: torch.tensor([list(v) + [0.0] * (32 - len(v))], device="cuda")  # noqa: E731
+    tops = [127.0, 127.49999, 127.5, 127.50001, 128.0, 63.5, 63.75, 1.9921875, 1.9921874, 1.0, 0.99999994, 2.0 ** -120 * 1.5, 2.0 ** -126, 1e-40, 1e-45, 0.0, 3.4028235e38, 3.38e38,
+            float("inf"), -float("inf"), float("nan")]
+    check_format(torch.cat([f(t, 0.5, 1.5, 2.5, -0.5, -1.5, -t / 3 if t == t and abs(t) < 1e39 else 1.0) for t in tops]))
+    check_format(torch.cat([-f(t, t / 254, -t / 254, t * 3 / 254) for t in tops[:18]]))
+    check_format(torch.tensor([[1.0] * 40, [float("inf")] + [1.0] * 39, [1.0] * 39 + [float("nan")]], device="cuda"))  # the other block of a row is not touched
+    check_format(torch.tensor([[65504.0, 1.0, 6e-8]], device="cuda", dtype=torch.float16))
+
+
+def test_strides_axes_and_nothing():
+    import torch
+
+    from ac_solver.agents.activation8 import pack8, unpack8
+
+    x = values(24, 50, "float32", 1)
+    wide = torch.zeros((24, 61), device="cuda")
+    wide[:, 7:57] = x
+    for a, b in ((wide[:, 7:57], x), (x.view(2, 3, 4, 50), x), (x.t().contiguous().t(), x)):
+        q, e = pack8(a)
+        assert q.shape == a.shape and torch.equal(q.view(24, 50), pack8(b)[0]) and torch.equal(e.view(24, 2), pack8(b)[1])
+    q, e = pack8(x[:0])
+    assert q.shape == (0, 50) and e.shape == (0, 2) and unpack8(q, e).shape == (0, 50)
+
+
+def check_weight_grad(M, O, I, dtype, seed=0, strided=False):
+    """Tolerance: a product of values that are exact in the matrix instruction, added up in float32: every one of the additions rounds by at
+    most 2^-24 of the running sum, which is at most the sum of the magnitudes of what has been added; M terms pass through at most M
+    additions, and the errors of these are independent in sign -- 8 sqrt(M) of them bounds what M can do with certainty for all practical
+    purposes, never more than M.  Plus the joins (<= 300 additions)."""
+    import torch
+
+    from ac_solver.agents.activation8 import pack8, unpack8, weight_grad8
+
+    print(f"M {M} O {O} I {I} {dtype} strided {strided}", flush=True)
+    x = values(M, I, "float32", seed)
+    q, e = pack8(x)
+    g = torch.Generator(device="cuda").manual_seed(seed + 1)
+    dy = (torch.randn((M, O), device="cuda", generator=g) * torch.exp(torch.randn((M, 1), device="cuda", generator=g))).to(getattr(torch, dtype))
+    if strided:
+        wide = torch.zeros((M, O + 3), device="cuda", dtype=dy.dtype)
+        wide[:, 1:O + 1] = dy
+        dy = wide[:, 1:O + 1]
+    dw, db = weight_grad8(dy, q, e)
+    xd, yd = unpack8(q, e).double(), dy.double()
+    want, mag = yd.t() @ xd, yd.abs().t() @ xd.abs()
+    adds = min(M, 8 * M ** 0.5) + 16
+    assert dw.dtype == torch.float32 and dw.shape == (O, I) and db.shape == (O,)
+    err, lim = (dw.double() - want).abs(), adds * 2.0 ** -24 * mag + 1e-37
+    assert not bool((err > lim).any()), f"d weight: worst {float((err - lim).max())} beyond the tolerance"
+    err, lim = (db.double() - yd.sum(0)).abs(), adds * 2.0 ** -24 * yd.abs().sum(0) + 1e-37
+    assert not bool((err > lim).any()), f"d bias: worst {float((err - lim).max())} beyond the tolerance"
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("O,I", [(1, 1), (12, 256), (1, 256), (64, 64), (65, 63), (64, 65), (50, 72), (256, 72), (255, 257), (257, 255), (768, 256), (130, 1031), (3, 33)])
+def test_weight_grad_sizes(O, I, dtype):
+    check_weight_grad(777, O, I, dtype)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("M", [1, 2, 7, 8, 9, 63, 64, 65, 255, 256, 257, 4097, 70001])
+def test_weight_grad_rows(M, dtype):
+    check_weight_grad(M, 72, 50, dtype, seed=M)
+    check_weight_grad(M, 300, 260, dtype, seed=M, strided=True)
+
+
+def test_weight_grad_of_every_single_place():
+    """one non-zero value of dy against one of x lands in its own place of dW, for places over the whole tile"""
+    import torch
+
+    from ac_solver.agents.activation8 import pack8, weight_grad8
+
+    for O, I in ((300, 300), (40, 300), (300, 40), (40, 40)):
+        M = max(O, I)
+        dy, x = torch.zeros(M, O, device="cuda"), torch.zeros(M, I, device="cuda")
+        n = min(O, I)
+        k = torch.arange(n, device="cuda")
+        o, i = (k * 7 + 3) % O, (k * 11 + 5) % I
+        dy[k, o] = (k + 1).float() * 1.0009765625
+        x[k, i] = 2.0
+        want = torch.zeros(O, I, device="cuda")
+        want.index_put_((o, i), (k + 1).float() * 2 * 1.0009765625, accumulate=True)
+        assert torch.equal(weight_grad8(dy, *pack8(x))[0], want)
+
+
+def test_weight_grad_shows_infinities_and_nans():
+    """they reach the outputs that their row and column reach, and no others"""
+    import torch
+
+    from ac_solver.agents.activation8 import pack8, weight_grad8
+
+    for dtype in DTYPES:
+        x, dy = values(100, 96, "float32", 3).clamp(-100, 100), values(100, 70, dtype, 4).clamp(-100, 100)
+        x[:, 5] = 1.0
+        dy[7, 9] = float("inf")
+        x[50, 40] = float("nan")
+        dw, db = weight_grad8(dy, *pack8(x))
+        assert torch.isnan(dw[:, 32:64]).all() and float(dw[9, 5]) == float("inf") and float(db[9]) == float("inf")
+        rest = torch.ones(70, 96, dtype=torch.bool, device="cuda")
+        rest[:, 32:64] = False
+        rest[9] = False
+        assert torch.isfinite(dw[rest]).all() and torch.isfinite(torch.cat((db[:9], db[10:]))).all()
+
+
+def test_linear8_and_its_gradients():
+    import torch
+
+    from ac_solver.agents.activation8 import linear8, pack8, unpack8
+
+    for dtype in DTYPES:
+        dt = getattr(torch, dtype)
+        x = values(500, 72, "float32", 2).clamp(-4, 4).to(dt).view(5, 100, 72).requires_grad_()
+        w = (torch.randn(33, 72, device="cuda") * 0.1).requires_grad_()
+        b = torch.randn(33, device="cuda").requires_grad_()
+        out = linear8(x, w, b)
+        assert torch.equal(out, torch.nn.functional.linear(x, w.to(dt), b.to(dt)))
+        d = torch.randn(5, 100, 33, device="cuda").to(dt)
+        dx, dw, db = torch.autograd.grad(out, (x, w, b), d)
+        assert dx.dtype == dt and torch.equal(dx, d @ w.to(dt))
+        kept = unpack8(*pack8(x)).double().view(-1, 72)
+        d2 = d.double().view(-1, 33)
+        assert bool(((dw.double() - d2.t() @ kept).abs() <= 500 * 2.0 ** -24 * (d2.abs().t() @ kept.abs())).all())
+        assert bool(((db.double() - d2.sum(0)).abs() <= 500 * 2.0 ** -24 * d2.abs().sum(0)).all())
+        with torch.no_grad():
+            assert not linear8(x, w, b).requires_grad
+
+
+def test_checkpoint8_restores_what_it_kept():
+    """tanh keeps its output: inside the block the gradient is 1 - y^2 of the restored y, outside that of y itself; a leaf stays exact"""
+    import torch
+
+    from ac_solver.agents.activation8 import checkpoint8, pack8, unpack8
+
+    a = torch.randn(64, 80, device="cuda", requires_grad=True)
+    with checkpoint8():
+        y = torch.tanh(a * 1.0)
+        z = y.square()
+    (g,) = torch.autograd.grad(z, a, torch.ones_like(z))
+    k = unpack8(*pack8(y.detach()))
+    want = 2 * k.double() * (1 - k.double() ** 2)
+    assert float((g.double() - want).abs().max()) < 2.0 ** -20
+    with checkpoint8():
+        out = (a * a).sum()  # (a is a leaf)
+    assert torch.equal(torch.autograd.grad(out, a)[0], 2 * a)
+    with checkpoint8():
+        out = (torch.tanh(a[:4] * 1.0) * 3).sum()  # small: as it is
+    y = torch.tanh(a[:4].detach())
+    assert float((torch.autograd.grad(out, a)[0][:4] - 3 * (1 - y * y)).abs().max()) < 2.0 ** -20
+
+
+def test_repeated_calls_side_streams_and_graph_replays_agree():
+    import torch
+
+    from ac_solver.agents.activation8 import pack8, unpack8, weight_grad8
+
+    x, dy = values(5000, 72, "float32", 1), values(5000, 256, "float32", 2)
+
+    def work():
+        q, e = pack8(x)
+        return (q, e, unpack8(q, e)) + weight_grad8(dy, q, e)
+
+    first = work()
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        again = work()
+    side.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(first, again))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = work()
+    for seed in (3, 5, 7):
+        x.copy_(values(5000, 72, "float32", seed))
+        dy.copy_(values(5000, 256, "float32", seed + 1))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, work()))

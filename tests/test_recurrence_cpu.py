@@ -95,3 +95,35 @@ def test_a_step_refuses_what_it_cannot_read():
         R.recurrent_step(x, p, h, w, reset=torch.zeros(5))
     with pytest.raises(ValueError, match="8192"):
         R.recurrent_step(torch.zeros(1, 8193), torch.zeros(1, 3 * 8193), torch.zeros(1, 8193), torch.zeros(8193))
+
+
+def test_8_bit_checkpoints_refuse_what_they_cannot_read():
+    from ac_solver.agents import activation8 as A
+
+    x, q, e = torch.zeros(5, 40), torch.zeros(5, 40, dtype=torch.int8), torch.zeros(5, 2, dtype=torch.uint8)
+    for call in (lambda: A.pack8(x), lambda: A.unpack8(q, e), lambda: A.weight_grad8(x, q, e), lambda: A.linear8(x, torch.zeros(3, 40), torch.zeros(3))):
+        with pytest.raises(ValueError, match="GPU"):
+            call()
+    with pytest.raises(TypeError, match="float32, bfloat16 or float16"):
+        A.pack8(x.double())
+    with pytest.raises(TypeError, match="q has to be"):
+        A.unpack8(x, e)
+    with pytest.raises(TypeError, match="q has to be a tensor"):
+        A.unpack8(None, e)
+    with pytest.raises(ValueError, match="exponent has the shape"):
+        A.unpack8(q, e[:, :1])
+    with pytest.raises(TypeError, match="dtype"):
+        A.unpack8(q, e, torch.float64)
+    with pytest.raises(ValueError, match="rows in common"):
+        A.weight_grad8(x[:4], q, e)
+    with pytest.raises(TypeError, match="weight"):
+        A.linear8(x, torch.zeros(3, 40).half())
+    with pytest.raises(TypeError, match="bias"):
+        A.linear8(x, torch.zeros(3, 40), torch.zeros(4))
+    with pytest.raises(ValueError, match="weight"):
+        A.linear8(x, torch.zeros(3, 41))
+    with A.checkpoint8():  # nothing on the CPU is packed
+        a = torch.randn(100, 100, requires_grad=True)
+        out = torch.tanh(a * 1.0).sum()
+    out.backward()
+    assert torch.allclose(a.grad, 1 - torch.tanh(a.detach()) ** 2)
