@@ -15,6 +15,7 @@
 // The state is float32 all the way.  The gradient needs h_(t-1) unrounded: the forward pass leaves the state in front of every segment
 // (4 bytes for 16 steps) and the backward pass runs the segment again from it in registers, which also saves it reading h.
 // k_t = 0 SELECTS zero: an infinite or NaN state of the last episode does not reach the next one through 0 * inf.
+#include <initializer_list>
 #include <type_traits>
 
 #include "acx_elem.h"
@@ -49,12 +50,15 @@ struct Affine {
 };
 __device__ __forceinline__ float apply(Affine m, float h) { return m.a < 0.0f ? m.b : __builtin_fmaf(m.a, h, m.b); }
 
+// A lane's place.  The lanes of a wave are neighbours in (row, feature): what differs between them fits 32 bits behind a base that the whole
+// wave shares, so an access takes a scalar pointer that moves with the steps and one register of offset for all of them.  (The last lane of a
+// row that V does not divide steps back and computes a few channels a second time: the same values, stored twice; the lanes behind the last
+// row do its first channels again.)
 struct Lane {
-    int64_t n;
+    int64_t n, n0;  // row; row of the wave's first lane
     int d;
+    __device__ __forceinline__ uint32_t offset(int64_t sn, int bytes) const { return (uint32_t)(((n - n0) * sn + d) * bytes); }
 };
-// (the last lane of a row that V does not divide steps back and computes a few channels a second time: the same values, stored twice;
-// the same for the lanes behind the last row)
 template <int V> __device__ __forceinline__ Lane lane_of(const Args& p) {
     const int64_t l = (int64_t)blockIdx.x * 64 + (threadIdx.x & 63);
     int64_t n = l / p.lpr;
@@ -63,69 +67,116 @@ template <int V> __device__ __forceinline__ Lane lane_of(const Args& p) {
         n = p.N - 1;
         j = 0;
     }
+    const int64_t n0 = (int64_t)blockIdx.x * 64 / p.lpr;
     const int d = j * V;
-    return {n, d + V <= p.D ? d : p.D - V};
+    return {n, n0, d + V <= p.D ? d : p.D - V};
 }
 
 // one segment's operands; steps at or behind `end` read the last step (in bounds) and are made the identity by the caller
-template <class E, int V> __device__ __forceinline__ void load_segment(const void* base, int64_t st, int64_t t0, int64_t end, float (&out)[kSeg][V]) {
-    const E* p = (const E*)base + t0 * st;
+template <class E, int V> __device__ __forceinline__ void load_segment(const void* base, int64_t first, int64_t st, uint32_t offset, int64_t t0, int64_t end, float (&out)[kSeg][V]) {
+    const char* p = (const char*)base + (first + t0 * st) * (int64_t)sizeof(E);  // (scalar)
 #pragma unroll
     for (int k = 0; k < kSeg; k++) {
-        load<E, V>(p, out[k]);
-        if (t0 + k + 1 < end) p += st;  // (uniform)
+        load<E, V>((const E*)(p + offset), out[k]);
+        p += t0 + k + 1 < end ? st * (int64_t)sizeof(E) : 0;
     }
 }
-__device__ __forceinline__ uint32_t load_resets(const Args& p, int64_t n, int64_t t0, int64_t end) {
+__device__ __forceinline__ uint32_t load_resets(const Args& p, const Lane& me, int64_t t0, int64_t end) {
     uint32_t bits = 0;
     if (p.reset) {
-        const uint8_t* r = p.reset + t0 * p.N + n;
+        const uint8_t* r = p.reset + t0 * p.N + me.n0;
+        const uint32_t offset = (uint32_t)(me.n - me.n0);
 #pragma unroll
         for (int k = 0; k < kSeg; k++) {
-            bits |= (uint32_t)(*r != 0) << k;
-            if (t0 + k + 1 < end) r += p.N;
+            bits |= (uint32_t)(r[offset] != 0) << k;
+            r += t0 + k + 1 < end ? p.N : 0;
         }
+        if (end - t0 < kSeg) bits &= (1u << (end - t0)) - 1;
     }
     return bits;
+}
+// `second` behind `first`
+__device__ __forceinline__ Affine join(Affine second, Affine first) {
+    return {second.a < 0.0f || first.a < 0.0f ? -1.0f : second.a * first.a, apply(second, first.b)};
+}
+// The chunks in front of this one (FORWARD; else those behind it), folded into `carry`: every wave composes a few of them, the waves' maps
+// meet in LDS.
+template <int V, int W, bool FORWARD> __device__ __forceinline__ void fold_chunks(const Args& p, int64_t ch, int64_t nd, int lane, int w, Affine (&s_map)[W][64 * V], float (&carry)[V]) {
+    const int n = FORWARD ? (int)blockIdx.y : (int)(gridDim.y - 1 - blockIdx.y), per = (n + W - 1) / W;
+    Affine m[V];
+#pragma unroll
+    for (int i = 0; i < V; i++) m[i] = {1.0f, 0.0f};
+    const int k1 = (w + 1) * per < n ? (w + 1) * per : n;
+    for (int k = w * per; k < k1; k++) {
+        const int q = FORWARD ? k : (int)gridDim.y - 1 - k;
+        float a[V], b[V];
+        load<float, V>(p.agg + (int64_t)q * 2 * nd + ch, a);
+        load<float, V>(p.agg + (int64_t)q * 2 * nd + nd + ch, b);
+#pragma unroll
+        for (int i = 0; i < V; i++) m[i] = join({a[i], b[i]}, m[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < V; i++) s_map[w][i * 64 + lane] = m[i];
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < W; k++)
+#pragma unroll
+        for (int i = 0; i < V; i++) carry[i] = apply(s_map[k][i * 64 + lane], carry[i]);
+    __syncthreads();
+}
+// This wave's place among the maps of a tile: `mine` in LDS, what the waves before it (w0 = 0, step = 1) or behind it (w0 = W - 1, step = -1) do to
+// `carry` into `front`, what all of them do into `carry`.  Two buffers take turns, so one barrier a tile is enough.
+template <int V, int W, bool FORWARD> __device__ __forceinline__ void meet(Affine (&s_map)[W][64 * V], int lane, int w, const Affine (&mine)[V], Affine (&carry)[V], float (&front)[V]) {
+#pragma unroll
+    for (int i = 0; i < V; i++) s_map[w][i * 64 + lane] = mine[i];
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < W; k++) {
+        const int q = FORWARD ? k : W - 1 - k;
+#pragma unroll
+        for (int i = 0; i < V; i++) {
+            front[i] = q == w ? carry[i].b : front[i];
+            carry[i] = join(s_map[q][i * 64 + lane], carry[i]);
+        }
+    }
+}
+
+// The compiler shall compute f and 1 - f again where it needs them next (two instructions) instead of holding both (two registers a value).
+template <int V> __device__ __forceinline__ void forget(float (&s)[kSeg][V]) {
+#pragma unroll
+    for (int k = 0; k < kSeg; k++)
+#pragma unroll
+        for (int i = 0; i < V; i++) asm volatile("" : "+v"(s[k][i]));
 }
 
 // FINAL: write h, last, bounds.  Otherwise only compose the chunk (agg).
 template <class E, int V, int W, bool FINAL> __global__ void __launch_bounds__(64 * W) k_scan_fwd(const Args p) {
     constexpr bool kPrecise = sizeof(E) == 4;
-    __shared__ Affine s_map[W > 1 ? 2 : 1][W][64 * V];
+    __shared__ Affine s_map[2][W][64 * V];
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const Lane me = lane_of<V>(p);
     const int64_t ch = me.n * p.D + me.d, nd = p.N * p.D;
     const int64_t begin = (int64_t)blockIdx.y * p.chunk, end = begin + p.chunk < p.T ? begin + p.chunk : p.T;
-    const E* cp = (const E*)p.c + me.n * p.c_sn + me.d;
-    const E* zp = (const E*)p.z + me.n * p.z_sn + me.d;
-    E* hp = (E*)p.h + ch;
+    const uint32_t c_off = me.offset(p.c_sn, sizeof(E)), z_off = me.offset(p.z_sn, sizeof(E)), h_off = me.offset(p.D, sizeof(E));
     Affine carry[V];  // FINAL: the state (in b); else the chunk so far
 #pragma unroll
     for (int i = 0; i < V; i++) carry[i] = {FINAL ? -1.0f : 1.0f, 0.0f};
     if constexpr (FINAL) {
-        if (p.state) {
+        float h[V] = {};
+        if (p.state) load<float, V>(p.state + ch, h);
+        if (gridDim.y > 1) fold_chunks<V, W, true>(p, ch, nd, lane, w, s_map[1], h);
 #pragma unroll
-            for (int i = 0; i < V; i++) carry[i].b = p.state[ch + i];
-        }
-        for (unsigned q = 0; q < blockIdx.y; q++) {
-            const float* m = p.agg + (int64_t)q * 2 * nd + ch;
-#pragma unroll
-            for (int i = 0; i < V; i++) carry[i].b = apply({m[i], m[nd + i]}, carry[i].b);
-        }
+        for (int i = 0; i < V; i++) carry[i].b = h[i];
     }
-    auto join = [](Affine second, Affine first) -> Affine {
-        return {second.a < 0.0f || first.a < 0.0f ? -1.0f : second.a * first.a, apply(second, first.b)};
-    };
     int buf = 0;
     for (int64_t tile = begin; tile < end; tile += W * kSeg, buf ^= 1) {
         const int64_t t0 = tile + w * kSeg;
         float f[kSeg][V], b[kSeg][V];
         uint32_t resets = 0;
         if (t0 < end) {
-            load_segment<E, V>(zp, p.z_st, t0, end, f);
-            load_segment<E, V>(cp, p.c_st, t0, end, b);
-            resets = load_resets(p, me.n, t0, end);
+            load_segment<E, V>(p.z, me.n0 * p.z_sn, p.z_st, z_off, t0, end, f);
+            load_segment<E, V>(p.c, me.n0 * p.c_sn, p.c_st, c_off, t0, end, b);
+            resets = load_resets(p, me, t0, end);
         }
 #pragma unroll
         for (int k = 0; k < kSeg; k++) {
@@ -136,56 +187,39 @@ template <class E, int V, int W, bool FINAL> __global__ void __launch_bounds__(6
                 f[k][i] = in ? keep_of(z, s) : 1.0f;
                 b[k][i] = in ? take_of(z, s) * b[k][i] : 0.0f;
             }
-            if (!in) resets &= ~(1u << k);
         }
-        Affine at[V];  // what stands in front of this segment
+        float h[V];
 #pragma unroll
-        for (int i = 0; i < V; i++) at[i] = carry[i];
+        for (int i = 0; i < V; i++) h[i] = carry[i].b;
         if constexpr (W > 1 || !FINAL) {
             Affine m[V];
 #pragma unroll
             for (int i = 0; i < V; i++) {
-                float a = 1.0f, h = 0.0f;
+                float a = 1.0f, x = 0.0f;
 #pragma unroll
                 for (int k = 0; k < kSeg; k++) {
-                    const bool r = resets >> k & 1;
                     a *= f[k][i];
-                    h = __builtin_fmaf(f[k][i], r ? 0.0f : h, b[k][i]);
+                    x = __builtin_fmaf(f[k][i], resets >> k & 1 ? 0.0f : x, b[k][i]);
                 }
-                m[i] = {resets ? -1.0f : a, h};
+                m[i] = {resets ? -1.0f : a, x};
             }
             if constexpr (W == 1) {
 #pragma unroll
                 for (int i = 0; i < V; i++) carry[i] = join(m[i], carry[i]);
             } else {
-#pragma unroll
-                for (int i = 0; i < V; i++) s_map[buf][w][i * 64 + lane] = m[i];
-                __syncthreads();  // (two buffers: the next tile's maps go into the other one, so one barrier a tile is enough)
-                for (int q = 0; q < W; q++) {
-#pragma unroll
-                    for (int i = 0; i < V; i++) {
-                        if (q == w) at[i] = carry[i];
-                        carry[i] = join(s_map[buf][q][i * 64 + lane], carry[i]);
-                    }
-                }
+                meet<V, W, true>(s_map[buf], lane, w, m, carry, h);
             }
         }
         if constexpr (FINAL) {
             if (t0 < end) {
-                float h[V];
-#pragma unroll
-                for (int i = 0; i < V; i++) h[i] = at[i].b;
                 if (p.bounds) store<float, V>(p.bounds + (t0 / kSeg) * nd + ch, h);
-                E* out = hp + t0 * nd;
+                char* hp = (char*)p.h + (t0 * nd + me.n0 * p.D) * (int64_t)sizeof(E);
 #pragma unroll
                 for (int k = 0; k < kSeg; k++) {
-                    const bool r = resets >> k & 1;
 #pragma unroll
-                    for (int i = 0; i < V; i++) h[i] = __builtin_fmaf(f[k][i], r ? 0.0f : h[i], b[k][i]);
-                    if (t0 + k < end) {
-                        store<E, V>(out, h);
-                        out += nd;
-                    }
+                    for (int i = 0; i < V; i++) h[i] = __builtin_fmaf(f[k][i], resets >> k & 1 ? 0.0f : h[i], b[k][i]);
+                    if (t0 + k < end) store<E, V>((E*)(hp + h_off), h);
+                    hp += nd * (int64_t)sizeof(E);
                 }
                 if constexpr (W == 1) {
 #pragma unroll
@@ -194,21 +228,15 @@ template <class E, int V, int W, bool FINAL> __global__ void __launch_bounds__(6
             }
         }
     }
-    if constexpr (FINAL) {
-        if (w == 0 && end == p.T) {
-            float h[V];
+    if (w == 0) {
+        float a[V], b[V];
 #pragma unroll
-            for (int i = 0; i < V; i++) h[i] = carry[i].b;
-            store<float, V>(p.last + ch, h);
-        }
-    } else {
-        if (w == 0) {
-            float a[V], b[V];
-#pragma unroll
-            for (int i = 0; i < V; i++) a[i] = carry[i].a, b[i] = carry[i].b;
-            float* m = p.agg + (int64_t)blockIdx.y * 2 * nd + ch;
-            store<float, V>(m, a);
-            store<float, V>(m + nd, b);
+        for (int i = 0; i < V; i++) a[i] = carry[i].a, b[i] = carry[i].b;
+        if constexpr (FINAL) {
+            if (end == p.T) store<float, V>(p.last + ch, b);
+        } else {
+            store<float, V>(p.agg + (int64_t)blockIdx.y * 2 * nd + ch, a);
+            store<float, V>(p.agg + (int64_t)blockIdx.y * 2 * nd + nd + ch, b);
         }
     }
 }
@@ -217,53 +245,41 @@ template <class E, int V, int W, bool FINAL> __global__ void __launch_bounds__(6
 // X_(t-1) = f_t k_t G_t; a segment is the map X -> A X + B of the X behind it to the X in front of it.
 template <class E, int V, int W, bool FINAL> __global__ void __launch_bounds__(64 * W) k_scan_bwd(const Args p) {
     constexpr bool kPrecise = sizeof(E) == 4;
-    __shared__ Affine s_map[W > 1 ? 2 : 1][W][64 * V];
+    __shared__ Affine s_map[2][W][64 * V];
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const Lane me = lane_of<V>(p);
     const int64_t ch = me.n * p.D + me.d, nd = p.N * p.D;
     const int64_t begin = (int64_t)blockIdx.y * p.chunk, end = begin + p.chunk < p.T ? begin + p.chunk : p.T;
-    const E* cp = (const E*)p.c + me.n * p.c_sn + me.d;
-    const E* zp = (const E*)p.z + me.n * p.z_sn + me.d;
-    const E* gp = (const E*)p.dh + me.n * p.dh_sn + me.d;
-    E* dcp = (E*)p.dc + me.n * p.dc_sn + me.d;
-    E* dzp = (E*)p.dz + me.n * p.dz_sn + me.d;
+    const uint32_t c_off = me.offset(p.c_sn, sizeof(E)), z_off = me.offset(p.z_sn, sizeof(E)), g_off = me.offset(p.dh_sn, sizeof(E));
+    const uint32_t dc_off = me.offset(p.dc_sn, sizeof(E)), dz_off = me.offset(p.dz_sn, sizeof(E));
     Affine carry[V];
 #pragma unroll
     for (int i = 0; i < V; i++) carry[i] = {FINAL ? -1.0f : 1.0f, 0.0f};
     if constexpr (FINAL) {
-        if (p.dlast) {
+        float x[V] = {};
+        if (p.dlast) load<float, V>(p.dlast + ch, x);
+        if (gridDim.y > 1) fold_chunks<V, W, false>(p, ch, nd, lane, w, s_map[1], x);
 #pragma unroll
-            for (int i = 0; i < V; i++) carry[i].b = p.dlast[ch + i];
-        }
-        for (unsigned q = gridDim.y - 1; q > blockIdx.y; q--) {
-            const float* m = p.agg + (int64_t)q * 2 * nd + ch;
-#pragma unroll
-            for (int i = 0; i < V; i++) carry[i].b = apply({m[i], m[nd + i]}, carry[i].b);
-        }
+        for (int i = 0; i < V; i++) carry[i].b = x[i];
     }
-    auto join = [](Affine second, Affine first) -> Affine {
-        return {second.a < 0.0f || first.a < 0.0f ? -1.0f : second.a * first.a, apply(second, first.b)};
-    };
+    // small_sigmoid is held with the sign of z: f = s for z < 0, else 1 - s
+    auto fkeep = [](float v) { return __builtin_signbitf(v) ? -v : 1.0f - v; };
+    auto ftake = [](float v) { return __builtin_signbitf(v) ? 1.0f + v : v; };
     int buf = 0;
     const int64_t tiles = (end - begin + W * kSeg - 1) / (W * kSeg);
     for (int64_t tile = begin + (tiles - 1) * (W * kSeg); tile >= begin; tile -= W * kSeg, buf ^= 1) {
         const int64_t t0 = tile + w * kSeg;
-        float s[kSeg][V], diff[kSeg][V], g[kSeg][V];  // +-small_sigmoid (the sign is z's), k h_(t-1) - c, dh
-        uint32_t resets = 0, steps = 0;
+        float s[kSeg][V], diff[kSeg][V], g[kSeg][V];  // diff: c, then k h_(t-1) - c; g: dh
+        uint32_t resets = 0;
         if (t0 < end) {
-            steps = end - t0 < kSeg ? (uint32_t)(end - t0) : kSeg;
-            load_segment<E, V>(zp, p.z_st, t0, end, s);
-            load_segment<E, V>(gp, p.dh_st, t0, end, g);
-            resets = load_resets(p, me.n, t0, end);
-            if constexpr (FINAL) load_segment<E, V>(cp, p.c_st, t0, end, diff);
+            load_segment<E, V>(p.z, me.n0 * p.z_sn, p.z_st, z_off, t0, end, s);
+            if constexpr (FINAL) load_segment<E, V>(p.c, me.n0 * p.c_sn, p.c_st, c_off, t0, end, diff);
+            load_segment<E, V>(p.dh, me.n0 * p.dh_sn, p.dh_st, g_off, t0, end, g);
+            resets = load_resets(p, me, t0, end);
         }
-        if (steps < kSeg) resets &= (1u << steps) - 1;
-        // the sign of s tells which side of zero z was on: f = s for z < 0 (s held as -s), else 1 - s
-        auto fkeep = [](float v) { return __builtin_signbitf(v) ? -v : 1.0f - v; };
-        auto ftake = [](float v) { return __builtin_signbitf(v) ? 1.0f + v : v; };
 #pragma unroll
         for (int k = 0; k < kSeg; k++) {
-            const bool in = (uint32_t)k < steps;
+            const bool in = t0 + k < end;
 #pragma unroll
             for (int i = 0; i < V; i++) {
                 const float z = s[k][i], v = small_sigmoid<kPrecise>(z);
@@ -277,16 +293,16 @@ template <class E, int V, int W, bool FINAL> __global__ void __launch_bounds__(6
                 load<float, V>(p.bounds + (t0 / kSeg) * nd + ch, h);
 #pragma unroll
                 for (int k = 0; k < kSeg; k++) {
-                    const bool r = resets >> k & 1;
 #pragma unroll
                     for (int i = 0; i < V; i++) {
-                        const float c = diff[k][i], before = r ? 0.0f : h[i];
+                        const float c = diff[k][i], before = resets >> k & 1 ? 0.0f : h[i];
                         h[i] = __builtin_fmaf(fkeep(s[k][i]), before, ftake(s[k][i]) * c);
                         diff[k][i] = before - c;
                     }
                 }
             }
         }
+        forget<V>(s);
         float x[V];  // X behind this segment
 #pragma unroll
         for (int i = 0; i < V; i++) x[i] = carry[i].b;
@@ -297,10 +313,9 @@ template <class E, int V, int W, bool FINAL> __global__ void __launch_bounds__(6
                 float a = 1.0f, b = 0.0f;
 #pragma unroll
                 for (int k = kSeg - 1; k >= 0; k--) {
-                    const bool r = resets >> k & 1;
                     const float f = fkeep(s[k][i]);
                     a *= f;
-                    b = r ? 0.0f : f * (g[k][i] + b);
+                    b = resets >> k & 1 ? 0.0f : f * (g[k][i] + b);
                 }
                 m[i] = {resets ? -1.0f : a, b};
             }
@@ -308,35 +323,30 @@ template <class E, int V, int W, bool FINAL> __global__ void __launch_bounds__(6
 #pragma unroll
                 for (int i = 0; i < V; i++) carry[i] = join(m[i], carry[i]);
             } else {
-#pragma unroll
-                for (int i = 0; i < V; i++) s_map[buf][w][i * 64 + lane] = m[i];
-                __syncthreads();
-                for (int q = W - 1; q >= 0; q--) {
-#pragma unroll
-                    for (int i = 0; i < V; i++) {
-                        if (q == w) x[i] = carry[i].b;
-                        carry[i] = join(s_map[buf][q][i * 64 + lane], carry[i]);
-                    }
-                }
+                meet<V, W, false>(s_map[buf], lane, w, m, carry, x);
+                forget<V>(s);
             }
         }
         if constexpr (FINAL) {
             if (t0 < end) {
+                const int64_t dc_st = p.dc_st * (int64_t)sizeof(E), dz_st = p.dz_st * (int64_t)sizeof(E);
+                char* dcp = (char*)p.dc + me.n0 * p.dc_sn * (int64_t)sizeof(E) + (t0 + kSeg - 1) * dc_st;
+                char* dzp = (char*)p.dz + me.n0 * p.dz_sn * (int64_t)sizeof(E) + (t0 + kSeg - 1) * dz_st;
 #pragma unroll
                 for (int k = kSeg - 1; k >= 0; k--) {
-                    const bool r = resets >> k & 1;
-                    float dc[V], dz[V];
+                    if (t0 + k < end) {
+                        float dc[V], dz[V];
 #pragma unroll
-                    for (int i = 0; i < V; i++) {
-                        const float f = fkeep(s[k][i]), u = ftake(s[k][i]), G = g[k][i] + x[i];
-                        dc[i] = u * G;
-                        dz[i] = f * u * diff[k][i] * G;
-                        x[i] = (uint32_t)k < steps ? (r ? 0.0f : f * G) : x[i];
+                        for (int i = 0; i < V; i++) {
+                            const float f = fkeep(s[k][i]), u = ftake(s[k][i]), G = g[k][i] + x[i];
+                            dc[i] = u * G;
+                            dz[i] = f * u * diff[k][i] * G;
+                            x[i] = resets >> k & 1 ? 0.0f : f * G;
+                        }
+                        store<E, V>((E*)(dcp + dc_off), dc);
+                        store<E, V>((E*)(dzp + dz_off), dz);
                     }
-                    if ((uint32_t)k < steps) {
-                        store<E, V>(dcp + (t0 + k) * p.dc_st, dc);
-                        store<E, V>(dzp + (t0 + k) * p.dz_st, dz);
-                    }
+                    dcp -= dc_st, dzp -= dz_st;
                 }
                 if constexpr (W == 1) {
 #pragma unroll
@@ -345,21 +355,15 @@ template <class E, int V, int W, bool FINAL> __global__ void __launch_bounds__(6
             }
         }
     }
-    if constexpr (FINAL) {
-        if (w == 0 && begin == 0 && p.dstate) {
-            float d[V];
+    if (w == 0) {
+        float a[V], b[V];
 #pragma unroll
-            for (int i = 0; i < V; i++) d[i] = carry[i].b;
-            store<float, V>(p.dstate + ch, d);
-        }
-    } else {
-        if (w == 0) {
-            float a[V], b[V];
-#pragma unroll
-            for (int i = 0; i < V; i++) a[i] = carry[i].a, b[i] = carry[i].b;
-            float* m = p.agg + (int64_t)blockIdx.y * 2 * nd + ch;
-            store<float, V>(m, a);
-            store<float, V>(m + nd, b);
+        for (int i = 0; i < V; i++) a[i] = carry[i].a, b[i] = carry[i].b;
+        if constexpr (FINAL) {
+            if (begin == 0 && p.dstate) store<float, V>(p.dstate + ch, b);
+        } else {
+            store<float, V>(p.agg + (int64_t)blockIdx.y * 2 * nd + ch, a);
+            store<float, V>(p.agg + (int64_t)blockIdx.y * 2 * nd + nd + ch, b);
         }
     }
 }
@@ -369,20 +373,21 @@ struct Plan {
     int v, w, lpr;
     int64_t groups, chunk, chunks;
 };
-static Plan plan_of(int64_t T, int64_t N, int64_t D, int dtype) {
+static Plan plan_of(int64_t T, int64_t N, int64_t D) {
     Plan p;
-    p.v = D >= 2 ? 2 : 1;
-    p.lpr = (int)((D + p.v - 1) / p.v);
-    p.groups = (N * p.lpr + 63) / 64;
     const int64_t segments = (T + kSeg - 1) / kSeg;
-    p.w = p.groups >= 2048 || segments == 1 ? 1 : p.groups >= 512 || segments <= 4 ? 4 : 16;
+    auto groups = [&](int v) { return (N * ((D + v - 1) / v) + 63) / 64; };
+    p.v = D >= 2 && groups(2) >= 512 ? 2 : 1;
+    p.lpr = (int)((D + p.v - 1) / p.v);
+    p.groups = groups(p.v);
+    p.w = p.groups >= 2048 || segments == 1 ? 1 : p.v == 2 || segments <= 4 ? 4 : 16;
     p.chunks = 1;
     p.chunk = T;
     const int64_t tile = (int64_t)p.w * kSeg, tiles = (T + tile - 1) / tile;
-    if (p.groups < 128 && tiles >= 16) {
+    if (p.groups < 128 && tiles >= 4) {
         int64_t want = 256 / p.groups;
-        if (want > 64) want = 64;
-        if (want > tiles / 4) want = tiles / 4;
+        if (want > 128) want = 128;
+        if (want > tiles) want = tiles;
         p.chunk = (tiles + want - 1) / want * tile;
         p.chunks = (T + p.chunk - 1) / p.chunk;
     }
@@ -404,10 +409,10 @@ template <class E, int V, int W> static void launch(bool forward, const Args& a,
 template <class E, int V> static void launch_w(bool forward, const Args& a, const Plan& p, hipStream_t st) {
     if (p.w == 1) launch<E, V, 1>(forward, a, p, st);
     else if (p.w == 4) launch<E, V, 4>(forward, a, p, st);
-    else launch<E, V, 16>(forward, a, p, st);
+    else if constexpr (V == 1) launch<E, V, 16>(forward, a, p, st);
 }
 static int run(bool forward, Args& a, int dtype, void* work, int64_t work_bytes, hipStream_t st, const char* who) {
-    const Plan p = plan_of(a.T, a.N, a.D, dtype);
+    const Plan p = plan_of(a.T, a.N, a.D);
     const int64_t need = p.chunks > 1 ? p.chunks * 2 * a.N * a.D * 4 : 0;
     if (work_bytes < need || (need && !work)) return fail(ACX_E_CAPACITY, "%s: a workspace of %lld bytes is needed (acx_scan_workspace_bytes)", who, (long long)need);
     a.agg = (float*)work;
@@ -420,6 +425,13 @@ static int run(bool forward, Args& a, int dtype, void* work, int64_t work_bytes,
     });
     ACX_HIP_TRY(hipGetLastError());
     return ACX_OK;
+}
+// the rows of a wave within 32 bits of offset of each other (see Lane)
+static bool strides_ok(int64_t D, int dtype, std::initializer_list<int64_t> rows) {
+    const int64_t apart = 63 / ((D + 1) / 2) + 1;  // rows that a wave can span
+    for (int64_t r : rows)
+        if (r < 0 || r > (((int64_t)1 << 32) / element_bytes(dtype) - D) / apart) return false;
+    return true;
 }
 static int check_sizes(int64_t T, int64_t N, int64_t D, int dtype, const char* who) {
     if (dtype != ACX_F32 && dtype != ACX_BF16 && dtype != ACX_F16) return fail(ACX_E_INVAL, "%s: activations are ACX_F32, ACX_BF16 or ACX_F16", who);
@@ -439,7 +451,7 @@ extern "C" int64_t acx_scan_bounds_bytes(int64_t T, int64_t N, int64_t D) {
 }
 extern "C" int64_t acx_scan_workspace_bytes(int64_t T, int64_t N, int64_t D, int dtype) {
     if (T <= 0 || N <= 0 || D <= 0) return 0;
-    const scan::Plan p = scan::plan_of(T, N, D, dtype);
+    const scan::Plan p = scan::plan_of(T, N, D);
     return p.chunks > 1 ? p.chunks * 2 * N * D * 4 : 0;
 }
 extern "C" int acx_scan_forward(const void* d_candidate, int64_t c_step, int64_t c_row, const void* d_gate, int64_t z_step, int64_t z_row, int dtype, const uint8_t* d_reset,
@@ -451,6 +463,7 @@ extern "C" int acx_scan_forward(const void* d_candidate, int64_t c_step, int64_t
     if (T == 0) return fail(ACX_E_INVAL, "acx_scan_forward: no steps");
     if (!d_candidate || !d_gate || !d_hidden || !d_last) return fail(ACX_E_INVAL, "acx_scan_forward: null pointer");
     if (d_last == d_state) return fail(ACX_E_INVAL, "acx_scan_forward: the last state does not replace the first in place");
+    if (!scan::strides_ok(D, dtype, {c_row, z_row})) return fail(ACX_E_INVAL, "acx_scan_forward: rows too far apart (4 GiB among the rows of 64 lanes)");
     scan::Args a = {};
     a.c = d_candidate, a.c_st = c_step, a.c_sn = c_row;
     a.z = d_gate, a.z_st = z_step, a.z_sn = z_row;
@@ -468,6 +481,8 @@ extern "C" int acx_scan_backward(const void* d_candidate, int64_t c_step, int64_
     if (N == 0 || D == 0) return ACX_OK;
     if (T == 0) return fail(ACX_E_INVAL, "acx_scan_backward: no steps");
     if (!d_candidate || !d_gate || !d_hidden_grad || !d_bounds || !d_candidate_grad || !d_gate_grad) return fail(ACX_E_INVAL, "acx_scan_backward: null pointer");
+    if (!scan::strides_ok(D, dtype, {c_row, z_row, g_row, dc_row, dz_row}))
+        return fail(ACX_E_INVAL, "acx_scan_backward: rows too far apart (4 GiB among the rows of 64 lanes)");
     scan::Args a = {};
     a.c = d_candidate, a.c_st = c_step, a.c_sn = c_row;
     a.z = d_gate, a.z_st = z_step, a.z_sn = z_row;
