@@ -95,7 +95,7 @@ template <class E, int V, int LR, int R, bool STEP> __global__ void __launch_bou
                 const bool start = live && p.reset && p.reset[row];
 #pragma unroll
                 for (int i = 0; i < V; i++) {
-                    const float s = small_sigmoid<kPrecise>(z[i]);
+                    const Sigmoid s = sigmoid_pair<kPrecise>(z[i]);
                     y[r][i] = __builtin_fmaf(keep_of(z[i], s), start ? 0.0f : h[i], take_of(z[i], s) * c[i]);
                 }
                 store_some<float, V>(p.next_state + row * p.D + d, valid, y[r]);
@@ -122,7 +122,7 @@ template <class E, int V, int LR, int R, bool STEP> __global__ void __launch_bou
                     float a = scale[r][i];
                     if (STEP || p.g) {
                         const float gv = g[r][i];
-                        a *= gv * keep_of(gv, small_sigmoid<kPrecise>(gv));
+                        a *= gv * keep_of(gv, sigmoid_pair<kPrecise>(gv));
                     }
                     x[r][i] = __builtin_fmaf(a, y[r][i] * ry * w[r][i], x[r][i]);
                 }
@@ -192,7 +192,7 @@ template <class E, int V, int LR, int R> __global__ void __launch_bounds__(LR > 
                     float a = scale[r][i];
                     if (p.g) {
                         const float gv = g[r][i];
-                        a *= gv * keep_of(gv, small_sigmoid<kPrecise>(gv));
+                        a *= gv * keep_of(gv, sigmoid_pair<kPrecise>(gv));
                     }
                     x[r][i] = __builtin_fmaf(a, yn[r][i] * w[r][i], x[r][i]);
                 }
@@ -224,7 +224,9 @@ template <class E, int V, int LR, int R> __global__ void __launch_bounds__(LR > 
                 const float n = yn[r][i] * w[r][i], dp = dx[r][i] * scale[r][i];
                 float a = 1.0f;
                 if (p.g) {
-                    const float gv = g[r][i], s = small_sigmoid<kPrecise>(gv), sig = keep_of(gv, s);
+                    const float gv = g[r][i];
+                    const Sigmoid s = sigmoid_pair<kPrecise>(gv);
+                    const float sig = keep_of(gv, s);
                     a = gv * sig;
                     g[r][i] = dp * n * __builtin_fmaf(a, take_of(gv, s), sig);
                 }

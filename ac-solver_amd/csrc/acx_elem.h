@@ -57,11 +57,14 @@ template <class E, int V> __device__ __forceinline__ void store_some(E* p, int v
     }
 }
 
-// sigmoid of z and of -z from one exponential: e = exp(-|z|), the smaller of the two is e / (1 + e), and the larger 1 minus it, which
-// loses nothing (the smaller one as 1 - sigmoid would).  exp(-|z|) = 2^t (1 + l ln 2) with t = -|z| log2 e rounded and l what the rounding
+// sigmoid of z and of -z from one exponential: with e = exp(-|z|) the larger of the two is 1 / (1 + e) and the smaller e / (1 + e), which
+// keeps its accuracy where 1 - sigmoid would lose it.  exp(-|z|) = 2^t (1 + l ln 2) with t = -|z| log2 e rounded and l what the rounding
 // and the constant left out: the error of t alone would grow to |z| 2^-24.  PRECISE false leaves l out: for 16-bit results.
 // NaN comes out as NaN, +-infinity as 0 and 1.
-template <bool PRECISE> __device__ __forceinline__ float small_sigmoid(float z) {
+struct Sigmoid {
+    float large, small;
+};
+template <bool PRECISE> __device__ __forceinline__ Sigmoid sigmoid_pair(float z) {
     constexpr float kLog2e = 1.44269502162933349609375f, kLog2eLow = 1.92596299e-8f, kLn2 = 0.693147182464599609375f;
     const float a = -__builtin_fabsf(z);
     const float t = a * kLog2e;
@@ -71,11 +74,12 @@ template <bool PRECISE> __device__ __forceinline__ float small_sigmoid(float z) 
         // (at infinity l is NaN and e is 0: the comparison keeps the 0, and a NaN of z is in e already)
         e = t < -126.0f ? e : __builtin_fmaf(e * l, kLn2, e);
     }
-    return e * __builtin_amdgcn_rcpf(1.0f + e);
+    const float r = __builtin_amdgcn_rcpf(1.0f + e);
+    return {r, e * r};
 }
-// sigmoid(z) and 1 - sigmoid(z) from small_sigmoid(z)
-__device__ __forceinline__ float keep_of(float z, float s) { return z < 0.0f ? s : 1.0f - s; }
-__device__ __forceinline__ float take_of(float z, float s) { return z < 0.0f ? 1.0f - s : s; }
+// sigmoid(z) and 1 - sigmoid(z)
+__device__ __forceinline__ float keep_of(float z, Sigmoid s) { return z < 0.0f ? s.small : s.large; }
+__device__ __forceinline__ float take_of(float z, Sigmoid s) { return z < 0.0f ? s.large : s.small; }
 
 // run fn.template operator()<E>() for the element type of an ACX_* code; false for any other code
 template <class F> static inline bool with_element(int dtype, F&& fn) {

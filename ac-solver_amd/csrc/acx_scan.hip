@@ -81,19 +81,18 @@ template <class E, int V> __device__ __forceinline__ void load_segment(const voi
         p += t0 + k + 1 < end ? st * (int64_t)sizeof(E) : 0;
     }
 }
-__device__ __forceinline__ uint32_t load_resets(const Args& p, const Lane& me, int64_t t0, int64_t end) {
-    uint32_t bits = 0;
-    if (p.reset) {
-        const uint8_t* r = p.reset + t0 * p.N + me.n0;
-        const uint32_t offset = (uint32_t)(me.n - me.n0);
+// Where an episode starts: one lane mask per step in scalar registers, so that a select on it is one instruction.  -> whether this lane has any
+__device__ __forceinline__ bool load_starts(const Args& p, const Lane& me, int64_t t0, int64_t end, bool (&start)[kSeg]) {
+    bool any = false;
+    const uint8_t* r = p.reset + t0 * p.N + me.n0;
+    const uint32_t offset = (uint32_t)(me.n - me.n0);
 #pragma unroll
-        for (int k = 0; k < kSeg; k++) {
-            bits |= (uint32_t)(r[offset] != 0) << k;
-            r += t0 + k + 1 < end ? p.N : 0;
-        }
-        if (end - t0 < kSeg) bits &= (1u << (end - t0)) - 1;
+    for (int k = 0; k < kSeg; k++) {
+        start[k] = t0 + k < end && r[offset] != 0;
+        any |= start[k];
+        r += t0 + k + 1 < end ? p.N : 0;
     }
-    return bits;
+    return any;
 }
 // `second` behind `first`
 __device__ __forceinline__ Affine join(Affine second, Affine first) {
@@ -141,13 +140,45 @@ template <int V, int W, bool FORWARD> __device__ __forceinline__ void meet(Affin
     }
 }
 
-// The compiler shall compute f and 1 - f again where it needs them next (two instructions) instead of holding both (two registers a value).
-template <int V> __device__ __forceinline__ void forget(float (&s)[kSeg][V]) {
+// f and 1 - f of a segment.  COMPACT holds one register for the two, the smaller one with the sign of z, and makes the larger one from it where it
+// is needed (the compiler would keep both across the passes over a segment: `forget` stops it); for two channels a lane.
+template <int V, bool COMPACT> struct Gates {
+    float s[kSeg][V];
+    float u[COMPACT ? 1 : kSeg][COMPACT ? 1 : V];
+    template <bool PRECISE> __device__ __forceinline__ void set(int k, int i, float z) {
+        const Sigmoid q = sigmoid_pair<PRECISE>(z);
+        if constexpr (COMPACT) {
+            s[k][i] = __builtin_copysignf(q.small, z);
+        } else {
+            s[k][i] = keep_of(z, q);
+            u[k][i] = take_of(z, q);
+        }
+    }
+    __device__ __forceinline__ void identity(int k, int i) {  // f = 1
+        if constexpr (COMPACT) {
+            s[k][i] = 0.0f;
+        } else {
+            s[k][i] = 1.0f;
+            u[k][i] = 0.0f;
+        }
+    }
+    __device__ __forceinline__ float f(int k, int i) const {
+        if constexpr (COMPACT) return __builtin_signbitf(s[k][i]) ? -s[k][i] : 1.0f - s[k][i];
+        else return s[k][i];
+    }
+    __device__ __forceinline__ float take(int k, int i) const {
+        if constexpr (COMPACT) return __builtin_signbitf(s[k][i]) ? 1.0f + s[k][i] : s[k][i];
+        else return u[k][i];
+    }
+    __device__ __forceinline__ void forget() {
+        if constexpr (COMPACT) {
 #pragma unroll
-    for (int k = 0; k < kSeg; k++)
+            for (int k = 0; k < kSeg; k++)
 #pragma unroll
-        for (int i = 0; i < V; i++) asm volatile("" : "+v"(s[k][i]));
-}
+                for (int i = 0; i < V; i++) asm volatile("" : "+v"(s[k][i]));
+        }
+    }
+};
 
 // FINAL: write h, last, bounds.  Otherwise only compose the chunk (agg).
 template <class E, int V, int W, bool FINAL> __global__ void __launch_bounds__(64 * W) k_scan_fwd(const Args p) {
@@ -172,21 +203,29 @@ template <class E, int V, int W, bool FINAL> __global__ void __launch_bounds__(6
     for (int64_t tile = begin; tile < end; tile += W * kSeg, buf ^= 1) {
         const int64_t t0 = tile + w * kSeg;
         float f[kSeg][V], b[kSeg][V];
-        uint32_t resets = 0;
+        bool start[kSeg] = {}, starts = false;
         if (t0 < end) {
             load_segment<E, V>(p.z, me.n0 * p.z_sn, p.z_st, z_off, t0, end, f);
             load_segment<E, V>(p.c, me.n0 * p.c_sn, p.c_st, c_off, t0, end, b);
-            resets = load_resets(p, me, t0, end);
+            if (p.reset) starts = load_starts(p, me, t0, end, start);
         }
 #pragma unroll
-        for (int k = 0; k < kSeg; k++) {
-            const bool in = t0 + k < end;
+        for (int k = 0; k < kSeg; k++)
 #pragma unroll
             for (int i = 0; i < V; i++) {
-                const float z = f[k][i], s = small_sigmoid<kPrecise>(z);
-                f[k][i] = in ? keep_of(z, s) : 1.0f;
-                b[k][i] = in ? take_of(z, s) * b[k][i] : 0.0f;
+                const float z = f[k][i];
+                const Sigmoid s = sigmoid_pair<kPrecise>(z);
+                f[k][i] = keep_of(z, s);
+                b[k][i] *= take_of(z, s);
             }
+        if (t0 + kSeg > end) {  // (uniform) steps behind the end: the identity
+#pragma unroll
+            for (int k = 0; k < kSeg; k++)
+#pragma unroll
+                for (int i = 0; i < V; i++) {
+                    f[k][i] = t0 + k < end ? f[k][i] : 1.0f;
+                    b[k][i] = t0 + k < end ? b[k][i] : 0.0f;
+                }
         }
         float h[V];
 #pragma unroll
@@ -199,9 +238,9 @@ template <class E, int V, int W, bool FINAL> __global__ void __launch_bounds__(6
 #pragma unroll
                 for (int k = 0; k < kSeg; k++) {
                     a *= f[k][i];
-                    x = __builtin_fmaf(f[k][i], resets >> k & 1 ? 0.0f : x, b[k][i]);
+                    x = __builtin_fmaf(f[k][i], start[k] ? 0.0f : x, b[k][i]);
                 }
-                m[i] = {resets ? -1.0f : a, x};
+                m[i] = {starts ? -1.0f : a, x};
             }
             if constexpr (W == 1) {
 #pragma unroll
@@ -217,7 +256,7 @@ template <class E, int V, int W, bool FINAL> __global__ void __launch_bounds__(6
 #pragma unroll
                 for (int k = 0; k < kSeg; k++) {
 #pragma unroll
-                    for (int i = 0; i < V; i++) h[i] = __builtin_fmaf(f[k][i], resets >> k & 1 ? 0.0f : h[i], b[k][i]);
+                    for (int i = 0; i < V; i++) h[i] = __builtin_fmaf(f[k][i], start[k] ? 0.0f : h[i], b[k][i]);
                     if (t0 + k < end) store<E, V>((E*)(hp + h_off), h);
                     hp += nd * (int64_t)sizeof(E);
                 }
@@ -262,30 +301,30 @@ template <class E, int V, int W, bool FINAL> __global__ void __launch_bounds__(6
 #pragma unroll
         for (int i = 0; i < V; i++) carry[i].b = x[i];
     }
-    // small_sigmoid is held with the sign of z: f = s for z < 0, else 1 - s
-    auto fkeep = [](float v) { return __builtin_signbitf(v) ? -v : 1.0f - v; };
-    auto ftake = [](float v) { return __builtin_signbitf(v) ? 1.0f + v : v; };
     int buf = 0;
     const int64_t tiles = (end - begin + W * kSeg - 1) / (W * kSeg);
     for (int64_t tile = begin + (tiles - 1) * (W * kSeg); tile >= begin; tile -= W * kSeg, buf ^= 1) {
         const int64_t t0 = tile + w * kSeg;
-        float s[kSeg][V], diff[kSeg][V], g[kSeg][V];  // diff: c, then k h_(t-1) - c; g: dh
-        uint32_t resets = 0;
+        Gates<V, (V > 1)> gate;
+        float diff[kSeg][V], g[kSeg][V];  // c, then k h_(t-1) - c; dh
+        bool start[kSeg] = {}, starts = false;
         if (t0 < end) {
-            load_segment<E, V>(p.z, me.n0 * p.z_sn, p.z_st, z_off, t0, end, s);
+            load_segment<E, V>(p.z, me.n0 * p.z_sn, p.z_st, z_off, t0, end, gate.s);
             if constexpr (FINAL) load_segment<E, V>(p.c, me.n0 * p.c_sn, p.c_st, c_off, t0, end, diff);
             load_segment<E, V>(p.dh, me.n0 * p.dh_sn, p.dh_st, g_off, t0, end, g);
-            resets = load_resets(p, me, t0, end);
+            if (p.reset) starts = load_starts(p, me, t0, end, start);
         }
 #pragma unroll
-        for (int k = 0; k < kSeg; k++) {
-            const bool in = t0 + k < end;
+        for (int k = 0; k < kSeg; k++)
 #pragma unroll
-            for (int i = 0; i < V; i++) {
-                const float z = s[k][i], v = small_sigmoid<kPrecise>(z);
-                s[k][i] = in ? (z < 0.0f ? -v : v) : 0.0f;  // (a step behind the end: f = 1)
-                g[k][i] = in ? g[k][i] : 0.0f;
-            }
+            for (int i = 0; i < V; i++) gate.template set<kPrecise>(k, i, gate.s[k][i]);
+        if (t0 + kSeg > end) {  // (uniform) steps behind the end: the identity
+#pragma unroll
+            for (int k = 0; k < kSeg; k++)
+                if (t0 + k >= end) {
+#pragma unroll
+                    for (int i = 0; i < V; i++) gate.identity(k, i), g[k][i] = 0.0f;
+                }
         }
         if constexpr (FINAL) {
             if (t0 < end) {
@@ -295,14 +334,14 @@ template <class E, int V, int W, bool FINAL> __global__ void __launch_bounds__(6
                 for (int k = 0; k < kSeg; k++) {
 #pragma unroll
                     for (int i = 0; i < V; i++) {
-                        const float c = diff[k][i], before = resets >> k & 1 ? 0.0f : h[i];
-                        h[i] = __builtin_fmaf(fkeep(s[k][i]), before, ftake(s[k][i]) * c);
+                        const float c = diff[k][i], before = start[k] ? 0.0f : h[i];
+                        h[i] = __builtin_fmaf(gate.f(k, i), before, gate.take(k, i) * c);
                         diff[k][i] = before - c;
                     }
                 }
             }
         }
-        forget<V>(s);
+        gate.forget();
         float x[V];  // X behind this segment
 #pragma unroll
         for (int i = 0; i < V; i++) x[i] = carry[i].b;
@@ -313,18 +352,18 @@ template <class E, int V, int W, bool FINAL> __global__ void __launch_bounds__(6
                 float a = 1.0f, b = 0.0f;
 #pragma unroll
                 for (int k = kSeg - 1; k >= 0; k--) {
-                    const float f = fkeep(s[k][i]);
+                    const float f = gate.f(k, i);
                     a *= f;
-                    b = resets >> k & 1 ? 0.0f : f * (g[k][i] + b);
+                    b = start[k] ? 0.0f : f * (g[k][i] + b);
                 }
-                m[i] = {resets ? -1.0f : a, b};
+                m[i] = {starts ? -1.0f : a, b};
             }
             if constexpr (W == 1) {
 #pragma unroll
                 for (int i = 0; i < V; i++) carry[i] = join(m[i], carry[i]);
             } else {
                 meet<V, W, false>(s_map[buf], lane, w, m, carry, x);
-                forget<V>(s);
+                gate.forget();
             }
         }
         if constexpr (FINAL) {
@@ -338,10 +377,11 @@ template <class E, int V, int W, bool FINAL> __global__ void __launch_bounds__(6
                         float dc[V], dz[V];
 #pragma unroll
                         for (int i = 0; i < V; i++) {
-                            const float f = fkeep(s[k][i]), u = ftake(s[k][i]), G = g[k][i] + x[i];
+                            const float u = gate.take(k, i), G = g[k][i] + x[i];
                             dc[i] = u * G;
-                            dz[i] = f * u * diff[k][i] * G;
-                            x[i] = resets >> k & 1 ? 0.0f : f * G;
+                            const float fG = gate.f(k, i) * G;
+                            dz[i] = diff[k][i] * u * fG;
+                            x[i] = start[k] ? 0.0f : fG;
                         }
                         store<E, V>((E*)(dcp + dc_off), dc);
                         store<E, V>((E*)(dzp + dz_off), dz);
@@ -380,12 +420,12 @@ static Plan plan_of(int64_t T, int64_t N, int64_t D) {
     p.v = D >= 2 && groups(2) >= 512 ? 2 : 1;
     p.lpr = (int)((D + p.v - 1) / p.v);
     p.groups = groups(p.v);
-    p.w = p.groups >= 2048 || segments == 1 ? 1 : p.v == 2 || segments <= 4 ? 4 : 16;
+    p.w = p.groups >= 2048 || segments == 1 ? 1 : p.v == 2 || segments <= 4 ? 4 : 8;
     p.chunks = 1;
     p.chunk = T;
     const int64_t tile = (int64_t)p.w * kSeg, tiles = (T + tile - 1) / tile;
-    if (p.groups < 128 && tiles >= 4) {
-        int64_t want = 256 / p.groups;
+    if (p.groups < 256 && tiles >= 4) {
+        int64_t want = 512 / p.groups;
         if (want > 128) want = 128;
         if (want > tiles) want = tiles;
         p.chunk = (tiles + want - 1) / want * tile;
@@ -409,7 +449,7 @@ template <class E, int V, int W> static void launch(bool forward, const Args& a,
 template <class E, int V> static void launch_w(bool forward, const Args& a, const Plan& p, hipStream_t st) {
     if (p.w == 1) launch<E, V, 1>(forward, a, p, st);
     else if (p.w == 4) launch<E, V, 4>(forward, a, p, st);
-    else if constexpr (V == 1) launch<E, V, 16>(forward, a, p, st);
+    else if constexpr (V == 1) launch<E, V, 8>(forward, a, p, st);
 }
 static int run(bool forward, Args& a, int dtype, void* work, int64_t work_bytes, hipStream_t st, const char* who) {
     const Plan p = plan_of(a.T, a.N, a.D);
