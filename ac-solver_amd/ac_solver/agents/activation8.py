@@ -85,7 +85,7 @@ class _Linear8(torch.autograd.Function):
         return out
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @T.once
     def backward(ctx, d_out):
         q, exponent, weight = ctx.saved_tensors
         need_x, need_w, need_b = ctx.needs_input_grad

@@ -97,7 +97,7 @@ class _BlockOutput(torch.autograd.Function):
         return new, u
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @T.once
     def backward(ctx, d_new, d_u):
         if d_new is None and d_u is None:
             return (None,) * 7

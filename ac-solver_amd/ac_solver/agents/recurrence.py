@@ -16,9 +16,7 @@ def _operands(candidate, gate, reset, state):
     if steps < 1:
         raise ValueError("a scan needs at least one step")
     if reset is not None:
-        if isinstance(reset, torch.Tensor) and reset.dtype == torch.bool:
-            reset = reset.view(torch.uint8)
-        reset = T.plain(reset, "reset", (steps, rows), candidate.device, torch.uint8)
+        reset = T.flags(reset, "reset", (steps, rows), candidate.device)
     if state is not None:
         state = T.plain(state, "state", (rows, width), candidate.device)
     T.require_gpu(candidate)
@@ -79,7 +77,7 @@ class _GatedScan(torch.autograd.Function):
         return hidden, last
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @T.once
     def backward(ctx, d_hidden, d_last):
         candidate, gate, reset, bounds = ctx.saved_tensors
         if d_hidden is None:
@@ -126,9 +124,7 @@ def recurrent_step(x, projected, state, weight, scale=None, next_weight=None, re
     scale = None if scale is None else T.plain(scale, "scale", (width,), dev)
     next_weight = None if next_weight is None else T.plain(next_weight, "next_weight", (width,), dev)
     if reset is not None:
-        if isinstance(reset, torch.Tensor) and reset.dtype == torch.bool:
-            reset = reset.view(torch.uint8)
-        reset = T.plain(reset, "reset", (rows,), dev, torch.uint8)
+        reset = T.flags(reset, "reset", (rows,), dev)
     if next_state is not None and T.plain(next_state, "next_state", (rows, width), dev) is not next_state:
         raise ValueError("next_state has to be contiguous")
     T.require_gpu(x)
