@@ -5,7 +5,7 @@ import torch
 from ac_solver import _acx
 from ac_solver.agents import _tensors as T
 
-MAX_WIDTH = 8192
+MAX_WIDTH = 4096
 
 
 def _rows(t):
@@ -106,7 +106,7 @@ class _BlockOutput(torch.autograd.Function):
 
 
 def block_output(x, y, gate, weight, scale=None, next_weight=None, eps=1e-6):
-    """The end of a block in one pass over the rows (last axis of x, y, gate: float32, bfloat16 or float16, up to 8192 features; weights
+    """The end of a block in one pass over the rows (last axis of x, y, gate: float32, bfloat16 or float16, up to 4096 features; weights
     float32 [width]):
 
         new = x + scale * silu(gate) * rms(y) * weight;  u = rms(new) * next_weight;  rms(v) = v / sqrt(mean(v^2) + eps)

@@ -42,18 +42,18 @@ struct Args {
     float* partial;                  // [workgroups, 3, D]
 };
 
-// sum over the LR lanes of a row, in every one of them
+// sum over the LR lanes of a row, in every one of them (s_red: one float per wave of the workgroup)
 template <int LR> __device__ __forceinline__ float row_sum(float v, float* s_red) {
-#pragma unroll
-    for (int m = 1; m < (LR < 64 ? LR : 64); m *= 2) v += __shfl_xor(v, m);
+    v = lane_sum<(LR < 64 ? LR : 64)>(v);
     if constexpr (LR > 64) {
         constexpr int kWaves = LR / 64;
         __syncthreads();  // (the sums of the last call have been read)
         if ((threadIdx.x & 63) == 0) s_red[threadIdx.x >> 6] = v;
         __syncthreads();
         v = 0.0f;
+        const float* mine = s_red + threadIdx.x / LR * kWaves;
 #pragma unroll
-        for (int i = 0; i < kWaves; i++) v += s_red[i];
+        for (int i = 0; i < kWaves; i++) v += mine[i];
     }
     return v;
 }
@@ -66,7 +66,7 @@ template <int V> __device__ __forceinline__ void load_weight(const float* p, int
 template <class E, int V, int LR, int R, bool STEP> __global__ void __launch_bounds__(LR > 256 ? LR : 256) k_block_fwd(const Args p) {
     constexpr bool kPrecise = sizeof(E) == 4;
     constexpr int kThreads = LR > 256 ? LR : 256, kRows = kThreads / LR;
-    __shared__ float s_red[LR > 64 ? LR / 64 : 1];
+    __shared__ float s_red[kThreads / 64];
     const int j = threadIdx.x % LR;
     float w[R][V], scale[R][V], next[R][V];
 #pragma unroll
@@ -153,7 +153,7 @@ template <class E, int V, int LR, int R, bool STEP> __global__ void __launch_bou
 template <class E, int V, int LR, int R> __global__ void __launch_bounds__(LR > 256 ? LR : 256) k_block_bwd(const Args p) {
     constexpr bool kPrecise = sizeof(E) == 4;
     constexpr int kThreads = LR > 256 ? LR : 256, kRows = kThreads / LR;
-    __shared__ float s_red[LR > 64 ? LR / 64 : 1];
+    __shared__ float s_red[kThreads / 64];
     __shared__ float s_join[kRows > 1 ? kThreads * R * V : 1];
     const int j = threadIdx.x % LR;
     float w[R][V], scale[R][V], next[R][V];
@@ -165,21 +165,40 @@ template <class E, int V, int LR, int R> __global__ void __launch_bounds__(LR > 
         load_weight<V>(p.scale, d, p.D, 1.0f, scale[r]);
         load_weight<V>(p.next, d, p.D, 0.0f, next[r]);
     }
-    for (int64_t row0 = (int64_t)blockIdx.x * kRows; row0 < p.M; row0 += (int64_t)gridDim.x * kRows) {
-        const int64_t row = row0 + threadIdx.x / LR;
+    // The next row's operands are on their way while the current row is worked on (as they lie in memory: 16-bit types take half the registers).
+    typename Vec<E, V>::type in[5][R];
+    float in_ry = 0.0f, in_rx = 0.0f;
+    auto fetch = [&](int64_t row) {
         const bool live = row < p.M;
-        float x[R][V], yn[R][V], g[R][V], dx[R][V], t[R][V];
-        const float ry = live ? p.stats[2 * row] : 0.0f, rx = live ? p.stats[2 * row + 1] : 0.0f;
-        float sum = 0.0f;
+        if (live) in_ry = p.stats[2 * row], in_rx = p.stats[2 * row + 1];
 #pragma unroll
         for (int r = 0; r < R; r++) {
             const int d = (r * LR + j) * V, valid = live ? p.D - d : 0;
-            load_some<E, V>((const E*)p.x + row * p.x_sn + d, valid, x[r]);
-            if (p.y) load_some<E, V>((const E*)p.y + row * p.y_sn + d, valid, yn[r]);
-            if (p.g) load_some<E, V>((const E*)p.g + row * p.g_sn + d, valid, g[r]);
-            if (p.d_out) load_some<E, V>((const E*)p.d_out + row * p.do_sn + d, valid, dx[r]);
-            if (p.d_u) load_some<E, V>((const E*)p.d_u + row * p.du_sn + d, valid, t[r]);
+            in[0][r] = load_raw<E, V>((const E*)p.x + row * p.x_sn + d, valid);
+            if (p.y) in[1][r] = load_raw<E, V>((const E*)p.y + row * p.y_sn + d, valid);
+            if (p.g) in[2][r] = load_raw<E, V>((const E*)p.g + row * p.g_sn + d, valid);
+            if (p.d_out) in[3][r] = load_raw<E, V>((const E*)p.d_out + row * p.do_sn + d, valid);
+            if (p.d_u) in[4][r] = load_raw<E, V>((const E*)p.d_u + row * p.du_sn + d, valid);
         }
+    };
+    constexpr bool kAhead = LR <= 256 && R == 1;  // (wider rows have no registers left for it)
+    if (kAhead) fetch((int64_t)blockIdx.x * kRows + threadIdx.x / LR);
+    for (int64_t row0 = (int64_t)blockIdx.x * kRows; row0 < p.M; row0 += (int64_t)gridDim.x * kRows) {
+        const int64_t row = row0 + threadIdx.x / LR;
+        const bool live = row < p.M;
+        if (!kAhead) fetch(row);
+        float x[R][V], yn[R][V], g[R][V], dx[R][V], t[R][V];
+        const float ry = live ? in_ry : 0.0f, rx = live ? in_rx : 0.0f;
+        float sum = 0.0f;
+#pragma unroll
+        for (int r = 0; r < R; r++) {
+            widen<E, V>(in[0][r], x[r]);
+            if (p.y) widen<E, V>(in[1][r], yn[r]);
+            if (p.g) widen<E, V>(in[2][r], g[r]);
+            if (p.d_out) widen<E, V>(in[3][r], dx[r]);
+            if (p.d_u) widen<E, V>(in[4][r], t[r]);
+        }
+        if (kAhead) fetch(row + (int64_t)gridDim.x * kRows);
         // yn = y ry; x becomes xn = new rx; t = d_u (then d_u next)
 #pragma unroll
         for (int r = 0; r < R; r++) {
@@ -284,44 +303,57 @@ template <class E, int V, int LR, int R> __global__ void __launch_bounds__(LR > 
     }
 }
 
-// out[c] = sum over k of partial[k][c]: 64 columns a workgroup, four waves over the workgroups' sums, in a fixed order
-__global__ void __launch_bounds__(256) k_block_sum(const float* __restrict__ partial, int n, int64_t columns, float* __restrict__ out) {
-    __shared__ float s[4][64];
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-    const int64_t c = (int64_t)blockIdx.x * 64 + lane;
+// out[c] = sum over k of partial[k][c], in a fixed order: 64 columns a workgroup, four a lane, 64 threads over the workgroups' sums
+__global__ void __launch_bounds__(1024) k_block_sum(const float* __restrict__ partial, int n, int columns, float* __restrict__ out) {
+    __shared__ float s[64][65];
+    const int q = threadIdx.x & 15, part = threadIdx.x >> 4;
+    const int c = blockIdx.x * 64 + q * 4, valid = columns - c;
     float a[4] = {};
-    if (c < columns) {
-        int k = w;
-        for (; k + 12 < n; k += 16) {
+#pragma unroll 8
+    for (int k = part; k < n; k += 64) {
+        float v[4];
+        load_some<float, 4>(partial + (int64_t)k * columns + c, valid, v);
 #pragma unroll
-            for (int i = 0; i < 4; i++) a[i] += partial[(int64_t)(k + 4 * i) * columns + c];
-        }
-        for (; k < n; k += 4) a[0] += partial[(int64_t)k * columns + c];
+        for (int i = 0; i < 4; i++) a[i] += v[i];
     }
-    s[w][lane] = (a[0] + a[1]) + (a[2] + a[3]);
+#pragma unroll
+    for (int i = 0; i < 4; i++) s[part][q * 4 + i] = a[i];
     __syncthreads();
-    if (w == 0 && c < columns) out[c] = (s[0][lane] + s[1][lane]) + (s[2][lane] + s[3][lane]);
+    const int column = threadIdx.x & 63, w = threadIdx.x >> 6;
+    const float v = (s[w * 4][column] + s[w * 4 + 1][column]) + (s[w * 4 + 2][column] + s[w * 4 + 3][column]);
+    __syncthreads();
+    s[w][column] = v;
+    __syncthreads();
+    if (w == 0 && blockIdx.x * 64 + column < columns) {
+        float t = 0.0f;
+#pragma unroll
+        for (int k = 0; k < 16; k++) t += s[k][column];
+        out[blockIdx.x * 64 + column] = t;
+    }
 }
 
-constexpr int kMaxWidth = 8192;
+constexpr int kMaxWidth = 4096;  // 1024 lanes with a vector of 4 each; with two they would spill
 
-// lanes of a row and vectors of a lane, by width; 16-bit rows of up to 1024 take vectors of 8, wider ones vectors of 4 (registers)
+// lanes of a row and vectors of a lane, by width.  16-bit rows of up to 512 take vectors of 8 (16-byte loads); beyond, a lane with two of them would
+// hold 256 registers in the backward pass: vectors of 4 and more lanes.
 template <class E, class F> static void with_shape(int64_t D, F&& fn) {
     using std::integral_constant;
     auto pick = [&](auto v) {
         constexpr int V = decltype(v)::value;
         const int64_t n = (D + V - 1) / V;
-        if (n <= 8) fn(v, integral_constant<int, 8>{}, integral_constant<int, 1>{});
-        else if (n <= 16) fn(v, integral_constant<int, 16>{}, integral_constant<int, 1>{});
-        else if (n <= 32) fn(v, integral_constant<int, 32>{}, integral_constant<int, 1>{});
-        else if (n <= 64) fn(v, integral_constant<int, 64>{}, integral_constant<int, 1>{});
-        else if (n <= 128) fn(v, integral_constant<int, 64>{}, integral_constant<int, 2>{});
+        constexpr integral_constant<int, 1> one{};
+        if (n <= 8) fn(v, integral_constant<int, 8>{}, one);
+        else if (n <= 16) fn(v, integral_constant<int, 16>{}, one);
+        else if (n <= 32) fn(v, integral_constant<int, 32>{}, one);
+        else if (n <= 64) fn(v, integral_constant<int, 64>{}, one);
         else if constexpr (V == 4) {
-            if (n <= 512) fn(v, integral_constant<int, 256>{}, integral_constant<int, 2>{});
-            else fn(v, integral_constant<int, 1024>{}, integral_constant<int, 2>{});
+            if (n <= 128) fn(v, integral_constant<int, 128>{}, one);
+            else if (n <= 256) fn(v, integral_constant<int, 256>{}, one);
+            else if (n <= 512) fn(v, integral_constant<int, 256>{}, integral_constant<int, 2>{});
+            else fn(v, integral_constant<int, 1024>{}, one);
         }
     };
-    if (sizeof(E) == 2 && D <= 1024) pick(integral_constant<int, 8>{});
+    if (sizeof(E) == 2 && D <= 512) pick(integral_constant<int, 8>{});
     else pick(integral_constant<int, 4>{});
 }
 static int64_t workgroups(int64_t M, int lr) {
@@ -426,7 +458,7 @@ extern "C" int acx_block_backward(const void* d_x, int64_t x_row, const void* d_
         });
     });
     ACX_HIP_TRY(hipGetLastError());
-    hipLaunchKernelGGL(block::k_block_sum, dim3((unsigned)((3 * D + 63) / 64)), dim3(256), 0, (hipStream_t)stream, (const float*)d_work, (int)n, 3 * D, d_weight_grads);
+    hipLaunchKernelGGL(block::k_block_sum, dim3((unsigned)((3 * D + 63) / 64)), dim3(1024), 0, (hipStream_t)stream, (const float*)d_work, (int)n, (int)(3 * D), d_weight_grads);
     ACX_HIP_TRY(hipGetLastError());
     return ACX_OK;
 }

@@ -57,6 +57,38 @@ template <class E, int V> __device__ __forceinline__ void store_some(E* p, int v
     }
 }
 
+// The same in two steps, for loads that are started well before their values are looked at: the vector as it lies in memory, and its values.
+template <class E, int V> __device__ __forceinline__ typename Vec<E, V>::type load_raw(const E* p, int valid) {
+    typename Vec<E, V>::type v = {};
+    if (valid >= V) {
+        v = *(const typename Vec<E, V>::type*)p;
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; i++)
+            if (i < valid) v[i] = p[i];
+    }
+    return v;
+}
+template <class E, int V> __device__ __forceinline__ void widen(const typename Vec<E, V>::type& v, float (&out)[V]) {
+#pragma unroll
+    for (int i = 0; i < V; i++) out[i] = (float)v[i];
+}
+
+// v + the value of the lane that a DPP control names: neighbours 1, 2, 4 and 8 apart cost one vector instruction and no trip through LDS
+template <int CTRL> __device__ __forceinline__ float add_dpp(float v) {
+    return v + __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xF, 0xF, true));
+}
+// sum over groups of LANES (1 ... 64, a power of two) neighbouring lanes, the same bits in every one of them
+template <int LANES> __device__ __forceinline__ float lane_sum(float v) {
+    if constexpr (LANES > 1) v = add_dpp<0xB1>(v);   // quad_perm 1 0 3 2
+    if constexpr (LANES > 2) v = add_dpp<0x4E>(v);   // quad_perm 2 3 0 1
+    if constexpr (LANES > 4) v = add_dpp<0x141>(v);  // mirrored within 8
+    if constexpr (LANES > 8) v = add_dpp<0x140>(v);  // mirrored within 16
+    if constexpr (LANES > 16) v += __shfl_xor(v, 16);
+    if constexpr (LANES > 32) v += __shfl_xor(v, 32);
+    return v;
+}
+
 // sigmoid of z and of -z from one exponential: with e = exp(-|z|) the larger of the two is 1 / (1 + e) and the smaller e / (1 + e), which
 // keeps its accuracy where 1 - sigmoid would lose it.  exp(-|z|) = 2^t (1 + l ln 2) with t = -|z| log2 e rounded and l what the rounding
 // and the constant left out: the error of t alone would grow to |z| 2^-24.  PRECISE false leaves l out: for 16-bit results.

@@ -367,7 +367,7 @@ int acx_scan_backward(const void *d_candidate, int64_t c_step, int64_t c_row, co
                       void *d_gate_grad, int64_t dz_step, int64_t dz_row, float *d_state_grad, void *d_work, int64_t work_bytes, void *stream);
 
 /* ---- recurrent agent: the end of a block (csrc/acx_block.hip) -------------------------------------------------------------------
- * For each of M rows of D <= 8192 features (rms(v) = v / sqrt(mean(v^2) + eps)):
+ * For each of M rows of D <= 4096 features (rms(v) = v / sqrt(mean(v^2) + eps)):
  *     new = x + scale * silu(gate) * rms(y) * weight,   u = rms(new) * next_weight
  * acx_block_forward: d_gate NULL: without the gate, d_scale NULL: 1, d_next_weight NULL: no u; d_y NULL: u = rms(x) * next_weight alone
  * (d_new is not written).  Activations of type `dtype` with a stride between rows in elements, d_new and d_u contiguous; weights float32.

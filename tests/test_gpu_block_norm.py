@@ -121,7 +121,7 @@ def check(M, D, dtype, seed=0, layout="contiguous", gate=True, scale=True, nxt=T
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("D", [1, 2, 3, 7, 8, 9, 31, 32, 33, 50, 64, 65, 127, 130, 255, 256, 257, 500, 512, 513, 1000, 1024, 1025, 2047, 2048, 2049, 4097, 8192])
+@pytest.mark.parametrize("D", [1, 2, 3, 7, 8, 9, 31, 32, 33, 50, 64, 65, 127, 130, 255, 256, 257, 500, 512, 513, 1000, 1024, 1025, 2047, 2048, 2049, 3001, 4095, 4096])
 def test_widths(D, dtype):
     check(70 if D < 600 else 9, D, dtype)
 
@@ -244,7 +244,7 @@ def step_definition(x, p, h, w, s, v, r):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("N,D", [(1, 1), (1, 256), (3, 50), (70, 130), (9, 1031), (3, 8192), (5000, 72), (1025, 256)])
+@pytest.mark.parametrize("N,D", [(1, 1), (1, 256), (3, 50), (70, 130), (9, 1031), (3, 4096), (5000, 72), (1025, 256)])
 def test_one_step(N, D, dtype):
     import torch
 

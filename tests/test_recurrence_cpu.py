@@ -59,8 +59,8 @@ def test_the_block_end_refuses_what_it_cannot_read():
         B.block_output(x, x, x, w, w, w)
     with pytest.raises(ValueError, match="GPU"):
         B.block_input(x, w)
-    with pytest.raises(ValueError, match="8192"):
-        B.block_input(torch.zeros(1, 8193), torch.zeros(8193))
+    with pytest.raises(ValueError, match="4096"):
+        B.block_input(torch.zeros(1, 4097), torch.zeros(4097))
     with pytest.raises(ValueError, match="y has the shape"):
         B.block_output(x, x[:4], x, w)
     with pytest.raises(ValueError, match="gate is"):
@@ -93,8 +93,8 @@ def test_a_step_refuses_what_it_cannot_read():
         R.recurrent_step(x, p, h, w, next_state=torch.zeros(8, 5).t())
     with pytest.raises(TypeError, match="reset"):
         R.recurrent_step(x, p, h, w, reset=torch.zeros(5))
-    with pytest.raises(ValueError, match="8192"):
-        R.recurrent_step(torch.zeros(1, 8193), torch.zeros(1, 3 * 8193), torch.zeros(1, 8193), torch.zeros(8193))
+    with pytest.raises(ValueError, match="4096"):
+        R.recurrent_step(torch.zeros(1, 4097), torch.zeros(1, 3 * 4097), torch.zeros(1, 4097), torch.zeros(4097))
 
 
 def test_8_bit_checkpoints_refuse_what_they_cannot_read():
