@@ -67,11 +67,14 @@ def weight_grad8(d_out, q, exponent):
     if not rows or not outputs:
         return torch.zeros((outputs, inputs), device=dev), d_out.reshape(-1, outputs).float().sum(0) if outputs else torch.zeros(0, device=dev)
     g = d_out.reshape(-1, outputs)
+    if rows > 1 and not outputs <= g.stride(0) < 1 << 24:  # (the expanded gradient of a sum over the rows, say)
+        g = g.contiguous()
+    stride = g.stride(0) if rows > 1 else outputs
     dw = torch.empty((outputs, inputs), dtype=torch.float32, device=dev)
     db = torch.empty(outputs, dtype=torch.float32, device=dev)
     work = T.scratch(_acx.lib.acx_act8_workspace_bytes(rows, outputs, inputs), dev)
     with T.on_device_of(d_out):
-        _acx.check(_acx.lib.acx_act8_weight_grad(g.data_ptr(), g.stride(0), T.DTYPES[d_out.dtype], q.data_ptr(), exponent.data_ptr(), rows, outputs, inputs, dw.data_ptr(),
+        _acx.check(_acx.lib.acx_act8_weight_grad(g.data_ptr(), stride, T.DTYPES[d_out.dtype], q.data_ptr(), exponent.data_ptr(), rows, outputs, inputs, dw.data_ptr(),
                                                  db.data_ptr(), T.ptr(work), 0 if work is None else work.numel(), T.stream_of(d_out)), "acx_act8_weight_grad")
     return dw, db
 

@@ -88,12 +88,12 @@ template <class E, int V> __global__ void __launch_bounds__(256) k_unpack8(const
 }
 
 // ---- weight gradient ----------------------------------------------------------------------------------------------------------------
-// A workgroup owns a TO x TI tile of dW and a share of the rows, kRows at a time: dy and q of these rows go from memory through registers
-// (the next rows' while the current ones are multiplied) into LDS as the 16-byte operands of v_mfma_f32_32x32x16_bf16, 8 rows of one column
-// each.  Columns are stored in the order in which the threads bring them (column c of a vector of V stands at (c % V) TO / V + c / V): a
-// wave's stores and its operand loads are both contiguous, and the order is undone when dW is written.
-constexpr int kRows = 64;
-
+// A workgroup owns a TO x TI tile of dW and a share of the rows, ROWS at a time: dy and q of these rows go from memory through registers into
+// LDS as the 16-byte operands of v_mfma_f32_32x32x16_bf16, 8 rows of one column each.  Columns are stored in the order in which the threads
+// bring them (column c of a vector of V stands at (c % V) TO / V + c / V): a wave's stores and its operand loads are both contiguous, and
+// the order is undone when dW is written.
+// LDS holds two sets of rows and registers a third that is on its way from memory: a step multiplies one set and writes the next.  The two
+// waves of a SIMD take these halves in opposite order, so one's conversions (vector pipe) run under the other's products (matrix pipe).
 typedef __bf16 frag __attribute__((ext_vector_type(8)));
 typedef float acc16 __attribute__((ext_vector_type(16)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
@@ -103,7 +103,7 @@ struct Args {
     int64_t dy_sn;
     const int8_t* q;
     const uint8_t* exps;
-    int64_t M, share;  // rows of a workgroup's share (a multiple of kRows)
+    int64_t M, share, whole;  // rows; rows of a workgroup's share, rows that are read in whole vectors (multiples of the rows of a step)
     int O, I, nb;
     float *dw, *db;    // [shares, O, I], [shares, O] (db nullable)
 };
@@ -113,105 +113,156 @@ __device__ __forceinline__ uint32_t bits_of(float v) { return __builtin_bit_cast
 __device__ __forceinline__ uint32_t high_halves(float lo, float hi) { return __builtin_amdgcn_perm(bits_of(hi), bits_of(lo), 0x07060302u); }
 __device__ __forceinline__ float truncated(float v) { return __builtin_bit_cast(float, bits_of(v) & 0xFFFF0000u); }
 
-template <class E> struct Pieces { static constexpr int n = 3; };
-template <> struct Pieces<bf16_t> { static constexpr int n = 1; };
-template <> struct Pieces<f16_t> { static constexpr int n = 2; };
+// bfloat16 pieces of a value, and the rows of a step (as many as two sets of 256 + 256 columns leave room for in LDS)
+template <class E> struct Pieces { static constexpr int n = 3, rows = 32; };
+template <> struct Pieces<bf16_t> { static constexpr int n = 1, rows = 64; };
+template <> struct Pieces<f16_t> { static constexpr int n = 2, rows = 32; };
 
-template <class E, int TO, int TI, int NT> __global__ void __launch_bounds__(NT) k_weight_grad8(const Args p) {
-    constexpr int kP = Pieces<E>::n, VO = sizeof(E) == 4 ? 4 : 4, VI = 4, kChunks = kRows / 8;
-    constexpr int kWaves = NT / 64;
-    constexpr int kWO = TO / 64 < 1 ? 1 : (TO == 256 ? 4 : (NT == 256 ? 2 : 1)), kWI = kWaves / kWO;  // waves over the tile
-    constexpr int kFO = TO / kWO / 32, kFI = TI / kWI / 32;                                           // 32 x 32 products of a wave
-    static_assert(kFO >= 1 && kFI >= 1 && kWO * kWI == kWaves, "tile");
-    constexpr int kItemsA = kChunks * (TO / VO), kItemsB = kChunks * (TI / VI);
-    constexpr int kPerA = (kItemsA + NT - 1) / NT, kPerB = (kItemsB + NT - 1) / NT;
-    extern __shared__ u32x4 s_mem[];
-    u32x4* sA = s_mem;                          // [piece][chunk][TO]
-    u32x4* sB = s_mem + kP * kChunks * TO;      // [chunk][TI]
+template <class E, int TO, int TI, int NT> struct Tile {
+    static constexpr int kP = Pieces<E>::n, kRows = Pieces<E>::rows, kChunks = kRows / 8;
+    static constexpr int VO = kRows / 16, VI = 4;
+    static constexpr int kWaves = NT / 64, kWO = TO == 256 ? 4 : NT == 256 ? 2 : 1, kWI = kWaves / kWO;  // waves over the tile
+    static constexpr int kFO = TO / kWO / 32, kFI = TI / kWI / 32;                                       // 32 x 32 products of a wave
+    static_assert(kFO >= 1 && kFI >= 1 && kFO * kWO * 32 == TO && kFI * kWI * 32 == TI, "tile");
+    static constexpr int kItemsA = kChunks * (TO / VO), kItemsB = kChunks * (TI / VI);
+    static constexpr int kPerA = (kItemsA + NT - 1) / NT, kPerB = (kItemsB + NT - 1) / NT;
+    static constexpr int kSet = (kP * TO + TI) * kChunks;  // 16-byte operands of a set
+    static constexpr size_t kLds = (size_t)2 * kSet * 16;
+};
+
+// TAIL: the last few rows of all, value by value with every bound checked, as a share of their own; else a share of the rows that are read in
+// whole vectors.
+template <class E, int TO, int TI, int NT, bool TAIL> __device__ __forceinline__ void weight_grad8(const Args& p) {
+    using T = Tile<E, TO, TI, NT>;
+    constexpr int kP = T::kP, kRows = T::kRows, kChunks = T::kChunks, VO = T::VO, VI = T::VI, kFO = T::kFO, kFI = T::kFI;
+    extern __shared__ u32x4 s_mem[];  // two sets of [piece][chunk][TO], [chunk][TI]
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int o0 = blockIdx.x * TO, i0 = blockIdx.y * TI;
-    const int64_t begin = (int64_t)blockIdx.z * p.share, end = begin + p.share < p.M ? begin + p.share : p.M;
-    float a[kPerA][8][VO];
-    uint32_t b[kPerB][8], be[kPerB][8];
-    float bias[kPerA][VO] = {};
+    const int64_t begin = TAIL ? p.whole : (int64_t)blockIdx.z * p.share, end = TAIL ? p.M : begin + p.share < p.whole ? begin + p.share : p.whole;
+    typename Vec<E, VO>::type a[T::kPerA][8];
+    uint32_t b[T::kPerB][8], be[T::kPerB][8];
+    float bias[T::kPerA][VO] = {};
+    // The rows of a step start at a pointer that the whole workgroup shares; a lane's place among them takes 32 bits (the host checks that).  Whole
+    // vectors are read whatever O and I are: behind the last column stand values of the next row, which end up in columns of the tile that are not
+    // written; p.whole leaves rows enough behind it for that.
+    uint32_t off_a[T::kPerA], off_b[T::kPerB], off_e[T::kPerB];
+#pragma unroll
+    for (int k = 0; k < T::kPerA; k++) {
+        const int item = tid + k * NT, chunk = item / (TO / VO), o = o0 + item % (TO / VO) * VO;
+        off_a[k] = item < T::kItemsA && o < p.O ? ((uint32_t)(chunk * 8) * (uint32_t)p.dy_sn + (uint32_t)o) * (uint32_t)sizeof(E) : 0;
+    }
+#pragma unroll
+    for (int k = 0; k < T::kPerB; k++) {
+        const int item = tid + k * NT, chunk = item / (TI / VI), i = i0 + item % (TI / VI) * VI;
+        const bool on = item < T::kItemsB && i < p.I;
+        off_b[k] = on ? (uint32_t)(chunk * 8) * (uint32_t)p.I + (uint32_t)i : 0;
+        off_e[k] = on ? (uint32_t)(chunk * 8) * (uint32_t)p.nb + (uint32_t)(i / kBlock) : 0;
+    }
     auto fetch = [&](int64_t m0) {
+        const char* dy = (const char*)p.dy + m0 * p.dy_sn * (int64_t)sizeof(E);
+        const int8_t* q = p.q + m0 * p.I;
+        const uint8_t* exps = p.exps + m0 * p.nb;
 #pragma unroll
-        for (int k = 0; k < kPerA; k++) {
-            const int item = tid + k * NT, chunk = item / (TO / VO), o = o0 + item % (TO / VO) * VO;
-            const bool on = item < kItemsA;
+        for (int r = 0; r < 8; r++) {
 #pragma unroll
-            for (int r = 0; r < 8; r++) {
-                const int64_t m = m0 + chunk * 8 + r;
-                load_some<E, VO>((const E*)p.dy + m * p.dy_sn + o, on && m < end ? p.O - o : 0, a[k][r]);
+            for (int k = 0; k < T::kPerA; k++) a[k][r] = *(const typename Vec<E, VO>::type*)(dy + off_a[k]);
+#pragma unroll
+            for (int k = 0; k < T::kPerB; k++) {
+                b[k][r] = *(const typename Bytes<4>::type*)(q + off_b[k]);
+                be[k][r] = exps[off_e[k]];
             }
+            dy += p.dy_sn * (int64_t)sizeof(E), q += p.I, exps += p.nb;
         }
+    };
+    // eight rows of an item's columns -> the 16-byte operands of every column (and the column sums)
+    auto write_a = [&](u32x4* sA, int chunk, int g, int v, float (&x)[8], float& sum) {
 #pragma unroll
-        for (int k = 0; k < kPerB; k++) {
-            const int item = tid + k * NT, chunk = item / (TI / VI), i = i0 + item % (TI / VI) * VI;
-            const bool on = item < kItemsB;
+        for (int r = 0; r < 8; r++) sum += x[r];
 #pragma unroll
-            for (int r = 0; r < 8; r++) {
-                const int64_t m = m0 + chunk * 8 + r;
-                const int valid = on && m < end ? p.I - i : 0;
-                const int8_t* src = p.q + m * p.I + i;
-                b[k][r] = 0;
-                if (valid >= VI) {
-                    b[k][r] = *(const typename Bytes<4>::type*)src;
-                } else {
+        for (int piece = 0; piece < kP; piece++) {
+            u32x4 w;
 #pragma unroll
-                    for (int v = 0; v < VI; v++)
-                        if (v < valid) b[k][r] |= (uint32_t)(uint8_t)src[v] << (8 * v);
+            for (int r = 0; r < 4; r++) w[r] = high_halves(x[2 * r], x[2 * r + 1]);
+            sA[(piece * kChunks + chunk) * TO + v * (TO / VO) + g] = w;
+            if (piece + 1 < kP) {
+#pragma unroll
+                for (int r = 0; r < 8; r++) {  // what the piece left out (an infinity is its own first piece: nothing)
+                    const float t = truncated(x[r]);
+                    x[r] = t == x[r] ? 0.0f : x[r] - t;
                 }
-                be[k][r] = valid > 0 ? p.exps[m * p.nb + i / kBlock] : 0;
             }
         }
     };
-    auto stage = [&]() {
+    auto write_b = [&](u32x4* sB, int chunk, int g, const uint32_t (&q)[8], const uint32_t (&e)[8]) {
+        float f[8];
 #pragma unroll
-        for (int k = 0; k < kPerA; k++) {
-            const int item = tid + k * NT, chunk = item / (TO / VO), g = item % (TO / VO);
-            if (item < kItemsA) {
+        for (int r = 0; r < 8; r++) f[r] = exponent_factor(e[r]);
+#pragma unroll
+        for (int v = 0; v < VI; v++) {
+            u32x4 w;
+#pragma unroll
+            for (int r = 0; r < 4; r++) w[r] = high_halves((float)(int8_t)(q[2 * r] >> (8 * v)) * f[2 * r], (float)(int8_t)(q[2 * r + 1] >> (8 * v)) * f[2 * r + 1]);
+            sB[chunk * TI + v * (TI / VI) + g] = w;
+        }
+    };
+    auto stage = [&](u32x4* set) {
+#pragma unroll
+        for (int k = 0; k < T::kPerA; k++) {
+            const int item = tid + k * NT;
+            if (item < T::kItemsA) {
 #pragma unroll
                 for (int v = 0; v < VO; v++) {
+                    float x[8];
 #pragma unroll
-                    for (int r = 0; r < 8; r++) bias[k][v] += a[k][r][v];
-#pragma unroll
-                    for (int piece = 0; piece < kP; piece++) {
-                        u32x4 w;
-#pragma unroll
-                        for (int r = 0; r < 4; r++) {
-                            float &lo = a[k][2 * r][v], &hi = a[k][2 * r + 1][v];
-                            w[r] = high_halves(lo, hi);
-                            if (piece + 1 < kP) {  // (an infinity is its own first piece: nothing is left)
-                                const float tl = truncated(lo), th = truncated(hi);
-                                lo = tl == lo ? 0.0f : lo - tl;
-                                hi = th == hi ? 0.0f : hi - th;
-                            }
-                        }
-                        sA[(piece * kChunks + chunk) * TO + v * (TO / VO) + g] = w;
-                    }
+                    for (int r = 0; r < 8; r++) x[r] = (float)a[k][r][v];
+                    write_a(set, item / (TO / VO), item % (TO / VO), v, x, bias[k][v]);
                 }
             }
         }
 #pragma unroll
-        for (int k = 0; k < kPerB; k++) {
-            const int item = tid + k * NT, chunk = item / (TI / VI), g = item % (TI / VI);
-            if (item < kItemsB) {
-                float f[8];
+        for (int k = 0; k < T::kPerB; k++) {
+            const int item = tid + k * NT;
+            if (item < T::kItemsB) write_b(set + kP * kChunks * TO, item / (TI / VI), item % (TI / VI), b[k], be[k]);
+        }
+    };
+    auto stage_tail = [&](u32x4* set, int64_t m0) {
 #pragma unroll
-                for (int r = 0; r < 8; r++) f[r] = exponent_factor(be[k][r]);
+        for (int k = 0; k < T::kPerA; k++) {
+            const int item = tid + k * NT, chunk = item / (TO / VO), g = item % (TO / VO);
+            if (item < T::kItemsA) {
 #pragma unroll
-                for (int v = 0; v < VI; v++) {
-                    u32x4 w;
+                for (int v = 0; v < VO; v++) {
+                    float x[8];
 #pragma unroll
-                    for (int r = 0; r < 4; r++)
-                        w[r] = high_halves((float)(int8_t)(b[k][2 * r] >> (8 * v)) * f[2 * r], (float)(int8_t)(b[k][2 * r + 1] >> (8 * v)) * f[2 * r + 1]);
-                    sB[chunk * TI + v * (TI / VI) + g] = w;
+                    for (int r = 0; r < 8; r++) {
+                        const int64_t m = m0 + chunk * 8 + r;
+                        x[r] = m < p.M && o0 + g * VO + v < p.O ? (float)((const E*)p.dy)[m * p.dy_sn + o0 + g * VO + v] : 0.0f;
+                    }
+                    write_a(set, chunk, g, v, x, bias[k][v]);
                 }
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < T::kPerB; k++) {
+            const int item = tid + k * NT, chunk = item / (TI / VI), g = item % (TI / VI);
+            if (item < T::kItemsB) {
+                uint32_t q[8], e[8];
+#pragma unroll
+                for (int r = 0; r < 8; r++) {
+                    const int64_t m = m0 + chunk * 8 + r;
+                    q[r] = 0, e[r] = 0;
+                    if (m < p.M && i0 + g * VI < p.I) {
+                        e[r] = p.exps[m * p.nb + (i0 + g * VI) / kBlock];
+#pragma unroll
+                        for (int v = 0; v < VI; v++)
+                            if (i0 + g * VI + v < p.I) q[r] |= (uint32_t)(uint8_t)p.q[m * p.I + i0 + g * VI + v] << (8 * v);
+                    }
+                }
+                write_b(set + kP * kChunks * TO, chunk, g, q, e);
             }
         }
     };
-    const int wo = wave % kWO, wi = wave / kWO;
+    const int wo = wave % T::kWO, wi = wave / T::kWO;
     acc16 acc[kFO][kFI];
 #pragma unroll
     for (int x = 0; x < kFO; x++)
@@ -219,12 +270,8 @@ template <class E, int TO, int TI, int NT> __global__ void __launch_bounds__(NT)
         for (int y = 0; y < kFI; y++)
 #pragma unroll
             for (int r = 0; r < 16; r++) acc[x][y][r] = 0.0f;
-    fetch(begin);
-    for (int64_t m0 = begin; m0 < end; m0 += kRows) {
-        __syncthreads();  // (the operands of the last rows have been read)
-        stage();
-        __syncthreads();
-        if (m0 + kRows < end) fetch(m0 + kRows);
+    auto multiply = [&](const u32x4* set) {
+        const u32x4 *sA = set, *sB = set + kP * kChunks * TO;
 #pragma unroll
         for (int ks = 0; ks < kRows / 16; ks++) {
             const int chunk = 2 * ks + (lane >> 5), col = lane & 31;
@@ -241,6 +288,33 @@ template <class E, int TO, int TI, int NT> __global__ void __launch_bounds__(NT)
                 }
             }
         }
+    };
+    if constexpr (TAIL) {
+#pragma unroll 1
+        for (int64_t m0 = begin; m0 < end; m0 += kRows) {
+            stage_tail(s_mem, m0);
+            __syncthreads();
+            multiply(s_mem);
+            __syncthreads();
+        }
+    } else {
+        const bool first = wave < T::kWaves / 2;
+        int set = 0;
+        fetch(begin);
+        // what is staged in a round is multiplied in the next one
+#pragma unroll 1
+        for (int64_t m0 = begin - kRows; m0 < end; m0 += kRows, set ^= 1) {
+#pragma unroll 1
+            for (int half = 0; half < 2; half++) {  // (a loop: one copy of either half in the code, or the registers do not suffice)
+                if ((half == 0) == first) {
+                    if (m0 + kRows < end) stage(s_mem + (set ^ 1) * T::kSet);
+                    if (m0 + 2 * kRows < end) fetch(m0 + 2 * kRows);
+                } else if (m0 >= begin) {
+                    multiply(s_mem + set * T::kSet);
+                }
+            }
+            __syncthreads();  // (the set that was multiplied may be written again, the other one is complete)
+        }
     }
     float* dw = p.dw + (int64_t)blockIdx.z * p.O * p.I;
 #pragma unroll
@@ -256,11 +330,10 @@ template <class E, int TO, int TI, int NT> __global__ void __launch_bounds__(NT)
         }
     if (p.db && blockIdx.y == 0) {
         float* s = (float*)s_mem;  // [chunk][TO]
-        __syncthreads();
 #pragma unroll
-        for (int k = 0; k < kPerA; k++) {
+        for (int k = 0; k < T::kPerA; k++) {
             const int item = tid + k * NT, chunk = item / (TO / VO), g = item % (TO / VO);
-            if (item < kItemsA) {
+            if (item < T::kItemsA) {
 #pragma unroll
                 for (int v = 0; v < VO; v++) s[chunk * TO + g * VO + v] = bias[k][v];
             }
@@ -273,6 +346,11 @@ template <class E, int TO, int TI, int NT> __global__ void __launch_bounds__(NT)
             p.db[(int64_t)blockIdx.z * p.O + o0 + o] = v;
         }
     }
+}
+
+template <class E, int TO, int TI, int NT> __global__ void __launch_bounds__(NT) k_weight_grad8(const Args p) {
+    if (blockIdx.z + 1 == gridDim.z) weight_grad8<E, TO, TI, NT, true>(p);
+    else weight_grad8<E, TO, TI, NT, false>(p);
 }
 
 // out[c] = sum over the shares, in their order; dW and db in one launch
@@ -296,26 +374,27 @@ __global__ void __launch_bounds__(256) k_join_shares(const float* __restrict__ d
 
 struct Plan {
     int to, ti;
-    int64_t go, gi, shares, share;
+    int64_t go, gi, whole, share, shares;
 };
 static Plan plan_of(int64_t M, int64_t O, int64_t I) {
+    constexpr int kStep = 64;  // rows of a step of every type divide it
     Plan p;
     p.to = O <= 64 ? 64 : 256;
     p.ti = I <= 64 ? 64 : 256;
     p.go = (O + p.to - 1) / p.to;
     p.gi = (I + p.ti - 1) / p.ti;
-    int64_t want = 256 / (p.go * p.gi);
+    p.whole = M >= 4 ? (M - 4) / kStep * kStep : 0;  // behind these rows at least four more: a vector of up to four values that starts in them ends in bounds
+    int64_t want = 256 / (p.go * p.gi) - 1;
     if (want < 1) want = 1;
-    const int64_t steps = (M + kRows - 1) / kRows;
-    const int64_t per = (steps + want - 1) / want;
-    p.share = (per < 4 ? 4 : per) * kRows;
-    p.shares = (M + p.share - 1) / p.share;
+    const int64_t steps = p.whole / kStep, per = (steps + want - 1) / want;
+    p.share = (per < 4 ? 4 : per) * kStep;
+    p.shares = (p.whole + p.share - 1) / p.share + 1;  // and the rows behind them
     return p;
 }
 static int64_t work_floats(const Plan& p, int64_t O, int64_t I) { return p.shares > 1 ? p.shares * O * (I + 1) : 0; }
 
 template <class E, int TO, int TI, int NT> static hipError_t launch(const Args& a, const Plan& p, hipStream_t st) {
-    const size_t lds = (size_t)(Pieces<E>::n * TO + TI) * (kRows / 8) * 16;
+    constexpr size_t lds = Tile<E, TO, TI, NT>::kLds;
     const hipError_t e = hipFuncSetAttribute((const void*)k_weight_grad8<E, TO, TI, NT>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
     if (e != hipSuccess) return e;
     hipLaunchKernelGGL((k_weight_grad8<E, TO, TI, NT>), dim3((unsigned)p.go, (unsigned)p.gi, (unsigned)p.shares), dim3(NT), lds, st, a);
@@ -376,12 +455,14 @@ extern "C" int acx_act8_weight_grad(const void* d_out_grad, int64_t o_row, int d
     if (rc) return rc;
     if (O == 0 || I == 0 || M == 0) return fail(ACX_E_INVAL, "acx_act8_weight_grad: no rows, outputs or inputs");
     if (O > (1 << 16) || I > (1 << 16)) return fail(ACX_E_INVAL, "acx_act8_weight_grad: up to 65536 outputs and inputs");
+    if (o_row < O || o_row >= ((int64_t)1 << 24)) return fail(ACX_E_INVAL, "acx_act8_weight_grad: rows of d_out_grad overlap or lie too far apart (2^24 elements)");
     if (!d_out_grad || !d_q || !d_exponent || !d_weight_grad) return fail(ACX_E_INVAL, "acx_act8_weight_grad: null pointer");
     const act8::Plan p = act8::plan_of(M, O, I);
     const int64_t need = act8::work_floats(p, O, I) * 4;
     if (need && (!d_work || work_bytes < need)) return fail(ACX_E_CAPACITY, "acx_act8_weight_grad: a workspace of %lld bytes is needed (acx_act8_workspace_bytes)", (long long)need);
     act8::Args a = {};
     a.dy = d_out_grad, a.dy_sn = o_row, a.q = d_q, a.exps = d_exponent, a.M = M, a.share = p.share, a.O = (int)O, a.I = (int)I, a.nb = (int)((I + act8::kBlock - 1) / act8::kBlock);
+    a.whole = p.whole;
     a.dw = need ? (float*)d_work : d_weight_grad;
     a.db = !d_bias_grad ? nullptr : need ? (float*)d_work + p.shares * O * I : d_bias_grad;
     hipError_t err = hipSuccess;

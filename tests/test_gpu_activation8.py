@@ -148,6 +148,22 @@ def test_weight_grad_of_every_single_place():
         assert torch.equal(weight_grad8(dy, *pack8(x))[0], want)
 
 
+def test_weight_grad_of_an_expanded_gradient():
+    import torch
+
+    from ac_solver.agents.activation8 import pack8, unpack8, weight_grad8
+
+    q, e = pack8(values(300, 40, "float32", 9))
+    row = torch.randn(1, 20, device="cuda")
+    one = torch.ones((), device="cuda")
+    for d in (row.expand(300, 20), one.expand(300, 20)):
+        dw, db = weight_grad8(d, q, e)
+        same, sb = weight_grad8(d.contiguous(), q, e)
+        assert torch.equal(dw, same) and torch.equal(db, sb)
+    one_row = weight_grad8(row.expand(5, 20)[:1], q[:1].contiguous(), e[:1].contiguous())[0]
+    assert torch.equal(one_row, row.t() @ unpack8(q[:1], e[:1])) or float((one_row - row.t() @ unpack8(q[:1], e[:1])).abs().max()) < 1e-5
+
+
 def test_weight_grad_shows_infinities_and_nans():
     """they reach the outputs that their row and column reach, and no others"""
     import torch
