@@ -130,17 +130,24 @@ template <class E, int TO, int TI, int NT> struct Tile {
     static constexpr size_t kLds = (size_t)2 * kSet * 16;
 };
 
-// TAIL: the last few rows of all, value by value with every bound checked, as a share of their own; else a share of the rows that are read in
-// whole vectors.
-template <class E, int TO, int TI, int NT, bool TAIL> __device__ __forceinline__ void weight_grad8(const Args& p) {
+// PART kTail: the last few rows of all, value by value with every bound checked, as a share of their own; else a share of the rows that are read in
+// whole vectors, kStageFirst and kMultiplyFirst for the two halves of the workgroup's waves (apart from each other as functions: together
+// they need more registers than there are).
+enum { kTail, kStageFirst, kMultiplyFirst };
+template <class E, int TO, int TI, int NT, int PART> __device__ __forceinline__ void weight_grad8(const Args& p) {
     using T = Tile<E, TO, TI, NT>;
+    constexpr bool TAIL = PART == kTail;
+    asm volatile("; part %0" ::"n"(PART));  // (unlike each other from here on: nothing of one is moved in front of the branch between them)
     constexpr int kP = T::kP, kRows = T::kRows, kChunks = T::kChunks, VO = T::VO, VI = T::VI, kFO = T::kFO, kFI = T::kFI;
     extern __shared__ u32x4 s_mem[];  // two sets of [piece][chunk][TO], [chunk][TI]
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int o0 = blockIdx.x * TO, i0 = blockIdx.y * TI;
     const int64_t begin = TAIL ? p.whole : (int64_t)blockIdx.z * p.share, end = TAIL ? p.M : begin + p.share < p.whole ? begin + p.share : p.whole;
-    typename Vec<E, VO>::type a[T::kPerA][8];
-    uint32_t b[T::kPerB][8], be[T::kPerB][8];
+    // two steps on their way from memory
+    struct Rows {
+        typename Vec<E, VO>::type a[T::kPerA][8];
+        uint32_t b[T::kPerB][8], e[T::kPerB];
+    } in[2];
     float bias[T::kPerA][VO] = {};
     // The rows of a step start at a pointer that the whole workgroup shares; a lane's place among them takes 32 bits (the host checks that).  Whole
     // vectors are read whatever O and I are: behind the last column stand values of the next row, which end up in columns of the tile that are not
@@ -154,30 +161,31 @@ template <class E, int TO, int TI, int NT, bool TAIL> __device__ __forceinline__
 #pragma unroll
     for (int k = 0; k < T::kPerB; k++) {
         const int item = tid + k * NT, chunk = item / (TI / VI), i = i0 + item % (TI / VI) * VI;
-        const bool on = item < T::kItemsB && i < p.I;
-        off_b[k] = on ? (uint32_t)(chunk * 8) * (uint32_t)p.I + (uint32_t)i : 0;
-        off_e[k] = on ? (uint32_t)(chunk * 8) * (uint32_t)p.nb + (uint32_t)(i / kBlock) : 0;
+        const bool on = item < T::kItemsB;
+        off_b[k] = on && i < p.I ? (uint32_t)(chunk * 8) * (uint32_t)p.I + (uint32_t)i : 0;
+        // (the eight lanes of a block of features bring the exponents of one row each, those behind the last feature too)
+        off_e[k] = on && i / kBlock < p.nb ? (uint32_t)(chunk * 8 + (tid & 7)) * (uint32_t)p.nb + (uint32_t)(i / kBlock) : 0;
     }
-    auto fetch = [&](int64_t m0) {
+    auto fetch = [&](Rows& to, int64_t m0) {
         const char* dy = (const char*)p.dy + m0 * p.dy_sn * (int64_t)sizeof(E);
         const int8_t* q = p.q + m0 * p.I;
-        const uint8_t* exps = p.exps + m0 * p.nb;
+#pragma unroll
+        for (int k = 0; k < T::kPerB; k++) to.e[k] = p.exps[m0 * p.nb + off_e[k]];
 #pragma unroll
         for (int r = 0; r < 8; r++) {
 #pragma unroll
-            for (int k = 0; k < T::kPerA; k++) a[k][r] = *(const typename Vec<E, VO>::type*)(dy + off_a[k]);
+            for (int k = 0; k < T::kPerA; k++) to.a[k][r] = *(const typename Vec<E, VO>::type*)(dy + off_a[k]);
 #pragma unroll
-            for (int k = 0; k < T::kPerB; k++) {
-                b[k][r] = *(const typename Bytes<4>::type*)(q + off_b[k]);
-                be[k][r] = exps[off_e[k]];
-            }
-            dy += p.dy_sn * (int64_t)sizeof(E), q += p.I, exps += p.nb;
+            for (int k = 0; k < T::kPerB; k++) to.b[k][r] = *(const typename Bytes<4>::type*)(q + off_b[k]);
+            dy += p.dy_sn * (int64_t)sizeof(E), q += p.I;
         }
     };
     // eight rows of an item's columns -> the 16-byte operands of every column (and the column sums)
-    auto write_a = [&](u32x4* sA, int chunk, int g, int v, float (&x)[8], float& sum) {
-#pragma unroll
-        for (int r = 0; r < 8; r++) sum += x[r];
+    auto write_a = [&](u32x4* sA, int chunk, int g, int v, float (&x)[8], float& sum, bool count) {
+        const float s8 = ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]));
+        sum += count ? s8 : 0.0f;
+        // what a piece leaves out of an infinity would be NaN: 0 then.  The sum tells whether there is one (or finite values that add up to one).
+        const bool wild = kP > 1 && __any(!(__builtin_fabsf(s8) < __builtin_inff()));
 #pragma unroll
         for (int piece = 0; piece < kP; piece++) {
             u32x4 w;
@@ -185,10 +193,15 @@ template <class E, int TO, int TI, int NT, bool TAIL> __device__ __forceinline__
             for (int r = 0; r < 4; r++) w[r] = high_halves(x[2 * r], x[2 * r + 1]);
             sA[(piece * kChunks + chunk) * TO + v * (TO / VO) + g] = w;
             if (piece + 1 < kP) {
+                if (!wild) {
 #pragma unroll
-                for (int r = 0; r < 8; r++) {  // what the piece left out (an infinity is its own first piece: nothing)
-                    const float t = truncated(x[r]);
-                    x[r] = t == x[r] ? 0.0f : x[r] - t;
+                    for (int r = 0; r < 8; r++) x[r] -= truncated(x[r]);
+                } else {
+#pragma unroll
+                    for (int r = 0; r < 8; r++) {
+                        const float t = truncated(x[r]);
+                        x[r] = t == x[r] ? 0.0f : x[r] - t;
+                    }
                 }
             }
         }
@@ -203,9 +216,10 @@ template <class E, int TO, int TI, int NT, bool TAIL> __device__ __forceinline__
 #pragma unroll
             for (int r = 0; r < 4; r++) w[r] = high_halves((float)(int8_t)(q[2 * r] >> (8 * v)) * f[2 * r], (float)(int8_t)(q[2 * r + 1] >> (8 * v)) * f[2 * r + 1]);
             sB[chunk * TI + v * (TI / VI) + g] = w;
+            __builtin_amdgcn_sched_barrier(0);
         }
     };
-    auto stage = [&](u32x4* set) {
+    auto stage = [&](u32x4* set, const Rows& from, bool count) {
 #pragma unroll
         for (int k = 0; k < T::kPerA; k++) {
             const int item = tid + k * NT;
@@ -214,15 +228,28 @@ template <class E, int TO, int TI, int NT, bool TAIL> __device__ __forceinline__
                 for (int v = 0; v < VO; v++) {
                     float x[8];
 #pragma unroll
-                    for (int r = 0; r < 8; r++) x[r] = (float)a[k][r][v];
-                    write_a(set, item / (TO / VO), item % (TO / VO), v, x, bias[k][v]);
+                    for (int r = 0; r < 8; r++) x[r] = (float)from.a[k][r][v];
+                    write_a(set, item / (TO / VO), item % (TO / VO), v, x, bias[k][v], count);
+                    __builtin_amdgcn_sched_barrier(0);
                 }
             }
         }
 #pragma unroll
         for (int k = 0; k < T::kPerB; k++) {
             const int item = tid + k * NT;
-            if (item < T::kItemsB) write_b(set + kP * kChunks * TO, item / (TI / VI), item % (TI / VI), b[k], be[k]);
+            if (item < T::kItemsB) {
+                uint32_t e[8];
+                // (ds_swizzle, bit mask mode: the lane of the same eight whose low bits are r)
+                e[0] = __builtin_amdgcn_ds_swizzle(from.e[k], 0x0018 | 0 << 5);
+                e[1] = __builtin_amdgcn_ds_swizzle(from.e[k], 0x0018 | 1 << 5);
+                e[2] = __builtin_amdgcn_ds_swizzle(from.e[k], 0x0018 | 2 << 5);
+                e[3] = __builtin_amdgcn_ds_swizzle(from.e[k], 0x0018 | 3 << 5);
+                e[4] = __builtin_amdgcn_ds_swizzle(from.e[k], 0x0018 | 4 << 5);
+                e[5] = __builtin_amdgcn_ds_swizzle(from.e[k], 0x0018 | 5 << 5);
+                e[6] = __builtin_amdgcn_ds_swizzle(from.e[k], 0x0018 | 6 << 5);
+                e[7] = __builtin_amdgcn_ds_swizzle(from.e[k], 0x0018 | 7 << 5);
+                write_b(set + kP * kChunks * TO, item / (TI / VI), item % (TI / VI), from.b[k], e);
+            }
         }
     };
     auto stage_tail = [&](u32x4* set, int64_t m0) {
@@ -238,7 +265,7 @@ template <class E, int TO, int TI, int NT, bool TAIL> __device__ __forceinline__
                         const int64_t m = m0 + chunk * 8 + r;
                         x[r] = m < p.M && o0 + g * VO + v < p.O ? (float)((const E*)p.dy)[m * p.dy_sn + o0 + g * VO + v] : 0.0f;
                     }
-                    write_a(set, chunk, g, v, x, bias[k][v]);
+                    write_a(set, chunk, g, v, x, bias[k][v], true);
                 }
             }
         }
@@ -287,6 +314,7 @@ template <class E, int TO, int TI, int NT, bool TAIL> __device__ __forceinline__
                     for (int y = 0; y < kFI; y++) acc[x][y] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fa, fb[y], acc[x][y], 0, 0, 0);
                 }
             }
+            __builtin_amdgcn_sched_barrier(0);  // (operands of one k-step at a time: there are no registers for more)
         }
     };
     if constexpr (TAIL) {
@@ -298,22 +326,44 @@ template <class E, int TO, int TI, int NT, bool TAIL> __device__ __forceinline__
             __syncthreads();
         }
     } else {
-        const bool first = wave < T::kWaves / 2;
-        int set = 0;
-        fetch(begin);
-        // what is staged in a round is multiplied in the next one
+        // Everything on the way is unconditional (behind the last step the last one again, not counted and not multiplied): the waits before a use
+        // then count the loads issued since, and the other set of registers stays in flight.
+        auto at_most = [&](int64_t m) { return m < end ? m : end - kRows; };
+        auto renew = [&](Rows& rows, u32x4* to, int64_t m0) {  // step m0 from its registers into LDS, the registers to the step two further on
+            stage(to, rows, m0 < end);
+            __builtin_amdgcn_sched_barrier(0);
+            fetch(rows, at_most(m0 + 2 * kRows));
+            __builtin_amdgcn_sched_barrier(0);
+        };
+        auto product = [&](const u32x4* from, int64_t m0) {
+            if (m0 < end) multiply(from);
+            __builtin_amdgcn_sched_barrier(0);
+        };
+        u32x4 *const s0 = s_mem, *const s1 = s_mem + T::kSet;
+        fetch(in[0], begin);
+        fetch(in[1], at_most(begin + kRows));
+        renew(in[0], s0, begin);
+        __syncthreads();
+        if constexpr (PART == kStageFirst) {
 #pragma unroll 1
-        for (int64_t m0 = begin - kRows; m0 < end; m0 += kRows, set ^= 1) {
-#pragma unroll 1
-            for (int half = 0; half < 2; half++) {  // (a loop: one copy of either half in the code, or the registers do not suffice)
-                if ((half == 0) == first) {
-                    if (m0 + kRows < end) stage(s_mem + (set ^ 1) * T::kSet);
-                    if (m0 + 2 * kRows < end) fetch(m0 + 2 * kRows);
-                } else if (m0 >= begin) {
-                    multiply(s_mem + set * T::kSet);
-                }
+            for (int64_t m0 = begin; m0 < end; m0 += 2 * kRows) {
+                renew(in[1], s1, m0 + kRows);
+                product(s0, m0);
+                __syncthreads();  // (the set that was multiplied may be written again, the other one is complete)
+                renew(in[0], s0, m0 + 2 * kRows);
+                product(s1, m0 + kRows);
+                __syncthreads();
             }
-            __syncthreads();  // (the set that was multiplied may be written again, the other one is complete)
+        } else {
+#pragma unroll 1
+            for (int64_t m0 = begin; m0 < end; m0 += 2 * kRows) {
+                product(s0, m0);
+                renew(in[1], s1, m0 + kRows);
+                __syncthreads();
+                product(s1, m0 + kRows);
+                renew(in[0], s0, m0 + 2 * kRows);
+                __syncthreads();
+            }
         }
     }
     float* dw = p.dw + (int64_t)blockIdx.z * p.O * p.I;
@@ -349,8 +399,9 @@ template <class E, int TO, int TI, int NT, bool TAIL> __device__ __forceinline__
 }
 
 template <class E, int TO, int TI, int NT> __global__ void __launch_bounds__(NT) k_weight_grad8(const Args p) {
-    if (blockIdx.z + 1 == gridDim.z) weight_grad8<E, TO, TI, NT, true>(p);
-    else weight_grad8<E, TO, TI, NT, false>(p);
+    if (blockIdx.z + 1 == gridDim.z) weight_grad8<E, TO, TI, NT, kTail>(p);
+    else if (__builtin_amdgcn_readfirstlane(threadIdx.x >> 6) < NT / 128) weight_grad8<E, TO, TI, NT, kStageFirst>(p);
+    else weight_grad8<E, TO, TI, NT, kMultiplyFirst>(p);
 }
 
 // out[c] = sum over the shares, in their order; dW and db in one launch
