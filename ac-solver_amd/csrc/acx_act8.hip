@@ -22,6 +22,9 @@ constexpr int kBlock = 32;
 __device__ __forceinline__ float exponent_factor(uint32_t e) { return __builtin_bit_cast(float, e == 255 ? 0x7FC00000u : e << 23); }
 
 template <int N> struct Bytes;
+template <> struct Bytes<2> {
+    typedef uint16_t type __attribute__((aligned(1)));
+};
 template <> struct Bytes<4> {
     typedef uint32_t type __attribute__((aligned(1)));
 };
@@ -91,7 +94,7 @@ template <class E, int V> __global__ void __launch_bounds__(256) k_unpack8(const
 // A workgroup owns a TO x TI tile of dW and a share of the rows, ROWS at a time: dy and q of these rows go from memory through registers into
 // LDS as the 16-byte operands of v_mfma_f32_32x32x16_bf16, 8 rows of one column each.  Columns are stored in the order in which the threads
 // bring them (column c of a vector of V stands at (c % V) TO / V + c / V): a wave's stores and its operand loads are both contiguous, and
-// the order is undone when dW is written.
+// the order is undone when dW is written (a lane's products then are neighbours in a row of dW: whole vectors are stored).
 // LDS holds two sets of rows and registers a third that is on its way from memory: a step multiplies one set and writes the next.  The two
 // waves of a SIMD take these halves in opposite order, so one's conversions (vector pipe) run under the other's products (matrix pipe).
 typedef __bf16 frag __attribute__((ext_vector_type(8)));
@@ -120,10 +123,10 @@ template <> struct Pieces<f16_t> { static constexpr int n = 2, rows = 32; };
 
 template <class E, int TO, int TI, int NT> struct Tile {
     static constexpr int kP = Pieces<E>::n, kRows = Pieces<E>::rows, kChunks = kRows / 8;
-    static constexpr int VO = kRows / 16, VI = 4;
-    static constexpr int kWaves = NT / 64, kWO = TO == 256 ? 4 : NT == 256 ? 2 : 1, kWI = kWaves / kWO;  // waves over the tile
-    static constexpr int kFO = TO / kWO / 32, kFI = TI / kWI / 32;                                       // 32 x 32 products of a wave
-    static_assert(kFO >= 1 && kFI >= 1 && kFO * kWO * 32 == TO && kFI * kWI * 32 == TI, "tile");
+    static constexpr int VO = kRows / 16, VI = TI == 64 ? 2 : 4;  // values of a load of dy and of q
+    // waves over the tile, 32 x 32 products of a wave: as many across as a load of q has values, so that a lane ends up with neighbouring columns
+    static constexpr int kWaves = NT / 64, kFI = VI, kWI = TI / 32 / kFI, kWO = kWaves / kWI, kFO = TO / kWO / 32;
+    static_assert(kFO >= 1 && kFO * kWO * 32 == TO && kFI * kWI * 32 == TI && kWO * kWI == kWaves, "tile");
     static constexpr int kItemsA = kChunks * (TO / VO), kItemsB = kChunks * (TI / VI);
     static constexpr int kPerA = (kItemsA + NT - 1) / NT, kPerB = (kItemsB + NT - 1) / NT;
     static constexpr int kSet = (kP * TO + TI) * kChunks;  // 16-byte operands of a set
@@ -137,10 +140,11 @@ enum { kTail, kStageFirst, kMultiplyFirst };
 template <class E, int TO, int TI, int NT, int PART> __device__ __forceinline__ void weight_grad8(const Args& p) {
     using T = Tile<E, TO, TI, NT>;
     constexpr bool TAIL = PART == kTail;
-    asm volatile("; part %0" ::"n"(PART));  // (unlike each other from here on: nothing of one is moved in front of the branch between them)
     constexpr int kP = T::kP, kRows = T::kRows, kChunks = T::kChunks, VO = T::VO, VI = T::VI, kFO = T::kFO, kFI = T::kFI;
     extern __shared__ u32x4 s_mem[];  // two sets of [piece][chunk][TO], [chunk][TI]
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    int tid = threadIdx.x;
+    asm volatile("; part %1" : "+v"(tid) : "n"(PART));  // (the parts have nothing in common from here on that would be worked out, and held, in front of the branch between them)
+    const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int o0 = blockIdx.x * TO, i0 = blockIdx.y * TI;
     const int64_t begin = TAIL ? p.whole : (int64_t)blockIdx.z * p.share, end = TAIL ? p.M : begin + p.share < p.whole ? begin + p.share : p.whole;
     // two steps on their way from memory
@@ -163,7 +167,7 @@ template <class E, int TO, int TI, int NT, int PART> __device__ __forceinline__ 
         const int item = tid + k * NT, chunk = item / (TI / VI), i = i0 + item % (TI / VI) * VI;
         const bool on = item < T::kItemsB;
         off_b[k] = on && i < p.I ? (uint32_t)(chunk * 8) * (uint32_t)p.I + (uint32_t)i : 0;
-        // (the eight lanes of a block of features bring the exponents of one row each, those behind the last feature too)
+        // (eight neighbouring lanes read the same block of features: they bring the exponents of one row each, those behind the last feature too)
         off_e[k] = on && i / kBlock < p.nb ? (uint32_t)(chunk * 8 + (tid & 7)) * (uint32_t)p.nb + (uint32_t)(i / kBlock) : 0;
     }
     auto fetch = [&](Rows& to, int64_t m0) {
@@ -176,7 +180,7 @@ template <class E, int TO, int TI, int NT, int PART> __device__ __forceinline__ 
 #pragma unroll
             for (int k = 0; k < T::kPerA; k++) to.a[k][r] = *(const typename Vec<E, VO>::type*)(dy + off_a[k]);
 #pragma unroll
-            for (int k = 0; k < T::kPerB; k++) to.b[k][r] = *(const typename Bytes<4>::type*)(q + off_b[k]);
+            for (int k = 0; k < T::kPerB; k++) to.b[k][r] = *(const typename Bytes<VI>::type*)(q + off_b[k]);
             dy += p.dy_sn * (int64_t)sizeof(E), q += p.I;
         }
     };
@@ -304,7 +308,7 @@ template <class E, int TO, int TI, int NT, int PART> __device__ __forceinline__ 
             const int chunk = 2 * ks + (lane >> 5), col = lane & 31;
             frag fb[kFI];
 #pragma unroll
-            for (int y = 0; y < kFI; y++) fb[y] = __builtin_bit_cast(frag, sB[chunk * TI + (wi * kFI + y) * 32 + col]);
+            for (int y = 0; y < kFI; y++) fb[y] = __builtin_bit_cast(frag, sB[chunk * TI + y * (TI / VI) + wi * 32 + col]);
 #pragma unroll
             for (int piece = kP - 1; piece >= 0; piece--) {
 #pragma unroll
@@ -367,16 +371,16 @@ template <class E, int TO, int TI, int NT, int PART> __device__ __forceinline__ 
         }
     }
     float* dw = p.dw + (int64_t)blockIdx.z * p.O * p.I;
+    const int i = i0 + (wi * 32 + (lane & 31)) * VI;
 #pragma unroll
     for (int x = 0; x < kFO; x++)
 #pragma unroll
-        for (int y = 0; y < kFI; y++) {
-            const int ui = (wi * kFI + y) * 32 + (lane & 31), i = i0 + ui % (TI / VI) * VI + ui / (TI / VI);
+        for (int r = 0; r < 16; r++) {
+            const int uo = (wo * kFO + x) * 32 + (r & 3) + 8 * (r >> 2) + 4 * (lane >> 5), o = o0 + uo % (TO / VO) * VO + uo / (TO / VO);
+            float v[VI];
 #pragma unroll
-            for (int r = 0; r < 16; r++) {
-                const int uo = (wo * kFO + x) * 32 + (r & 3) + 8 * (r >> 2) + 4 * (lane >> 5), o = o0 + uo % (TO / VO) * VO + uo / (TO / VO);
-                if (o < p.O && i < p.I) dw[(int64_t)o * p.I + i] = acc[x][y][r];
-            }
+            for (int y = 0; y < VI; y++) v[y] = acc[x][y][r];
+            if (o < p.O) store_some<float, VI>(dw + (int64_t)o * p.I + i, p.I - i, v);
         }
     if (p.db && blockIdx.y == 0) {
         float* s = (float*)s_mem;  // [chunk][TO]
@@ -404,23 +408,32 @@ template <class E, int TO, int TI, int NT> __global__ void __launch_bounds__(NT)
     else weight_grad8<E, TO, TI, NT, kMultiplyFirst>(p);
 }
 
-// out[c] = sum over the shares, in their order; dW and db in one launch
-__global__ void __launch_bounds__(256) k_join_shares(const float* __restrict__ dw, const float* __restrict__ db, int n, int64_t size, int O, float* __restrict__ out, float* __restrict__ out_db) {
-    const int64_t c = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    const bool bias = c >= size;
-    if (c >= size + (db ? O : 0)) return;
-    const float* src = bias ? db + (c - size) : dw + c;
-    const int64_t step = bias ? O : size;
-    float a[8] = {};
-    int k = 0;
-    for (; k + 8 <= n; k += 8) {
+// out[c] = sum over the shares, in a fixed order; dW and db in one launch.  64 columns a workgroup, four a lane, 16 threads over the shares.
+__global__ void __launch_bounds__(256) k_join_shares(const float* __restrict__ dw, const float* __restrict__ db, int n, int64_t size, int O, int64_t dw_groups, float* __restrict__ out,
+                                                     float* __restrict__ out_db) {
+    __shared__ float s[16][65];
+    const bool bias = blockIdx.x >= dw_groups;
+    const float* src = bias ? db : dw;
+    const int64_t columns = bias ? O : size, c0 = (blockIdx.x - (bias ? dw_groups : 0)) * 64;
+    const int q = threadIdx.x & 15, part = threadIdx.x >> 4;
+    const int valid = columns - c0 - q * 4 > 4 ? 4 : (int)(columns - c0 - q * 4);
+    float a[4] = {};
+#pragma unroll 8
+    for (int k = part; k < n; k += 16) {
+        float v[4];
+        load_some<float, 4>(src + k * columns + c0 + q * 4, valid, v);
 #pragma unroll
-        for (int i = 0; i < 8; i++) a[i] += src[(k + i) * step];
+        for (int i = 0; i < 4; i++) a[i] += v[i];
     }
-    for (; k < n; k++) a[k & 7] += src[k * step];
-    const float v = ((a[0] + a[1]) + (a[2] + a[3])) + ((a[4] + a[5]) + (a[6] + a[7]));
-    if (bias) out_db[c - size] = v;
-    else out[c] = v;
+#pragma unroll
+    for (int i = 0; i < 4; i++) s[part][q * 4 + i] = a[i];
+    __syncthreads();
+    if (threadIdx.x < 64 && c0 + threadIdx.x < columns) {
+        float v = 0.0f;
+#pragma unroll
+        for (int k = 0; k < 16; k++) v += s[k][threadIdx.x];
+        (bias ? out_db : out)[c0 + threadIdx.x] = v;
+    }
 }
 
 struct Plan {
@@ -431,13 +444,18 @@ static Plan plan_of(int64_t M, int64_t O, int64_t I) {
     constexpr int kStep = 64;  // rows of a step of every type divide it
     Plan p;
     p.to = O <= 64 ? 64 : 256;
-    p.ti = I <= 64 ? 64 : 256;
+    p.ti = p.to == 64 || I > 128 ? 256 : I <= 64 ? 64 : 128;
     p.go = (O + p.to - 1) / p.to;
     p.gi = (I + p.ti - 1) / p.ti;
     p.whole = M >= 4 ? (M - 4) / kStep * kStep : 0;  // behind these rows at least four more: a vector of up to four values that starts in them ends in bounds
-    int64_t want = 256 / (p.go * p.gi) - 1;
+    // A share costs its step's time, ~1.3 us where the chip is not full, and 8 O I bytes of partial sums written and read again at ~4.7 TB/s: n shares of
+    // `steps` cost steps / n * 1.3 us + n * 8 O I / 4.7e12 s, least at n^2 = steps * 764000 / (O I).  (65540 x 256 x 256 bf16: 64 us with 256 shares,
+    // 33 with the 109 of this rule.)  No more than the chip takes at once.
+    const int64_t steps = p.whole / kStep, most = 256 / (p.go * p.gi) - 1;
+    int64_t want = (int64_t)__builtin_sqrt((double)steps * 764000.0 / ((double)O * (double)I));
+    if (want > most) want = most;
     if (want < 1) want = 1;
-    const int64_t steps = p.whole / kStep, per = (steps + want - 1) / want;
+    const int64_t per = (steps + want - 1) / want;
     p.share = (per < 4 ? 4 : per) * kStep;
     p.shares = (p.whole + p.share - 1) / p.share + 1;  // and the rows behind them
     return p;
@@ -520,15 +538,16 @@ extern "C" int acx_act8_weight_grad(const void* d_out_grad, int64_t o_row, int d
     elem::with_element(dtype, [&](auto* e) {
         using E = std::remove_pointer_t<decltype(e)>;
         const hipStream_t st = (hipStream_t)stream;
-        if (p.to == 64 && p.ti == 64) err = act8::launch<E, 64, 64, 256>(a, p, st);
-        else if (p.to == 64) err = act8::launch<E, 64, 256, 512>(a, p, st);
+        if (p.to == 64) err = act8::launch<E, 64, 256, 256>(a, p, st);
         else if (p.ti == 64) err = act8::launch<E, 256, 64, 512>(a, p, st);
+        else if (p.ti == 128) err = act8::launch<E, 256, 128, 512>(a, p, st);
         else err = act8::launch<E, 256, 256, 512>(a, p, st);
     });
     ACX_HIP_TRY(err);
     if (need) {
-        const int64_t columns = O * I + (d_bias_grad ? O : 0);
-        hipLaunchKernelGGL(act8::k_join_shares, dim3((unsigned)((columns + 255) / 256)), dim3(256), 0, (hipStream_t)stream, a.dw, a.db, (int)p.shares, O * I, (int)O, d_weight_grad, d_bias_grad);
+        const int64_t groups = (O * I + 63) / 64;
+        hipLaunchKernelGGL(act8::k_join_shares, dim3((unsigned)(groups + (d_bias_grad ? (O + 63) / 64 : 0))), dim3(256), 0, (hipStream_t)stream, a.dw, a.db, (int)p.shares, O * I, (int)O,
+                           groups, d_weight_grad, d_bias_grad);
         ACX_HIP_TRY(hipGetLastError());
     }
     return ACX_OK;
