@@ -1,6 +1,8 @@
 """Activations kept in 8 bits for the backward pass, and the weight gradient that reads them as they are: `acx_act8_pack` / `_unpack` /
 `_weight_grad` (csrc/acx_act8.hip).  Opt-in (`--checkpoint-8bit` of ac_solver.agents.ppo); the reference keeps float32 activations
 (ac_solver/agents/ppo_agent.py:11-109, agents/training.py:273-330)."""
+import threading
+
 import torch
 from torch.nn import functional as F
 
@@ -123,20 +125,34 @@ class _Packed:
 
 
 MIN_VALUES = 1 << 12
+_inside = threading.local()
+
+
+def packing():
+    """whether this thread is inside a `checkpoint8` block (for functions that keep tensors which autograd does not know)"""
+    return getattr(_inside, "depth", 0) > 0
 
 
 class checkpoint8(torch.autograd.graph.saved_tensors_hooks):
     """`with checkpoint8(): ...` -- what autograd keeps of the activations computed inside the block is kept in 8 bits (pack8) and restored
-    in the backward pass: a quarter (float32) or half (16 bits) of the memory; the gradients are those of the restored values.  Leaves
-    (parameters, inputs that require no gradient), vectors, tensors of fewer than 4096 values and whole numbers are kept as they are, and
-    so is a float32 state that the caller needs exactly: pass it in as a leaf."""
+    in the backward pass: a quarter (float32) or half (16 bits) of the memory; the gradients are those of the restored values (row
+    statistics and states that an operator kept beside them stay what they were).  Kept as they are: leaves (parameters, inputs),
+    vectors, tensors of fewer than 4096 values, whole numbers, tensors on the CPU."""
 
     def __init__(self):
         super().__init__(self._keep, self._restore)
 
+    def __enter__(self):
+        _inside.depth = getattr(_inside, "depth", 0) + 1
+        return super().__enter__()
+
+    def __exit__(self, *exc):
+        _inside.depth -= 1
+        return super().__exit__(*exc)
+
     @staticmethod
     def _keep(t):
-        if t.dtype not in T.DTYPES or t.device.type != "cuda" or t.dim() < 2 or t.numel() < MIN_VALUES or t.grad_fn is None:
+        if t.dtype not in T.DTYPES or not t.is_cuda or t.dim() < 2 or t.numel() < MIN_VALUES or t.grad_fn is None:
             return t
         return _Packed(t)
 

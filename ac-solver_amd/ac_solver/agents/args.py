@@ -50,6 +50,12 @@ _FLAGS = [
     ("--tile-initial-states", "bool", False, "allow more environments than initial states: environment i starts from state i mod n"),
     ("--supermoves", str, "", "opt-in supermoves, e.g. '11,4,2;0,1': action 12 + s runs the s-th ';'-separated list of base moves as one step "
                                "(the reference's --use_supermoves has no implementation to follow: it raises NotImplementedError, here too)"),
+    # an agent with a memory (agents/recurrent_agent.py); not in the reference, whose --nodes-counts MLPs stay the default
+    ("--recurrent", "bool", False, "train an agent of gated recurrent blocks over the steps of an episode instead of the MLPs"),
+    ("--recurrent-width", int, 256, "features of the recurrent agent's blocks"),
+    ("--recurrent-blocks", int, 2, "number of the recurrent agent's blocks"),
+    ("--recurrent-dtype", str, "float32", "type of the recurrent agent's activations: float32 or bfloat16"),
+    ("--checkpoint-8bit", "bool", False, "the recurrent agent keeps its activations in 8 bits for the backward pass"),
     ("--fused-policy", "bool", False, "rollouts sample through the fused MFMA policy kernel (bf16 operands, f32 accumulation) instead of the f32 torch modules"),
 ]
 
@@ -78,4 +84,7 @@ def parse_args(argv=None):
     assert 0.0 <= args.warmup_period <= 1.0, "warmup period should be less than 1.0 as it is the fraction of total timesteps"
     assert args.lr_decay in ["linear", "cosine"], f"lr-decay must be linear or cosine, not {args.lr_decay}. Other LR schedules not supported yet"
     assert 0.0 <= args.min_lr_frac <= 1.0, "min-lr-frac is the fraction of maximum lr to which we anneal."
+    assert args.recurrent_dtype in ["float32", "bfloat16"], f"recurrent-dtype must be float32 or bfloat16, not {args.recurrent_dtype}"
+    assert not (args.recurrent and args.fused_policy), "the fused policy kernel evaluates the MLP agent: not with --recurrent"
+    assert args.recurrent or not args.checkpoint_8bit, "--checkpoint-8bit is an option of --recurrent"
     return args

@@ -38,7 +38,12 @@ def train_ppo(argv=None):
     torch.backends.cudnn.deterministic = args.torch_deterministic
 
     envs, initial_states, curr_states, success_record, ACMoves_hist, states_processed = get_env(args, device=device, rank=rank, world=world)
-    agent = Agent(envs, args.nodes_counts).to(device)
+    if args.recurrent:
+        from ac_solver.agents.recurrent_agent import RecurrentAgent
+
+        agent = RecurrentAgent(envs, args.recurrent_width, args.recurrent_blocks, args.recurrent_dtype, args.checkpoint_8bit).to(device)
+    else:
+        agent = Agent(envs, args.nodes_counts).to(device)
     if world > 1:  # identical initial weights on every rank
         for p in agent.parameters():
             torch.distributed.broadcast(p.data, 0)

@@ -1,10 +1,12 @@
 """The gated recurrence of the recurrent agent over a rollout [steps, environments, features], with its gradient: `acx_scan_forward` /
-`acx_scan_backward` (csrc/acx_scan.hip).  The reference's agent has no memory (ac_solver/agents/ppo_agent.py:11-109)."""
+`acx_scan_backward` (csrc/acx_scan.hip); a block of the agent made of it and its end (block_norm), over a rollout and, in one launch,
+for a single step (`acx_block_step`, csrc/acx_block.hip).  The reference's agent has no memory (ac_solver/agents/ppo_agent.py:11-109)."""
 import torch
 
 from ac_solver import _acx
 from ac_solver.agents import _tensors as T
-from ac_solver.agents.block_norm import MAX_WIDTH
+from ac_solver.agents import activation8
+from ac_solver.agents.block_norm import MAX_WIDTH, block_output_backward, block_output_forward
 
 
 def _operands(candidate, gate, reset, state):
@@ -98,6 +100,54 @@ def gated_scan(candidate, gate, reset=None, state=None):
     -> (hidden [steps, rows, features] of the activations' type, last state [rows, features] float32); both differentiable (once) with
     respect to candidate, gate and state."""
     return _GatedScan.apply(candidate, gate, reset, state)
+
+
+class _RecurrentBlock(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, projected, reset, state, weight, scale, next_weight, eps):
+        width = x.shape[-1]
+        candidate, gate, out_gate = (projected[..., k * width:(k + 1) * width] for k in range(3))
+        save = any(ctx.needs_input_grad)
+        hidden, last, bounds = gated_scan_forward(candidate, gate, reset, state, save=save)
+        new, u, stats = block_output_forward(x, hidden, out_gate, weight, scale, next_weight, eps, save=save)
+        if save:
+            # (autograd packs x and projected itself inside checkpoint8; hidden is nobody's input)
+            ctx.packed = activation8.packing() and hidden.numel() >= activation8.MIN_VALUES
+            kept = activation8.pack8(hidden) if ctx.packed else (hidden,)
+            ctx.save_for_backward(x, projected, reset, weight, scale, next_weight, bounds, stats, *kept)
+        ctx.set_materialize_grads(False)
+        return new, u, last
+
+    @staticmethod
+    @T.once
+    def backward(ctx, d_new, d_u, d_last):
+        if d_new is None and d_u is None and d_last is None:
+            return (None,) * 8
+        x, projected, reset, weight, scale, next_weight, bounds, stats, *kept = ctx.saved_tensors
+        hidden = activation8.unpack8(*kept, x.dtype) if ctx.packed else kept[0]
+        width = x.shape[-1]
+        thirds = lambda t: [t[..., k * width:(k + 1) * width] for k in range(3)]  # noqa: E731
+        candidate, gate, out_gate = thirds(projected)
+        d_projected = torch.empty(projected.shape, dtype=projected.dtype, device=projected.device)
+        d_candidate, d_gate, d_out_gate = thirds(d_projected)
+        dx, d_hidden, _, dw, ds, dn = block_output_backward(d_new, d_u, x, hidden, out_gate, weight, scale, next_weight, stats, d_gate_out=d_out_gate)
+        _, _, d_state = gated_scan_backward(d_hidden, d_last, candidate, gate, reset, bounds, want_state=ctx.needs_input_grad[3], out=(d_candidate, d_gate))
+        grads = (dx, d_projected, None, d_state, dw, ds, dn)
+        return tuple(g if need else None for g, need in zip(grads, ctx.needs_input_grad)) + (None,)
+
+
+def recurrent_block(x, projected, state, weight, scale=None, next_weight=None, reset=None, eps=1e-6):
+    """A block of the recurrent agent over a rollout, differentiable (once): with candidate, gate, output gate = the three thirds of projected
+    [steps, rows, 3 width] (a projection of the block's normalised input),
+
+        hidden, last = gated_scan(candidate, gate, reset, state);  new, u = block_output(x, hidden, output gate, weight, scale, next_weight, eps)
+
+    -> (new, u, last): the residual stream behind the block, its norm for the next one (None without `next_weight`), the last state.  The
+    gradient of `projected` is written in place by the two operators, without a copy of its thirds."""
+    if not isinstance(x, torch.Tensor) or x.dim() != 3:
+        raise ValueError("x has to be [steps, rows, features]")
+    T.activation(projected, "projected", like=T.activation(x, "x"), shape=x.shape[:-1] + (3 * x.shape[-1],))
+    return _RecurrentBlock.apply(x, projected, reset, state, weight, scale, next_weight, eps)
 
 
 def recurrent_step(x, projected, state, weight, scale=None, next_weight=None, reset=None, next_state=None, eps=1e-6):

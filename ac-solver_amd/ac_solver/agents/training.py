@@ -422,6 +422,12 @@ def ppo_training_loop(envs, args, device, optimizer, agent, curr_states, success
     round1_complete = False
     beta = None if args.is_loss_clip else args.beta
     params = list(agent.parameters())
+    # an agent with a memory (agents/recurrent_agent.py): its states, and where episodes start (done OR truncated: the memory ends with both)
+    recurrent = bool(getattr(agent, "is_recurrent", False))
+    if recurrent:
+        assert N % args.num_minibatches == 0, "a recurrent agent's minibatches are whole environments: num_envs has to be a multiple of num_minibatches"
+        memory = agent.initial_state(N, device)
+        starts = torch.ones((T + 1, N), dtype=torch.bool, device=device)
     fused = None
     if fused_on:  # opt-in: rollout inference on the matrix cores (agents/fused_policy.py); the update stays f32 torch
         from ac_solver.agents.fused_policy import FusedPolicy
@@ -451,7 +457,8 @@ def ppo_training_loop(envs, args, device, optimizer, agent, curr_states, success
             pass
     stats = {}
     stats_stream = _StatsStream(agent, device, int(os.environ.get("ACX_PPO_STATS_GROUP", "4"))) if fused_on and os.environ.get("ACX_PPO_STATS_STREAM", "1") != "0" else None
-    order = _MinibatchOrder(args.batch_size, args.update_epochs, device)
+    # (a recurrent agent's minibatches are environments with all their steps)
+    order = _MinibatchOrder(N if recurrent else args.batch_size, args.update_epochs, device)
     ph = _Phases(device)
     n_updates_done = 0
 
@@ -472,6 +479,8 @@ def ppo_training_loop(envs, args, device, optimizer, agent, curr_states, success
         try:  # (whatever the rollout raises, the generator state goes back into `random`: a caller that catches and continues must not find it stale)
             if fused is not None:
                 fused.refresh()  # the weights of the last update
+            if recurrent:
+                memory_before = memory.clone()
 
             # ---------------------------------------------------------------- rollout (device resident) ----
             for step in range(T):
@@ -481,6 +490,9 @@ def ppo_training_loop(envs, args, device, optimizer, agent, curr_states, success
                     action = actions[step]
                     if stats_stream is not None:  # rows up to `step` are final: their f32 behaviour statistics start on the second stream
                         stats_stream.rows_final(step + 1, obs, actions, logprobs, values, last=step == T - 1)
+                elif recurrent:
+                    action, logprob, value = agent.act(obs[step], starts[step], memory)
+                    actions[step], logprobs[step], values[step] = action, logprob, value
                 else:
                     with torch.no_grad():
                         action, logprob, _, value = agent.get_action_and_value(obs[step])
@@ -496,6 +508,8 @@ def ppo_training_loop(envs, args, device, optimizer, agent, curr_states, success
                 ep_return += rewards[step]
                 ep_length += 1
                 fin = term[step + 1] | trunc
+                if recurrent:
+                    starts[step + 1] = fin
                 # ---- episodes ended: bookkeeping of the reference (training.py:167-224) on the finished envs only ----
                 # two read-backs per step: how many (the size of `idx`), then index, done flag, return and length of each in one block
                 idx = torch.nonzero(fin).flatten()
@@ -571,8 +585,13 @@ def ppo_training_loop(envs, args, device, optimizer, agent, curr_states, success
             else:
                 refresh_behaviour_stats(agent, obs, actions, logprobs, values)
             ph.lap("behaviour stats (f32)")
+        if recurrent and agent.dtype != torch.float32:
+            # the rollout's steps keep the memory in float32 where a whole pass rounds it to the activations' type: the importance ratio is formed
+            # against what the update's own pass gives for the unchanged weights
+            with torch.no_grad():
+                logprobs, _, values = (t.view(T, N) for t in agent.evaluate(obs[:T], actions, starts[:T], memory_before))
         with torch.no_grad():
-            next_value = agent.get_value(obs[T].float()).reshape(-1)
+            next_value = (agent.get_value(obs[T].float(), starts[T], memory) if recurrent else agent.get_value(obs[T].float())).reshape(-1)
             advantages, returns = compute_gae(rewards, values, dones[:T], next_value, dones[T], args.gamma, args.gae_lambda)
 
         ph.lap("gae")
@@ -585,8 +604,13 @@ def ppo_training_loop(envs, args, device, optimizer, agent, curr_states, success
         clipfracs = []
         for epoch in range(args.update_epochs):
             for start in range(0, args.batch_size, args.minibatch_size):
-                mb = perms[epoch, start:start + args.minibatch_size]
-                _, newlogprob, entropy, newvalue = agent.get_action_and_value(b_obs[mb].float(), b_actions[mb])
+                if recurrent:
+                    some = perms[epoch, start // T:start // T + N // args.num_minibatches]  # environments
+                    mb = (torch.arange(T, device=device).unsqueeze(1) * N + some).reshape(-1)
+                    newlogprob, entropy, newvalue = agent.evaluate(obs[:T, some].float(), actions[:, some], starts[:T, some], memory_before[:, some])
+                else:
+                    mb = perms[epoch, start:start + args.minibatch_size]
+                    _, newlogprob, entropy, newvalue = agent.get_action_and_value(b_obs[mb].float(), b_actions[mb])
                 logratio = newlogprob - b_logprobs[mb]
                 ratio = logratio.exp()
                 kl_var = (ratio - 1) - logratio  # E[kl_var] approximates KL(pi_old || pi)
@@ -630,6 +654,8 @@ def ppo_training_loop(envs, args, device, optimizer, agent, curr_states, success
         # the next rollout continues where this one stopped
         obs[0].copy_(obs[T])
         term[0].copy_(term[T])
+        if recurrent:
+            starts[0].copy_(starts[T])
 
         # explained variance on the device (np.var's population variance, as the reference computes it on host copies: two 16 MB
         # read-backs per update at BASELINE config 5's shape, 20 ms)
@@ -664,6 +690,7 @@ def ppo_training_loop(envs, args, device, optimizer, agent, curr_states, success
                 "entropy_loss": entropy_loss.item(), "approx_kl": approx_kl.item(), "explained_var": explained_var,
                 "clipfrac": stats["losses/clipfrac"], "global_step": global_step, "round1_complete": round1_complete,
                 "curr_states": curr_states, "states_processed": states_processed, "ACMoves_hist": ACMoves_hist,
+                **({"recurrent": agent.state_dict()} if recurrent else {}),
                 "supermoves": ({12 + k: q for k, q in enumerate(envs.supermoves)} if getattr(envs, "supermoves", None) else None),
             }
             print(f"saving checkpoint to {out_dir}")

@@ -127,3 +127,33 @@ def test_8_bit_checkpoints_refuse_what_they_cannot_read():
         out = torch.tanh(a * 1.0).sum()
     out.backward()
     assert torch.allclose(a.grad, 1 - torch.tanh(a.detach()) ** 2)
+
+
+def test_arguments_of_the_recurrent_agent():
+    from ac_solver.agents.args import parse_args
+
+    a = parse_args(["--recurrent", "--recurrent-width", "64", "--recurrent-blocks", "3", "--recurrent-dtype", "bfloat16", "--checkpoint-8bit"])
+    assert a.recurrent and (a.recurrent_width, a.recurrent_blocks, a.recurrent_dtype, a.checkpoint_8bit) == (64, 3, "bfloat16", True)
+    d = parse_args([])
+    assert not d.recurrent and not d.checkpoint_8bit
+    for bad in (["--recurrent", "--fused-policy"], ["--checkpoint-8bit"], ["--recurrent", "--recurrent-dtype", "float64"]):
+        with pytest.raises(AssertionError):
+            parse_args(bad)
+
+
+def test_the_recurrent_agent_needs_a_gpu_and_says_so():
+    from types import SimpleNamespace
+
+    from ac_solver.agents.recurrent_agent import RecurrentAgent
+
+    spaces = SimpleNamespace(single_observation_space=SimpleNamespace(shape=(50,)), single_action_space=SimpleNamespace(n=12))
+    agent = RecurrentAgent(spaces, 32, 2)
+    assert sum(p.numel() for p in agent.parameters()) == 50 * 32 + 32 + 2 * (3 * 32 * 32 + 3 * 32 + 3 * 32) + 32 + 32 * 12 + 12 + 32 + 1
+    with pytest.raises(ValueError, match="GPU"):
+        agent.act(torch.zeros(4, 50), torch.zeros(4, dtype=torch.bool), agent.initial_state(4))
+    with pytest.raises(ValueError, match="at least one"):
+        RecurrentAgent(spaces, 32, 0)
+    with pytest.raises(ValueError, match="steps, rows, features"):
+        R.recurrent_block(torch.zeros(4, 8), torch.zeros(4, 24), None, torch.ones(8))
+    with pytest.raises(ValueError, match="projected has the shape"):
+        R.recurrent_block(torch.zeros(2, 4, 8), torch.zeros(2, 4, 16), None, torch.ones(8))
