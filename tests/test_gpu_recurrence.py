@@ -255,3 +255,60 @@ def test_a_captured_pass_replays():
         wg = gated_scan_backward(dh, dl, c, z, r, want[2])
         for a, b in zip((hidden, last, bounds) + grads, want + wg):
             assert torch.equal(a, b)
+
+
+def test_the_gradient_of_the_gradient_is_refused_not_zero():
+    import torch
+
+    from ac_solver.agents.block_norm import block_output
+    from ac_solver.agents.recurrence import gated_scan, recurrent_block
+
+    c, z, r, s, dh, dl = inputs(6, 2, 8, "float32", 2)
+    leaves = [t.clone().requires_grad_() for t in (c, z)]
+    w = torch.ones(8, device="cuda", requires_grad=True)
+    p = torch.cat((c, z, dh), dim=-1).requires_grad_()
+    for out, wrt in ((gated_scan(*leaves)[0], leaves), (block_output(leaves[0], leaves[1], None, w, w, w)[1], leaves + [w]),
+                     (recurrent_block(leaves[0], p, None, w, w, w)[1], [leaves[0], p, w])):
+        first = torch.autograd.grad(out.square().sum(), wrt, create_graph=True)
+        assert all(g.requires_grad for g in first)
+        with pytest.raises(RuntimeError, match="again"):
+            torch.autograd.grad(sum(g.sum() for g in first), wrt)
+
+
+def test_two_threads_at_once():
+    """calls from two host threads on streams of their own: the interpreter's lock is not held meanwhile, scratch memory is each call's own"""
+    import threading
+
+    import torch
+
+    from ac_solver.agents.recurrence import gated_scan
+
+    jobs = [inputs(4100, 2, 66, "float32", k) for k in range(2)]
+
+    def run(c, z, r, s, dh, dl):
+        leaves = [t.clone().requires_grad_() for t in (c, z, s)]
+        h, last = gated_scan(leaves[0], leaves[1], reset=r, state=leaves[2])
+        return [h.detach(), last.detach(), *torch.autograd.grad((h, last), leaves, (dh, dl))]
+
+    want = [run(*j) for j in jobs]
+    torch.cuda.synchronize()
+    bad = []
+
+    def work(k):
+        try:
+            stream = torch.cuda.Stream()
+            with torch.cuda.stream(stream):
+                for _ in range(20):
+                    got = run(*jobs[k])
+                    stream.synchronize()
+                    if not all(torch.equal(a, b) for a, b in zip(got, want[k])):
+                        bad.append(k)
+        except BaseException as e:  # noqa: BLE001
+            bad.append(e)
+
+    threads = [threading.Thread(target=work, args=(k,)) for k in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not bad, bad

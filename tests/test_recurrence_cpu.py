@@ -126,7 +126,8 @@ def test_8_bit_checkpoints_refuse_what_they_cannot_read():
         a = torch.randn(100, 100, requires_grad=True)
         out = torch.tanh(a * 1.0).sum()
     out.backward()
-    assert torch.allclose(a.grad, 1 - torch.tanh(a.detach()) ** 2)
+    # (values up to 1, a product and a difference on either side: four roundings of at most 2^-24)
+    assert float((a.grad - (1 - torch.tanh(a.detach()) ** 2)).abs().max()) <= 2.0 ** -22
 
 
 def test_arguments_of_the_recurrent_agent():
