@@ -271,8 +271,10 @@ def test_the_gradient_of_the_gradient_is_refused_not_zero():
                      (recurrent_block(leaves[0], p, None, w, w, w)[1], [leaves[0], p, w])):
         first = torch.autograd.grad(out.square().sum(), wrt, create_graph=True)
         assert all(g.requires_grad for g in first)
+        with pytest.raises(RuntimeError):  # (the leaves are not reached at all)
+            torch.autograd.grad(sum(g.sum() for g in first), wrt, retain_graph=True)
         with pytest.raises(RuntimeError, match="again"):
-            torch.autograd.grad(sum(g.sum() for g in first), wrt)
+            sum(g.sum() for g in first).backward()
 
 
 def test_two_threads_at_once():
