@@ -19,7 +19,7 @@ for p in (PKG, ROOT):
 def _ensure_native_built():
     """The suite needs libacx.so (cross-compiled by hipcc, no GPU required) and the oracle; build them once if a
     fresh checkout has not run __graft_entry__.build() yet."""
-    if not os.path.exists(os.path.join(PKG, "lib", "libacx.so")) or not os.path.exists(os.path.join(PKG, "lib", "acx_torch.so")) or not os.path.exists(os.path.join(ROOT, "oracle", "libac_oracle.so")):
+    if not os.path.exists(os.path.join(PKG, "lib", "libacx.so")) or not os.path.exists(os.path.join(ROOT, "oracle", "libac_oracle.so")):
         import __graft_entry__
 
         __graft_entry__.build()
