@@ -38,7 +38,7 @@ template <class E, int V> __global__ void __launch_bounds__(256) k_pack8(const E
     const int64_t row = l / lpr;
     const int j = (int)(l - row * lpr), d = j * V, valid = row < M ? K - d : 0;
     float v[V];
-    load_some<E, V>(x + row * x_sn + d, valid, v);
+    load_some<E, V>(x + row * x_sn + d, valid, v, row * x_sn + d <= (M - 1) * x_sn + (K - V));
     uint32_t top = 0;
 #pragma unroll
     for (int i = 0; i < V; i++) {

@@ -5,8 +5,8 @@
 //
 // Forward: 3 rows read, 2 written, two row sums; backward: 5 read, 3 written, two row sums, and three sums over all rows (the gradients
 // of weight, scale and next_weight).  About 50 vector instructions per element: bound by HBM.
-//   - A row belongs to LR neighbouring lanes that hold all of it in registers, R vectors of V elements each (16 bytes a load); narrow rows
-//     share a wave, rows over 64 lanes take a workgroup (row sums through LDS).
+//   - A row belongs to LR neighbouring lanes that hold all of it in registers, a vector of V elements each (16 bytes a load); narrow rows share a
+//     wave, a row over 64 lanes takes a workgroup of as many waves as it needs (row sums through LDS).
 //   - The backward pass recomputes `new` from x, y and gate (it reads them anyway) unrounded and takes the two reciprocal roots of a row
 //     from the forward pass (8 bytes a row instead of two more row sums).
 //   - Sums over rows: every lane adds its features over the rows that its workgroup walks, the workgroup's row groups join in LDS, and a second
@@ -42,18 +42,26 @@ struct Args {
     float* partial;                  // [workgroups, 3, D]
 };
 
-// sum over the LR lanes of a row, in every one of them (s_red: one float per wave of the workgroup)
+// V elements of row `row` from feature d on; the vector may end behind the row where the tensor goes on that far
+template <class E, int V> __device__ __forceinline__ typename Vec<E, V>::type load_row(const Args& p, const void* base, int64_t sn, int64_t row, int d, int valid) {
+    const int64_t at = row * sn + d;
+    return load_raw<E, V>((const E*)base + at, valid, at <= (p.M - 1) * sn + (p.D - V));
+}
+
+// LR > 64 stands for rows of a workgroup: LR is then the largest workgroup of the variant, and blockDim.x lanes have the row.
+template <int LR> constexpr int kThreads = LR > 64 ? LR : 256;
+template <int LR> constexpr int kRows = LR > 64 ? 1 : 256 / LR;  // rows that a workgroup holds at a time
+
+// sum over the lanes of a row, in every one of them (s_red: one float per wave of the workgroup)
 template <int LR> __device__ __forceinline__ float row_sum(float v, float* s_red) {
     v = lane_sum<(LR < 64 ? LR : 64)>(v);
     if constexpr (LR > 64) {
-        constexpr int kWaves = LR / 64;
         __syncthreads();  // (the sums of the last call have been read)
         if ((threadIdx.x & 63) == 0) s_red[threadIdx.x >> 6] = v;
         __syncthreads();
+        const int waves = blockDim.x >> 6;
         v = 0.0f;
-        const float* mine = s_red + threadIdx.x / LR * kWaves;
-#pragma unroll
-        for (int i = 0; i < kWaves; i++) v += mine[i];
+        for (int i = 0; i < waves; i++) v += s_red[i];
     }
     return v;
 }
@@ -63,85 +71,67 @@ template <int V> __device__ __forceinline__ void load_weight(const float* p, int
     for (int i = 0; i < V; i++) out[i] = p && d + i < D ? p[d + i] : fallback;
 }
 
-template <class E, int V, int LR, int R, bool STEP> __global__ void __launch_bounds__(LR > 256 ? LR : 256) k_block_fwd(const Args p) {
+template <class E, int V, int LR, bool STEP> __global__ void __launch_bounds__(kThreads<LR>) k_block_fwd(const Args p) {
     constexpr bool kPrecise = sizeof(E) == 4;
-    constexpr int kThreads = LR > 256 ? LR : 256, kRows = kThreads / LR;
-    __shared__ float s_red[kThreads / 64];
-    const int j = threadIdx.x % LR;
-    float w[R][V], scale[R][V], next[R][V];
-#pragma unroll
-    for (int r = 0; r < R; r++) {
-        const int d = (r * LR + j) * V;
-        load_weight<V>(p.w, d, p.D, 0.0f, w[r]);
-        load_weight<V>(p.scale, d, p.D, 1.0f, scale[r]);
-        load_weight<V>(p.next, d, p.D, 0.0f, next[r]);
-    }
-    for (int64_t row0 = (int64_t)blockIdx.x * kRows; row0 < p.M; row0 += (int64_t)gridDim.x * kRows) {
-        const int64_t row = row0 + threadIdx.x / LR;
+    __shared__ float s_red[kThreads<LR> / 64];
+    const int j = LR > 64 ? threadIdx.x : threadIdx.x % LR, d = j * V;
+    float w[V], scale[V], next[V];
+    load_weight<V>(p.w, d, p.D, 0.0f, w);
+    load_weight<V>(p.scale, d, p.D, 1.0f, scale);
+    load_weight<V>(p.next, d, p.D, 0.0f, next);
+    for (int64_t row0 = (int64_t)blockIdx.x * kRows<LR>; row0 < p.M; row0 += (int64_t)gridDim.x * kRows<LR>) {
+        const int64_t row = row0 + (LR > 64 ? 0 : threadIdx.x / LR);
         const bool live = row < p.M;  // (lanes behind the last row run along for the row sums)
-        float x[R][V], y[R][V], g[R][V];
+        const int valid = live ? p.D - d : 0;
+        float x[V], y[V], g[V];
         float sum = 0.0f;
+        const auto x_raw = load_row<E, V>(p, p.x, p.x_sn, row, d, valid);
+        if constexpr (STEP) {
+            const E* proj = (const E*)p.proj + row * p.p_sn + d;
+            const auto c_raw = load_raw<E, V>(proj, valid, p.D >= V), z_raw = load_raw<E, V>(proj + p.D, valid, p.D >= V);  // (another third of the row follows)
+            const auto g_raw = load_row<E, V>(p, (const E*)p.proj + 2 * (int64_t)p.D, p.p_sn, row, d, valid);
+            const auto h_raw = load_row<float, V>(p, p.state, p.D, row, d, valid);
+            const bool start = live && p.reset && p.reset[row];
+            float c[V], z[V], h[V];
+            widen<E, V>(c_raw, valid, c);
+            widen<E, V>(z_raw, valid, z);
+            widen<E, V>(g_raw, valid, g);
+            widen<float, V>(h_raw, valid, h);
 #pragma unroll
-        for (int r = 0; r < R; r++) {
-            const int d = (r * LR + j) * V, valid = live ? p.D - d : 0;
-            load_some<E, V>((const E*)p.x + row * p.x_sn + d, valid, x[r]);
-            if constexpr (STEP) {
-                const E* proj = (const E*)p.proj + row * p.p_sn + d;
-                float c[V], z[V], h[V];
-                load_some<E, V>(proj, valid, c);
-                load_some<E, V>(proj + p.D, valid, z);
-                load_some<E, V>(proj + 2 * (int64_t)p.D, valid, g[r]);
-                load_some<float, V>(p.state + row * p.D + d, valid, h);
-                const bool start = live && p.reset && p.reset[row];
-#pragma unroll
-                for (int i = 0; i < V; i++) {
-                    const Sigmoid s = sigmoid_pair<kPrecise>(z[i]);
-                    y[r][i] = __builtin_fmaf(keep_of(z[i], s), start ? 0.0f : h[i], take_of(z[i], s) * c[i]);
-                }
-                store_some<float, V>(p.next_state + row * p.D + d, valid, y[r]);
-            } else if (p.y) {
-                load_some<E, V>((const E*)p.y + row * p.y_sn + d, valid, y[r]);
-                if (p.g) load_some<E, V>((const E*)p.g + row * p.g_sn + d, valid, g[r]);
+            for (int i = 0; i < V; i++) {
+                const Sigmoid s = sigmoid_pair<kPrecise>(z[i]);
+                y[i] = __builtin_fmaf(keep_of(z[i], s), start ? 0.0f : h[i], take_of(z[i], s) * c[i]);
             }
-            if (STEP || p.y) {
-#pragma unroll
-                for (int i = 0; i < V; i++) sum = i < valid ? __builtin_fmaf(y[r][i], y[r][i], sum) : sum;
-            }
+            store_some<float, V>(p.next_state + row * p.D + d, valid, y);
+        } else if (p.y) {
+            const auto y_raw = load_row<E, V>(p, p.y, p.y_sn, row, d, valid);
+            if (p.g) widen<E, V>(load_row<E, V>(p, p.g, p.g_sn, row, d, valid), valid, g);
+            widen<E, V>(y_raw, valid, y);
         }
+        widen<E, V>(x_raw, valid, x);
         float ry = 0.0f;
         if (STEP || p.y) {
+#pragma unroll
+            for (int i = 0; i < V; i++) sum = __builtin_fmaf(y[i], y[i], sum);
             ry = rsqrtf(__builtin_fmaf(row_sum<LR>(sum, s_red), p.inv_d, p.eps));
-            sum = 0.0f;
-        }
 #pragma unroll
-        for (int r = 0; r < R; r++) {
-            const int d = (r * LR + j) * V, valid = live ? p.D - d : 0;
-            if (STEP || p.y) {
-#pragma unroll
-                for (int i = 0; i < V; i++) {
-                    float a = scale[r][i];
-                    if (STEP || p.g) {
-                        const float gv = g[r][i];
-                        a *= gv * keep_of(gv, sigmoid_pair<kPrecise>(gv));
-                    }
-                    x[r][i] = __builtin_fmaf(a, y[r][i] * ry * w[r][i], x[r][i]);
-                }
-                store_some<E, V>((E*)p.out + row * p.D + d, valid, x[r]);
+            for (int i = 0; i < V; i++) {
+                float a = scale[i];
+                if (STEP || p.g) a *= g[i] * keep_of(g[i], sigmoid_pair<kPrecise>(g[i]));
+                x[i] = __builtin_fmaf(a, y[i] * ry * w[i], x[i]);
             }
-#pragma unroll
-            for (int i = 0; i < V; i++) sum = i < valid ? __builtin_fmaf(x[r][i], x[r][i], sum) : sum;
+            store_some<E, V>((E*)p.out + row * p.D + d, valid, x);
         }
         float rx = 0.0f;
         if (p.next) {
+            sum = 0.0f;
+#pragma unroll
+            for (int i = 0; i < V; i++) sum = __builtin_fmaf(x[i], x[i], sum);
             rx = rsqrtf(__builtin_fmaf(row_sum<LR>(sum, s_red), p.inv_d, p.eps));
+            float u[V];
 #pragma unroll
-            for (int r = 0; r < R; r++) {
-                const int d = (r * LR + j) * V, valid = live ? p.D - d : 0;
-                float u[V];
-#pragma unroll
-                for (int i = 0; i < V; i++) u[i] = x[r][i] * rx * next[r][i];
-                store_some<E, V>((E*)p.u + row * p.D + d, valid, u);
-            }
+            for (int i = 0; i < V; i++) u[i] = x[i] * rx * next[i];
+            store_some<E, V>((E*)p.u + row * p.D + d, valid, u);
         }
         if (!STEP && p.stats && live && j == 0) {
             p.stats[2 * row] = ry;
@@ -150,155 +140,113 @@ template <class E, int V, int LR, int R, bool STEP> __global__ void __launch_bou
     }
 }
 
-template <class E, int V, int LR, int R> __global__ void __launch_bounds__(LR > 256 ? LR : 256) k_block_bwd(const Args p) {
+template <class E, int V, int LR> __global__ void __launch_bounds__(kThreads<LR>) k_block_bwd(const Args p) {
     constexpr bool kPrecise = sizeof(E) == 4;
-    constexpr int kThreads = LR > 256 ? LR : 256, kRows = kThreads / LR;
-    __shared__ float s_red[kThreads / 64];
-    __shared__ float s_join[kRows > 1 ? kThreads * R * V : 1];
-    const int j = threadIdx.x % LR;
-    float w[R][V], scale[R][V], next[R][V];
-    float dw[R][V] = {}, dscale[R][V] = {}, dnext[R][V] = {};
-#pragma unroll
-    for (int r = 0; r < R; r++) {
-        const int d = (r * LR + j) * V;
-        load_weight<V>(p.w, d, p.D, 0.0f, w[r]);
-        load_weight<V>(p.scale, d, p.D, 1.0f, scale[r]);
-        load_weight<V>(p.next, d, p.D, 0.0f, next[r]);
-    }
+    __shared__ float s_red[kThreads<LR> / 64];
+    __shared__ float s_join[kRows<LR> > 1 ? 256 * V : 1];
+    const int j = LR > 64 ? threadIdx.x : threadIdx.x % LR, d = j * V;
+    float w[V], scale[V], next[V], dw[V] = {}, dscale[V] = {}, dnext[V] = {};
+    load_weight<V>(p.w, d, p.D, 0.0f, w);
+    load_weight<V>(p.scale, d, p.D, 1.0f, scale);
+    load_weight<V>(p.next, d, p.D, 0.0f, next);
     // The next row's operands are on their way while the current row is worked on (as they lie in memory: 16-bit types take half the registers).
-    typename Vec<E, V>::type in[5][R];
+    typename Vec<E, V>::type in[5];
     float in_ry = 0.0f, in_rx = 0.0f;
     auto fetch = [&](int64_t row) {
-        const bool live = row < p.M;
-        if (live) in_ry = p.stats[2 * row], in_rx = p.stats[2 * row + 1];
-#pragma unroll
-        for (int r = 0; r < R; r++) {
-            const int d = (r * LR + j) * V, valid = live ? p.D - d : 0;
-            in[0][r] = load_raw<E, V>((const E*)p.x + row * p.x_sn + d, valid);
-            if (p.y) in[1][r] = load_raw<E, V>((const E*)p.y + row * p.y_sn + d, valid);
-            if (p.g) in[2][r] = load_raw<E, V>((const E*)p.g + row * p.g_sn + d, valid);
-            if (p.d_out) in[3][r] = load_raw<E, V>((const E*)p.d_out + row * p.do_sn + d, valid);
-            if (p.d_u) in[4][r] = load_raw<E, V>((const E*)p.d_u + row * p.du_sn + d, valid);
-        }
+        const int valid = row < p.M ? p.D - d : 0;
+        if (row < p.M) in_ry = p.stats[2 * row], in_rx = p.stats[2 * row + 1];
+        in[0] = load_row<E, V>(p, p.x, p.x_sn, row, d, valid);
+        if (p.y) in[1] = load_row<E, V>(p, p.y, p.y_sn, row, d, valid);
+        if (p.g) in[2] = load_row<E, V>(p, p.g, p.g_sn, row, d, valid);
+        if (p.d_out) in[3] = load_row<E, V>(p, p.d_out, p.do_sn, row, d, valid);
+        if (p.d_u) in[4] = load_row<E, V>(p, p.d_u, p.du_sn, row, d, valid);
     };
-    constexpr bool kAhead = LR <= 256 && R == 1;  // (wider rows have no registers left for it)
-    if (kAhead) fetch((int64_t)blockIdx.x * kRows + threadIdx.x / LR);
-    for (int64_t row0 = (int64_t)blockIdx.x * kRows; row0 < p.M; row0 += (int64_t)gridDim.x * kRows) {
-        const int64_t row = row0 + threadIdx.x / LR;
+    constexpr bool kAhead = LR <= 512;  // (workgroups of 1024 lanes have no registers left for it)
+    const int64_t row_of_lane = LR > 64 ? 0 : threadIdx.x / LR;
+    if (kAhead) fetch((int64_t)blockIdx.x * kRows<LR> + row_of_lane);
+    for (int64_t row0 = (int64_t)blockIdx.x * kRows<LR>; row0 < p.M; row0 += (int64_t)gridDim.x * kRows<LR>) {
+        const int64_t row = row0 + row_of_lane;
         const bool live = row < p.M;
+        const int valid = live ? p.D - d : 0;
         if (!kAhead) fetch(row);
-        float x[R][V], yn[R][V], g[R][V], dx[R][V], t[R][V];
+        float x[V], yn[V], g[V], dx[V] = {}, t[V] = {};
         const float ry = live ? in_ry : 0.0f, rx = live ? in_rx : 0.0f;
+        widen<E, V>(in[0], valid, x);
+        if (p.y) widen<E, V>(in[1], valid, yn);
+        if (p.g) widen<E, V>(in[2], valid, g);
+        if (p.d_out) widen<E, V>(in[3], valid, dx);
+        if (p.d_u) widen<E, V>(in[4], valid, t);
+        if (kAhead) fetch(row + (int64_t)gridDim.x * kRows<LR>);
+        // yn = y ry; x becomes xn = new rx; t = d_u (then d_u next)
         float sum = 0.0f;
 #pragma unroll
-        for (int r = 0; r < R; r++) {
-            widen<E, V>(in[0][r], x[r]);
-            if (p.y) widen<E, V>(in[1][r], yn[r]);
-            if (p.g) widen<E, V>(in[2][r], g[r]);
-            if (p.d_out) widen<E, V>(in[3][r], dx[r]);
-            if (p.d_u) widen<E, V>(in[4][r], t[r]);
-        }
-        if (kAhead) fetch(row + (int64_t)gridDim.x * kRows);
-        // yn = y ry; x becomes xn = new rx; t = d_u (then d_u next)
-#pragma unroll
-        for (int r = 0; r < R; r++) {
-#pragma unroll
-            for (int i = 0; i < V; i++) {
-                if (!p.d_out) dx[r][i] = 0.0f;
-                if (!p.d_u) t[r][i] = 0.0f;
-                if (p.y) {
-                    yn[r][i] *= ry;
-                    float a = scale[r][i];
-                    if (p.g) {
-                        const float gv = g[r][i];
-                        a *= gv * keep_of(gv, sigmoid_pair<kPrecise>(gv));
-                    }
-                    x[r][i] = __builtin_fmaf(a, yn[r][i] * w[r][i], x[r][i]);
-                }
-                x[r][i] *= rx;
-                dnext[r][i] = __builtin_fmaf(t[r][i], x[r][i], dnext[r][i]);
-                t[r][i] *= next[r][i];
-                sum = __builtin_fmaf(t[r][i], x[r][i], sum);
+        for (int i = 0; i < V; i++) {
+            if (p.y) {
+                yn[i] *= ry;
+                float a = scale[i];
+                if (p.g) a *= g[i] * keep_of(g[i], sigmoid_pair<kPrecise>(g[i]));
+                x[i] = __builtin_fmaf(a, yn[i] * w[i], x[i]);
             }
+            x[i] *= rx;
+            dnext[i] = __builtin_fmaf(t[i], x[i], dnext[i]);
+            t[i] *= next[i];
+            sum = __builtin_fmaf(t[i], x[i], sum);
         }
         if (p.d_u) {
             const float mean = row_sum<LR>(sum, s_red) * p.inv_d;
 #pragma unroll
-            for (int r = 0; r < R; r++)
-#pragma unroll
-                for (int i = 0; i < V; i++) dx[r][i] = __builtin_fmaf(rx, __builtin_fmaf(-mean, x[r][i], t[r][i]), dx[r][i]);
+            for (int i = 0; i < V; i++) dx[i] = __builtin_fmaf(rx, __builtin_fmaf(-mean, x[i], t[i]), dx[i]);
         }
-#pragma unroll
-        for (int r = 0; r < R; r++) {
-            const int d = (r * LR + j) * V, valid = live ? p.D - d : 0;
-            store_some<E, V>((E*)p.dx + row * p.D + d, valid, dx[r]);
-        }
+        store_some<E, V>((E*)p.dx + row * p.D + d, valid, dx);
         if (!p.y) continue;
         sum = 0.0f;
 #pragma unroll
-        for (int r = 0; r < R; r++) {
-            const int d = (r * LR + j) * V, valid = live ? p.D - d : 0;
-#pragma unroll
-            for (int i = 0; i < V; i++) {
-                const float n = yn[r][i] * w[r][i], dp = dx[r][i] * scale[r][i];
-                float a = 1.0f;
-                if (p.g) {
-                    const float gv = g[r][i];
-                    const Sigmoid s = sigmoid_pair<kPrecise>(gv);
-                    const float sig = keep_of(gv, s);
-                    a = gv * sig;
-                    g[r][i] = dp * n * __builtin_fmaf(a, take_of(gv, s), sig);
-                }
-                dscale[r][i] = __builtin_fmaf(dx[r][i], a * n, dscale[r][i]);
-                const float dn = dp * a;
-                dw[r][i] = __builtin_fmaf(dn, yn[r][i], dw[r][i]);
-                t[r][i] = dn * w[r][i];
-                sum = __builtin_fmaf(t[r][i], yn[r][i], sum);
+        for (int i = 0; i < V; i++) {
+            const float n = yn[i] * w[i], dp = dx[i] * scale[i];
+            float a = 1.0f;
+            if (p.g) {
+                const Sigmoid s = sigmoid_pair<kPrecise>(g[i]);
+                const float sig = keep_of(g[i], s);
+                a = g[i] * sig;
+                g[i] = dp * n * __builtin_fmaf(a, take_of(g[i], s), sig);
             }
-            if (p.g) store_some<E, V>((E*)p.dg + row * p.dg_sn + d, valid, g[r]);
+            dscale[i] = __builtin_fmaf(dx[i], a * n, dscale[i]);
+            const float dn = dp * a;
+            dw[i] = __builtin_fmaf(dn, yn[i], dw[i]);
+            t[i] = dn * w[i];
+            sum = __builtin_fmaf(t[i], yn[i], sum);
         }
+        if (p.g) store_some<E, V>((E*)p.dg + row * p.dg_sn + d, valid, g);
         const float mean = row_sum<LR>(sum, s_red) * p.inv_d;
+        float dy[V];
 #pragma unroll
-        for (int r = 0; r < R; r++) {
-            const int d = (r * LR + j) * V, valid = live ? p.D - d : 0;
-            float dy[V];
-#pragma unroll
-            for (int i = 0; i < V; i++) dy[i] = ry * __builtin_fmaf(-mean, yn[r][i], t[r][i]);
-            store_some<E, V>((E*)p.dy + row * p.D + d, valid, dy);
-        }
+        for (int i = 0; i < V; i++) dy[i] = ry * __builtin_fmaf(-mean, yn[i], t[i]);
+        store_some<E, V>((E*)p.dy + row * p.D + d, valid, dy);
     }
     // this workgroup's share of the three sums over rows
     float* out = p.partial + (int64_t)blockIdx.x * 3 * p.D;
 #pragma unroll
     for (int q = 0; q < 3; q++) {
-        float(&acc)[R][V] = q == 0 ? dw : q == 1 ? dscale : dnext;
-        if constexpr (kRows > 1) {
+        float(&acc)[V] = q == 0 ? dw : q == 1 ? dscale : dnext;
+        if constexpr (kRows<LR> > 1) {
             __syncthreads();
 #pragma unroll
-            for (int r = 0; r < R; r++)
-#pragma unroll
-                for (int i = 0; i < V; i++) s_join[((threadIdx.x / LR) * R * V + r * V + i) * LR + j] = acc[r][i];
+            for (int i = 0; i < V; i++) s_join[(threadIdx.x / LR * V + i) * LR + j] = acc[i];
             __syncthreads();
             if (threadIdx.x < LR) {
 #pragma unroll
-                for (int r = 0; r < R; r++)
+                for (int i = 0; i < V; i++) {
+                    float v = 0.0f;
 #pragma unroll
-                    for (int i = 0; i < V; i++) {
-                        float v = 0.0f;
-#pragma unroll
-                        for (int k = 0; k < kRows; k++) v += s_join[(k * R * V + r * V + i) * LR + j];
-                        acc[r][i] = v;
-                    }
+                    for (int k = 0; k < kRows<LR>; k++) v += s_join[(k * V + i) * LR + j];
+                    acc[i] = v;
+                }
             }
         }
-        if (threadIdx.x < LR) {
+        if (LR > 64 || threadIdx.x < LR) {
 #pragma unroll
-            for (int r = 0; r < R; r++)
-#pragma unroll
-                for (int i = 0; i < V; i++) {
-                    const int d = (r * LR + j) * V + i;
-                    if (d < p.D) out[q * p.D + d] = acc[r][i];
-                }
+            for (int i = 0; i < V; i++)
+                if (d + i < p.D) out[q * p.D + d + i] = acc[i];
         }
     }
 }
@@ -334,38 +282,38 @@ __global__ void __launch_bounds__(1024) k_block_sum(const float* __restrict__ pa
 
 constexpr int kMaxWidth = 4096;  // 1024 lanes with a vector of 4 each; with two they would spill
 
-// lanes of a row and vectors of a lane, by width.  16-bit rows of up to 512 take vectors of 8 (16-byte loads); beyond, a lane with two of them would
-// hold 256 registers in the backward pass: vectors of 4 and more lanes.
+// lanes of a row, by its vectors: fn(V, LR, workgroup).  16-byte loads, but for 16-bit rows of more than 2048 (a vector of 8 in each
+// of 1024 lanes would spill).
 template <class E, class F> static void with_shape(int64_t D, F&& fn) {
     using std::integral_constant;
-    auto pick = [&](auto v) {
-        constexpr int V = decltype(v)::value;
-        const int64_t n = (D + V - 1) / V;
-        constexpr integral_constant<int, 1> one{};
-        if (n <= 8) fn(v, integral_constant<int, 8>{}, one);
-        else if (n <= 16) fn(v, integral_constant<int, 16>{}, one);
-        else if (n <= 32) fn(v, integral_constant<int, 32>{}, one);
-        else if (n <= 64) fn(v, integral_constant<int, 64>{}, one);
-        else if constexpr (V == 4) {
-            if (n <= 128) fn(v, integral_constant<int, 128>{}, one);
-            else if (n <= 256) fn(v, integral_constant<int, 256>{}, one);
-            else if (n <= 512) fn(v, integral_constant<int, 256>{}, integral_constant<int, 2>{});
-            else fn(v, integral_constant<int, 1024>{}, one);
-        }
+    auto narrow = [&](auto v) {
+        const int n = (int)((D + decltype(v)::value - 1) / decltype(v)::value);
+        if (n <= 8) fn(v, integral_constant<int, 8>{}, 256);
+        else if (n <= 16) fn(v, integral_constant<int, 16>{}, 256);
+        else if (n <= 32) fn(v, integral_constant<int, 32>{}, 256);
+        else if (n <= 64) fn(v, integral_constant<int, 64>{}, 256);
+        else fn(v, integral_constant<int, 256>{}, (n + 63) / 64 * 64);
     };
-    if (sizeof(E) == 2 && D <= 512) pick(integral_constant<int, 8>{});
-    else pick(integral_constant<int, 4>{});
+    if constexpr (sizeof(E) == 2) {
+        if (D <= 2048) narrow(integral_constant<int, 8>{});
+        else fn(integral_constant<int, 4>{}, integral_constant<int, 1024>{}, (int)(D + 255) / 256 * 64);
+    } else {
+        if (D <= 1024) narrow(integral_constant<int, 4>{});
+        else if (D <= 2048) fn(integral_constant<int, 4>{}, integral_constant<int, 512>{}, (int)(D + 255) / 256 * 64);
+        else fn(integral_constant<int, 4>{}, integral_constant<int, 1024>{}, (int)(D + 255) / 256 * 64);
+    }
 }
-static int64_t workgroups(int64_t M, int lr) {
-    const int rows = lr > 256 ? 1 : 256 / lr;
-    const int64_t n = (M + rows - 1) / rows, most = lr > 256 ? 256 : 1024;
+// as many workgroups as stay resident: what is gained by more is less than their partial sums cost
+static int64_t workgroups(int64_t M, int lr, int threads) {
+    const int rows = lr > 64 ? 1 : 256 / lr;
+    const int64_t n = (M + rows - 1) / rows, most = 262144 / threads;
     return n < most ? n : most;
 }
 static int64_t partial_floats(int64_t M, int64_t D, int dtype) {
     int64_t n = 0;
     with_element(dtype, [&](auto* e) {
         using E = std::remove_pointer_t<decltype(e)>;
-        with_shape<E>(D, [&](auto, auto lr, auto) { n = workgroups(M, decltype(lr)::value) * 3 * D; });
+        with_shape<E>(D, [&](auto, auto lr, int threads) { n = workgroups(M, decltype(lr)::value, threads) * 3 * D; });
     });
     return n;
 }
@@ -399,10 +347,9 @@ extern "C" int acx_block_forward(const void* d_x, int64_t x_row, const void* d_y
     a.out = d_new, a.u = d_u, a.stats = d_stats;
     elem::with_element(dtype, [&](auto* e) {
         using E = std::remove_pointer_t<decltype(e)>;
-        block::with_shape<E>(D, [&](auto v, auto lr, auto r) {
+        block::with_shape<E>(D, [&](auto v, auto lr, int threads) {
             constexpr int LR = decltype(lr)::value;
-            hipLaunchKernelGGL((block::k_block_fwd<E, decltype(v)::value, LR, decltype(r)::value, false>), dim3((unsigned)block::workgroups(M, LR)), dim3(LR > 256 ? LR : 256), 0,
-                               (hipStream_t)stream, a);
+            hipLaunchKernelGGL((block::k_block_fwd<E, decltype(v)::value, LR, false>), dim3((unsigned)block::workgroups(M, LR, threads)), dim3(threads), 0, (hipStream_t)stream, a);
         });
     });
     ACX_HIP_TRY(hipGetLastError());
@@ -421,10 +368,9 @@ extern "C" int acx_block_step(const void* d_x, int64_t x_row, const void* d_proj
     a.out = d_new, a.u = d_u;
     elem::with_element(dtype, [&](auto* e) {
         using E = std::remove_pointer_t<decltype(e)>;
-        block::with_shape<E>(D, [&](auto v, auto lr, auto r) {
+        block::with_shape<E>(D, [&](auto v, auto lr, int threads) {
             constexpr int LR = decltype(lr)::value;
-            hipLaunchKernelGGL((block::k_block_fwd<E, decltype(v)::value, LR, decltype(r)::value, true>), dim3((unsigned)block::workgroups(M, LR)), dim3(LR > 256 ? LR : 256), 0,
-                               (hipStream_t)stream, a);
+            hipLaunchKernelGGL((block::k_block_fwd<E, decltype(v)::value, LR, true>), dim3((unsigned)block::workgroups(M, LR, threads)), dim3(threads), 0, (hipStream_t)stream, a);
         });
     });
     ACX_HIP_TRY(hipGetLastError());
@@ -451,10 +397,10 @@ extern "C" int acx_block_backward(const void* d_x, int64_t x_row, const void* d_
     int64_t n = 0;
     elem::with_element(dtype, [&](auto* e) {
         using E = std::remove_pointer_t<decltype(e)>;
-        block::with_shape<E>(D, [&](auto v, auto lr, auto r) {
+        block::with_shape<E>(D, [&](auto v, auto lr, int threads) {
             constexpr int LR = decltype(lr)::value;
-            n = block::workgroups(M, LR);
-            hipLaunchKernelGGL((block::k_block_bwd<E, decltype(v)::value, LR, decltype(r)::value>), dim3((unsigned)n), dim3(LR > 256 ? LR : 256), 0, (hipStream_t)stream, a);
+            n = block::workgroups(M, LR, threads);
+            hipLaunchKernelGGL((block::k_block_bwd<E, decltype(v)::value, LR>), dim3((unsigned)n), dim3(threads), 0, (hipStream_t)stream, a);
         });
     });
     ACX_HIP_TRY(hipGetLastError());

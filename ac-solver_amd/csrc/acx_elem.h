@@ -38,29 +38,12 @@ template <class E, int V> __device__ __forceinline__ void store(E* p, const floa
         *(typename Vec<E, V>::type*)p = v;
     }
 }
-// the first `valid` of V elements (the end of a row); the others read as zero and are not touched
-template <class E, int V> __device__ __forceinline__ void load_some(const E* p, int valid, float (&out)[V]) {
-    if (valid >= V) {
-        load<E, V>(p, out);
-    } else {
-#pragma unroll
-        for (int i = 0; i < V; i++) out[i] = i < valid ? (float)p[i] : 0.0f;
-    }
-}
-template <class E, int V> __device__ __forceinline__ void store_some(E* p, int valid, const float (&in)[V]) {
-    if (valid >= V) {
-        store<E, V>(p, in);
-    } else {
-#pragma unroll
-        for (int i = 0; i < V; i++)
-            if (i < valid) p[i] = (E)in[i];
-    }
-}
-
-// The same in two steps, for loads that are started well before their values are looked at: the vector as it lies in memory, and its values.
-template <class E, int V> __device__ __forceinline__ typename Vec<E, V>::type load_raw(const E* p, int valid) {
+// The first `valid` of V elements (the end of a row, or nothing at all), in two steps, for loads that are started well before their values are looked
+// at.  `ahead`: V elements can be read all the same, what stands behind the row's end is another row's or a gap's -- one load, where an
+// element at a time costs V.  `widen` takes the values and makes those behind the end zero.
+template <class E, int V> __device__ __forceinline__ typename Vec<E, V>::type load_raw(const E* p, int valid, bool ahead) {
     typename Vec<E, V>::type v = {};
-    if (valid >= V) {
+    if (valid >= V || (valid > 0 && ahead)) {
         v = *(const typename Vec<E, V>::type*)p;
     } else {
 #pragma unroll
@@ -69,9 +52,43 @@ template <class E, int V> __device__ __forceinline__ typename Vec<E, V>::type lo
     }
     return v;
 }
-template <class E, int V> __device__ __forceinline__ void widen(const typename Vec<E, V>::type& v, float (&out)[V]) {
+template <class E, int V> __device__ __forceinline__ void widen(const typename Vec<E, V>::type& v, int valid, float (&out)[V]) {
 #pragma unroll
     for (int i = 0; i < V; i++) out[i] = (float)v[i];
+    if (valid < V) {
+#pragma unroll
+        for (int i = 0; i < V; i++) out[i] = i < valid ? out[i] : 0.0f;
+    }
+}
+template <class E, int V> __device__ __forceinline__ void load_some(const E* p, int valid, float (&out)[V], bool ahead = false) { widen<E, V>(load_raw<E, V>(p, valid, ahead), valid, out); }
+// (in pieces of 4, 2 and 1, by the bits of `valid`)
+template <class E, int V> __device__ __forceinline__ void store_some(E* p, int valid, const float (&in)[V]) {
+    static_assert(V == 2 || V == 4 || V == 8, "pieces");
+    if (valid >= V) {
+        store<E, V>(p, in);
+    } else if (valid > 0) {
+        float v[V];
+#pragma unroll
+        for (int i = 0; i < V; i++) v[i] = in[i];
+        if constexpr (V > 4) {
+            if (valid & 4) {
+                const float a[4] = {v[0], v[1], v[2], v[3]};
+                store<E, 4>(p, a);
+                p += 4;
+#pragma unroll
+                for (int i = 0; i < 4; i++) v[i] = v[i + 4];
+            }
+        }
+        if constexpr (V > 2) {
+            if (valid & 2) {
+                const float a[2] = {v[0], v[1]};
+                store<E, 2>(p, a);
+                p += 2;
+                v[0] = v[2];
+            }
+        }
+        if (valid & 1) *p = (E)v[0];
+    }
 }
 
 // v + the value of the lane that a DPP control names: neighbours 1, 2, 4 and 8 apart cost one vector instruction and no trip through LDS
