@@ -81,14 +81,30 @@ template <class E, int V> __device__ __forceinline__ void load_segment(const voi
         p += t0 + k + 1 < end ? st * (int64_t)sizeof(E) : 0;
     }
 }
-// Where an episode starts: one lane mask per step in scalar registers, so that a select on it is one instruction.  -> whether this lane has any
+// Where an episode starts: one lane mask per step in scalar registers, so that a select on it is one instruction.  -> whether this lane has any.
+// A wave over at most four rows reads all its 16 x 4 flags with one load, a lane each; most segments have none and are done with it.
 __device__ __forceinline__ bool load_starts(const Args& p, const Lane& me, int64_t t0, int64_t end, bool (&start)[kSeg]) {
+    const int lane = threadIdx.x & 63, mine = (int)(me.n - me.n0), rows = __builtin_amdgcn_readlane(mine, 63);
+    if (rows < 4) {
+        const int k = lane & 15, r = lane >> 4;
+        const int64_t t = t0 + k < end ? t0 + k : end - 1;
+        const bool flag = t0 + k < end && r <= rows && p.reset[t * p.N + me.n0 + (r <= rows ? r : 0)] != 0;
+        const uint64_t all = __ballot(flag);
+        if (all == 0) return false;
+        uint32_t bits = (uint32_t)all & 0xFFFFu;
+        if (rows > 0) {
+            const uint32_t low = mine & 1 ? (uint32_t)all >> 16 : (uint32_t)all & 0xFFFFu, high = mine & 1 ? (uint32_t)(all >> 32) >> 16 : (uint32_t)(all >> 32) & 0xFFFFu;
+            bits = mine & 2 ? high : low;
+        }
+#pragma unroll
+        for (int i = 0; i < kSeg; i++) start[i] = bits >> i & 1;
+        return bits != 0;
+    }
     bool any = false;
     const uint8_t* r = p.reset + t0 * p.N + me.n0;
-    const uint32_t offset = (uint32_t)(me.n - me.n0);
 #pragma unroll
     for (int k = 0; k < kSeg; k++) {
-        start[k] = t0 + k < end && r[offset] != 0;
+        start[k] = t0 + k < end && r[(uint32_t)mine] != 0;
         any |= start[k];
         r += t0 + k + 1 < end ? p.N : 0;
     }
@@ -417,14 +433,20 @@ static Plan plan_of(int64_t T, int64_t N, int64_t D) {
     Plan p;
     const int64_t segments = (T + kSeg - 1) / kSeg;
     auto groups = [&](int v) { return (N * ((D + v - 1) / v) + 63) / 64; };
-    p.v = D >= 2 && groups(2) >= 512 ? 2 : 1;
+    // Two channels a lane where that leaves waves enough (424 x 399 x 150 f32: 240 us against 281 with one).
+    p.v = D >= 2 && groups(2) >= 256 ? 2 : 1;
     p.lpr = (int)((D + p.v - 1) / p.v);
     p.groups = groups(p.v);
-    p.w = p.groups >= 2048 || segments == 1 ? 1 : p.v == 2 || segments <= 4 ? 4 : 8;
+    // Eight waves a compute unit and more from the channels alone: a wave walks all steps.  Else the steps are shared by the waves of a workgroup:
+    // more of them the fewer workgroups there are (2709 x 19 x 846 bf16, 251 groups: 318 us with 16 waves, 374 with 8; from 512 groups on 8
+    // or 4 waves win, 1682 x 24366 x 2: 699 against 807) ...
+    p.w = p.groups >= 2048 || segments == 1 ? 1 : p.v == 2 || segments <= 4 ? 4 : p.groups >= 128 && p.groups < 512 && segments > 8 ? 16 : 8;
     p.chunks = 1;
     p.chunk = T;
+    // ... and under half a chip's workgroups by the workgroups of a grid as well, though that reads the operands twice (2000 x 4 x 256 f32, 16
+    // groups: 38 us in chunks, 70 without).  512 workgroups: more gain nothing (32769 x 3 x 130 bf16: 122 us with 512, 131 with 1024).
     const int64_t tile = (int64_t)p.w * kSeg, tiles = (T + tile - 1) / tile;
-    if (p.groups < 256 && tiles >= 4) {
+    if (p.groups < 128 && tiles >= 4) {
         int64_t want = 512 / p.groups;
         if (want > 128) want = 128;
         if (want > tiles) want = tiles;
@@ -449,7 +471,10 @@ template <class E, int V, int W> static void launch(bool forward, const Args& a,
 template <class E, int V> static void launch_w(bool forward, const Args& a, const Plan& p, hipStream_t st) {
     if (p.w == 1) launch<E, V, 1>(forward, a, p, st);
     else if (p.w == 4) launch<E, V, 4>(forward, a, p, st);
-    else if constexpr (V == 1) launch<E, V, 8>(forward, a, p, st);
+    else if constexpr (V == 1) {
+        if (p.w == 8) launch<E, V, 8>(forward, a, p, st);
+        else launch<E, V, 16>(forward, a, p, st);
+    }
 }
 static int run(bool forward, Args& a, int dtype, void* work, int64_t work_bytes, hipStream_t st, const char* who) {
     const Plan p = plan_of(a.T, a.N, a.D);
