@@ -12,6 +12,9 @@
 //     every wave applies the maps before it (behind it in the gradient).  W = 1 where the channels alone fill the chip.
 //   - Few channels and many steps: the steps are also cut into chunks over the grid; a first launch composes each chunk, and the second
 //     one (the same kernel) folds the chunks before its own.  That reads the operands twice, from the caches mostly.
+// Measured: 32 x 32768 x 256 f32 forward 0.59 ms, backward 1.01 ms, 5.6 and 5.4 TB/s of what they move (a copy kernel of torch: 4.8);
+// 2000 x 4 x 256 f32 33 us and 32769 x 3 x 130 bf16 122 us for both together, where the vector pipe (25 instructions an element in a composed
+// chunk, 37 forward, 58 backward, two of them transcendental) and the second reading share the time with the memory.
 // The state is float32 all the way.  The gradient needs h_(t-1) unrounded: the forward pass leaves the state in front of every segment
 // (4 bytes for 16 steps) and the backward pass runs the segment again from it in registers, which also saves it reading h.
 // k_t = 0 SELECTS zero: an infinite or NaN state of the last episode does not reach the next one through 0 * inf.
@@ -73,11 +76,11 @@ template <int V> __device__ __forceinline__ Lane lane_of(const Args& p) {
 }
 
 // one segment's operands; steps at or behind `end` read the last step (in bounds) and are made the identity by the caller
-template <class E, int V> __device__ __forceinline__ void load_segment(const void* base, int64_t first, int64_t st, uint32_t offset, int64_t t0, int64_t end, float (&out)[kSeg][V]) {
+template <class E, int V, bool STREAM> __device__ __forceinline__ void load_segment(const void* base, int64_t first, int64_t st, uint32_t offset, int64_t t0, int64_t end, float (&out)[kSeg][V]) {
     const char* p = (const char*)base + (first + t0 * st) * (int64_t)sizeof(E);  // (scalar)
 #pragma unroll
     for (int k = 0; k < kSeg; k++) {
-        load<E, V>((const E*)(p + offset), out[k]);
+        load<E, V, STREAM>((const E*)(p + offset), out[k]);
         p += t0 + k + 1 < end ? st * (int64_t)sizeof(E) : 0;
     }
 }
@@ -197,7 +200,7 @@ template <int V, bool COMPACT> struct Gates {
 };
 
 // FINAL: write h, last, bounds.  Otherwise only compose the chunk (agg).
-template <class E, int V, int W, bool FINAL> __global__ void __launch_bounds__(64 * W) k_scan_fwd(const Args p) {
+template <class E, int V, int W, bool FINAL, bool STREAM> __global__ void __launch_bounds__(64 * W) k_scan_fwd(const Args p) {
     constexpr bool kPrecise = sizeof(E) == 4;
     __shared__ Affine s_map[2][W][64 * V];
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -221,8 +224,8 @@ template <class E, int V, int W, bool FINAL> __global__ void __launch_bounds__(6
         float f[kSeg][V], b[kSeg][V];
         bool start[kSeg] = {}, starts = false;
         if (t0 < end) {
-            load_segment<E, V>(p.z, me.n0 * p.z_sn, p.z_st, z_off, t0, end, f);
-            load_segment<E, V>(p.c, me.n0 * p.c_sn, p.c_st, c_off, t0, end, b);
+            load_segment<E, V, STREAM>(p.z, me.n0 * p.z_sn, p.z_st, z_off, t0, end, f);
+            load_segment<E, V, STREAM>(p.c, me.n0 * p.c_sn, p.c_st, c_off, t0, end, b);
             if (p.reset) starts = load_starts(p, me, t0, end, start);
         }
 #pragma unroll
@@ -273,7 +276,7 @@ template <class E, int V, int W, bool FINAL> __global__ void __launch_bounds__(6
                 for (int k = 0; k < kSeg; k++) {
 #pragma unroll
                     for (int i = 0; i < V; i++) h[i] = __builtin_fmaf(f[k][i], start[k] ? 0.0f : h[i], b[k][i]);
-                    if (t0 + k < end) store<E, V>((E*)(hp + h_off), h);
+                    if (t0 + k < end) store<E, V, STREAM>((E*)(hp + h_off), h);
                     hp += nd * (int64_t)sizeof(E);
                 }
                 if constexpr (W == 1) {
@@ -298,7 +301,7 @@ template <class E, int V, int W, bool FINAL> __global__ void __launch_bounds__(6
 
 // The gradient runs from the last step to the first on X_t = what step t + 1 hands back (X_(T-1) = dlast): G_t = dh_t + X_t,
 // X_(t-1) = f_t k_t G_t; a segment is the map X -> A X + B of the X behind it to the X in front of it.
-template <class E, int V, int W, bool FINAL> __global__ void __launch_bounds__(64 * W) k_scan_bwd(const Args p) {
+template <class E, int V, int W, bool FINAL, bool STREAM> __global__ void __launch_bounds__(64 * W) k_scan_bwd(const Args p) {
     constexpr bool kPrecise = sizeof(E) == 4;
     __shared__ Affine s_map[2][W][64 * V];
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -325,9 +328,9 @@ template <class E, int V, int W, bool FINAL> __global__ void __launch_bounds__(6
         float diff[kSeg][V], g[kSeg][V];  // c, then k h_(t-1) - c; dh
         bool start[kSeg] = {}, starts = false;
         if (t0 < end) {
-            load_segment<E, V>(p.z, me.n0 * p.z_sn, p.z_st, z_off, t0, end, gate.s);
-            if constexpr (FINAL) load_segment<E, V>(p.c, me.n0 * p.c_sn, p.c_st, c_off, t0, end, diff);
-            load_segment<E, V>(p.dh, me.n0 * p.dh_sn, p.dh_st, g_off, t0, end, g);
+            load_segment<E, V, STREAM>(p.z, me.n0 * p.z_sn, p.z_st, z_off, t0, end, gate.s);
+            if constexpr (FINAL) load_segment<E, V, STREAM>(p.c, me.n0 * p.c_sn, p.c_st, c_off, t0, end, diff);
+            load_segment<E, V, STREAM>(p.dh, me.n0 * p.dh_sn, p.dh_st, g_off, t0, end, g);
             if (p.reset) starts = load_starts(p, me, t0, end, start);
         }
 #pragma unroll
@@ -399,8 +402,8 @@ template <class E, int V, int W, bool FINAL> __global__ void __launch_bounds__(6
                             dz[i] = diff[k][i] * u * fG;
                             x[i] = start[k] ? 0.0f : fG;
                         }
-                        store<E, V>((E*)(dcp + dc_off), dc);
-                        store<E, V>((E*)(dzp + dz_off), dz);
+                        store<E, V, STREAM>((E*)(dcp + dc_off), dc);
+                        store<E, V, STREAM>((E*)(dzp + dz_off), dz);
                     }
                     dcp -= dc_st, dzp -= dz_st;
                 }
@@ -433,18 +436,18 @@ static Plan plan_of(int64_t T, int64_t N, int64_t D) {
     Plan p;
     const int64_t segments = (T + kSeg - 1) / kSeg;
     auto groups = [&](int v) { return (N * ((D + v - 1) / v) + 63) / 64; };
-    // Two channels a lane where that leaves waves enough (424 x 399 x 150 f32: 240 us against 281 with one).
+    // (Times of one forward and one backward pass, episodes of about 200 steps.)  Two channels a lane where that leaves waves enough: 424 x 399 x 150 f32
+    // 210 us, 236 with one; with 256 groups or fewer one channel is no slower and leaves more workgroups.
     p.v = D >= 2 && groups(2) >= 256 ? 2 : 1;
     p.lpr = (int)((D + p.v - 1) / p.v);
     p.groups = groups(p.v);
-    // Eight waves a compute unit and more from the channels alone: a wave walks all steps.  Else the steps are shared by the waves of a workgroup:
-    // more of them the fewer workgroups there are (2709 x 19 x 846 bf16, 251 groups: 318 us with 16 waves, 374 with 8; from 512 groups on 8
-    // or 4 waves win, 1682 x 24366 x 2: 699 against 807) ...
+    // Eight waves a compute unit and more from the channels alone: a wave walks all steps.  Else the steps are shared by the waves of a workgroup, 16 where
+    // there is about a workgroup for each compute unit (2709 x 19 x 846 bf16, 251 groups: 265 us, 289 with 8 waves) and 8 or 4 where there are more ...
     p.w = p.groups >= 2048 || segments == 1 ? 1 : p.v == 2 || segments <= 4 ? 4 : p.groups >= 128 && p.groups < 512 && segments > 8 ? 16 : 8;
     p.chunks = 1;
     p.chunk = T;
-    // ... and under half a chip's workgroups by the workgroups of a grid as well, though that reads the operands twice (2000 x 4 x 256 f32, 16
-    // groups: 38 us in chunks, 70 without).  512 workgroups: more gain nothing (32769 x 3 x 130 bf16: 122 us with 512, 131 with 1024).
+    // ... and where there are fewer, by the workgroups of a grid as well, though that reads the operands twice (2000 x 4 x 256 f32, 16 groups: 33 us, 147
+    // in one chunk; 32769 x 3 x 130 bf16, 7 groups: 129 us, 2275 in one).  512 workgroups: that last one takes 149 us with 256 and 144 with 1024.
     const int64_t tile = (int64_t)p.w * kSeg, tiles = (T + tile - 1) / tile;
     if (p.groups < 128 && tiles >= 4) {
         int64_t want = 512 / p.groups;
@@ -457,15 +460,17 @@ static Plan plan_of(int64_t T, int64_t N, int64_t D) {
 }
 
 template <class E, int V, int W> static void launch(bool forward, const Args& a, const Plan& p, hipStream_t st) {
-    const dim3 block(64 * W);
-    const unsigned gx = (unsigned)p.groups, gy = (unsigned)p.chunks;
-    if (forward) {
-        // (the last chunk's own map is not asked for by anyone, the first one's in the gradient neither; they cost nothing beside the others)
-        if (gy > 1) hipLaunchKernelGGL((k_scan_fwd<E, V, W, false>), dim3(gx, gy), block, 0, st, a);
-        hipLaunchKernelGGL((k_scan_fwd<E, V, W, true>), dim3(gx, gy), block, 0, st, a);
+    const dim3 block(64 * W), grid((unsigned)p.groups, (unsigned)p.chunks);
+    if (p.chunks > 1) {  // (the last chunk's own map is not asked for by anyone, the first one's in the gradient neither; they cost nothing beside the others)
+        if (forward) hipLaunchKernelGGL((k_scan_fwd<E, V, W, false, false>), grid, block, 0, st, a);
+        else hipLaunchKernelGGL((k_scan_bwd<E, V, W, false, false>), grid, block, 0, st, a);
+    }
+    if (W == 1 && a.T * a.N * a.D * (int64_t)sizeof(E) > kStreamBytes) {
+        if (forward) hipLaunchKernelGGL((k_scan_fwd<E, V, W, true, W == 1>), grid, block, 0, st, a);
+        else hipLaunchKernelGGL((k_scan_bwd<E, V, W, true, W == 1>), grid, block, 0, st, a);
     } else {
-        if (gy > 1) hipLaunchKernelGGL((k_scan_bwd<E, V, W, false>), dim3(gx, gy), block, 0, st, a);
-        hipLaunchKernelGGL((k_scan_bwd<E, V, W, true>), dim3(gx, gy), block, 0, st, a);
+        if (forward) hipLaunchKernelGGL((k_scan_fwd<E, V, W, true, false>), grid, block, 0, st, a);
+        else hipLaunchKernelGGL((k_scan_bwd<E, V, W, true, false>), grid, block, 0, st, a);
     }
 }
 template <class E, int V> static void launch_w(bool forward, const Args& a, const Plan& p, hipStream_t st) {

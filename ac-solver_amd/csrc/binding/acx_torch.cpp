@@ -104,6 +104,13 @@ void require_gpu(const Tensor& t) {
     if (!t.is_cuda()) value_error("the activations have to live on a GPU, not on " + t.device().str() + ": there is no CPU path");
 }
 
+// a caller's tensor that results are written into: contiguous last axis, no element named twice
+void require_target(const Tensor& t, const char* name, const Tensor& like) {
+    if (!activation(t, name, &like, like.sizes()).is_same(t)) value_error(std::string(name) + " has to have a contiguous last axis");
+    for (int64_t k = 0; k + 1 < t.dim(); k++)
+        if (t.size(k) > 1 && t.stride(k) < t.size(-1)) value_error(std::string(name) + " has rows that overlap");
+}
+
 void* ptr(const Tensor& t) { return t.data_ptr(); }
 void* ptr(const Maybe& t) { return t ? t->data_ptr() : nullptr; }
 template <class T> T* ptr_as(const Tensor& t) { return static_cast<T*>(t.data_ptr()); }
@@ -178,11 +185,8 @@ std::tuple<Tensor, Tensor, Maybe> scan_backward(const Tensor& d_hidden, const Ma
     const Tensor b = plain(bounds, "bounds", {api.acx_scan_bounds_bytes(o.steps, o.rows, o.width) / 4}, o.c.device());
     const c10::OptionalDeviceGuard guard(o.c.device());
     auto target = [&](Maybe& t, const char* name) {
-        if (!t) {
-            t = same(o.c, o.c.sizes());
-        } else if (!activation(*t, name, &o.c, o.c.sizes()).is_same(*t)) {
-            value_error(std::string(name) + " has to have a contiguous last axis");
-        }
+        if (t) require_target(*t, name, o.c);
+        else t = same(o.c, o.c.sizes());
     };
     target(dc, "out[0]"), target(dz, "out[1]");
     const int code = code_of(o.c.scalar_type());
@@ -291,11 +295,8 @@ std::tuple<Tensor, Maybe, Maybe, Maybe, Maybe, Maybe> block_backward(const Maybe
     Maybe dy, dg_rows;
     if (o.y) dy = same(o.x, o.x.sizes());
     if (o.g) {
-        if (!dg) {
-            dg = same(o.x, o.x.sizes());
-        } else if (!activation(*dg, "d_gate_out", &o.x, o.x.sizes()).is_same(*dg)) {
-            value_error("d_gate_out has to have a contiguous last axis");
-        }
+        if (dg) require_target(*dg, "d_gate_out", o.x);
+        else dg = same(o.x, o.x.sizes());
     } else {
         dg = std::nullopt;
     }

@@ -256,3 +256,16 @@ def test_repeated_calls_side_streams_and_graph_replays_agree():
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(out, work()))
+
+
+def test_tensors_larger_than_the_caches():
+    import torch
+
+    from ac_solver.agents.activation8 import pack8, unpack8
+
+    x = values(70001, 1001, "float32", 5)
+    q, e = pack8(x)
+    back = unpack8(q, e)
+    for part in (slice(0, 30000), slice(30000, 70001)):
+        qh, eh = pack8(x[part])
+        assert torch.equal(q[part], qh) and torch.equal(e[part], eh) and torch.equal(back[part], unpack8(qh, eh))

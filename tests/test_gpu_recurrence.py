@@ -314,3 +314,74 @@ def test_two_threads_at_once():
     for t in threads:
         t.join()
     assert not bad, bad
+
+
+def test_targets_of_gradients_are_checked():
+    import torch
+
+    from ac_solver.agents.block_norm import block_output_backward, block_output_forward
+    from ac_solver.agents.recurrence import gated_scan_backward, gated_scan_forward
+
+    c, z, r, s, dh, dl = inputs(6, 3, 8, "float32", 2)
+    _, _, bounds = gated_scan_forward(c, z, r, s)
+    one = torch.zeros(1, 3, 8, device="cuda").expand(6, 3, 8)
+    with pytest.raises(ValueError, match="overlap"):
+        gated_scan_backward(dh, dl, c, z, r, bounds, out=(one, torch.empty_like(c)))
+    with pytest.raises(ValueError, match="contiguous last axis"):
+        gated_scan_backward(dh, dl, c, z, r, bounds, out=(torch.empty_like(c), torch.empty(6, 8, 3, device="cuda").transpose(1, 2)))
+    w = torch.ones(8, device="cuda")
+    _, _, stats = block_output_forward(c, z, dh, w, w, w)
+    with pytest.raises(ValueError, match="overlap"):
+        block_output_backward(c, c, c, z, dh, w, w, w, stats, d_gate_out=one)
+    with pytest.raises(ValueError, match="bounds has the shape"):
+        gated_scan_backward(dh, dl, c, z, r, bounds[1:])
+    with pytest.raises(ValueError, match="stats has the shape"):
+        block_output_backward(c, c, c, z, dh, w, w, w, stats[1:])
+
+
+def test_tensors_of_another_device_than_the_current_one():
+    """(one GPU: the current device is the tensors' own; a tensor elsewhere is refused by name)"""
+    import torch
+
+    from ac_solver.agents.recurrence import gated_scan
+
+    c, z, r, s, dh, dl = inputs(6, 3, 8, "float32", 2)
+    with pytest.raises(ValueError, match="state lives on cpu"):
+        gated_scan(c, z, state=s.cpu())
+    with pytest.raises(ValueError, match="gate is"):
+        gated_scan(c, z.cpu())
+    if torch.cuda.device_count() > 1:
+        with torch.cuda.device(1):
+            assert torch.equal(gated_scan(c, z, r, s)[0], gated_scan(c, z, r, s)[0])
+
+
+def test_in_place_changes_of_what_autograd_kept_are_noticed():
+    import torch
+
+    from ac_solver.agents.recurrence import gated_scan
+
+    c, z, r, s, dh, dl = inputs(6, 3, 8, "float32", 2)
+    c.requires_grad_()
+    z2 = z * 1.0
+    h, _ = gated_scan(c, z2)
+    z2.add_(1.0)
+    with pytest.raises(RuntimeError, match="inplace"):
+        h.sum().backward()
+
+
+def test_tensors_larger_than_the_caches():
+    """over 256 MiB a tensor the accesses go past the caches: the same bits as in halves that do not"""
+    import torch
+
+    from ac_solver.agents.recurrence import gated_scan_backward, gated_scan_forward
+
+    c, z, r, s, dh, dl = inputs(20, 13200, 257, "float32", 4)
+    whole = gated_scan_forward(c, z, r, s)
+    grads = gated_scan_backward(dh, dl, c, z, r, whole[2])
+    for part in (slice(0, 6600), slice(6600, 13200)):
+        cut = lambda t: t[:, part] if t.dim() == 3 or t.dtype == torch.bool else t[part]  # noqa: E731
+        args = [cut(c), cut(z), cut(r).contiguous(), cut(s).contiguous()]
+        half = gated_scan_forward(*args)
+        g = gated_scan_backward(cut(dh), cut(dl).contiguous(), args[0], args[1], args[2], half[2])
+        assert torch.equal(cut(whole[0]), half[0]) and torch.equal(cut(whole[1]), half[1])
+        assert all(torch.equal(cut(a), b) for a, b in zip(grads, g))
