@@ -12,7 +12,7 @@ from ac_solver.agents._ops import DTYPES, ops
 def pack8(x):
     """x [..., width] (float32, bfloat16 or float16) -> (q [..., width] int8, exponent [..., ceil(width / 32)] uint8): the value kept for x
     is q * 2^(exponent - 127), with one exponent for 32 neighbouring features -- the smallest for which the largest of them rounds to at
-    most 127, so the error is at most 2^-7 of that largest one.  A block that holds an infinity or a NaN is marked (exponent 255) and
+    most 127, so the error is at most 2^-7 of that largest one (rows of up to 2^20 features).  A block that holds an infinity or a NaN is marked (exponent 255) and
     restores to NaN."""
     return ops.pack8(x)
 
@@ -27,7 +27,7 @@ def unpack8(q, exponent, dtype=torch.float32):
 def weight_grad8(d_out, q, exponent):
     """The gradients of weight and bias of a linear layer whose input was kept by pack8: d_out [..., outputs] (float32, bfloat16 or float16),
     q [..., inputs] -> (d_out^T x [outputs, inputs], sum of d_out [outputs]), both float32, x the values the checkpoint stands for; float32
-    accuracy for every type of d_out."""
+    accuracy for every type of d_out.  Up to 65536 outputs and inputs, 2^29 weights."""
     return ops.weight_grad8(d_out, q, exponent)
 
 
@@ -76,7 +76,8 @@ class _Packed:
         self.dtype = t.dtype
 
 
-MIN_VALUES = 1 << 12
+MIN_VALUES = 1 << 12  # a tensor worth a launch
+MAX_WIDTH = 1 << 20  # of pack8
 _inside = threading.local()
 
 
@@ -89,7 +90,7 @@ class checkpoint8(torch.autograd.graph.saved_tensors_hooks):
     """`with checkpoint8(): ...` -- what autograd keeps of the activations computed inside the block is kept in 8 bits (pack8) and restored
     in the backward pass: a quarter (float32) or half (16 bits) of the memory; the gradients are those of the restored values (row
     statistics and states that an operator kept beside them stay what they were).  Kept as they are: leaves (parameters, inputs),
-    vectors, tensors of fewer than 4096 values, whole numbers, tensors on the CPU."""
+    vectors, tensors of fewer than 4096 values or with rows of more than 2^20, whole numbers, tensors on the CPU."""
 
     def __init__(self):
         super().__init__(self._keep, self._restore)
@@ -104,7 +105,7 @@ class checkpoint8(torch.autograd.graph.saved_tensors_hooks):
 
     @staticmethod
     def _keep(t):
-        if t.dtype not in DTYPES or not t.is_cuda or t.dim() < 2 or t.numel() < MIN_VALUES or t.grad_fn is None:
+        if t.dtype not in DTYPES or not t.is_cuda or t.dim() < 2 or t.numel() < MIN_VALUES or t.shape[-1] > MAX_WIDTH or t.grad_fn is None:
             return t
         return _Packed(t)
 

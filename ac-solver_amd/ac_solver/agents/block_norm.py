@@ -28,5 +28,6 @@ def block_output_forward(x, y, gate, weight, scale=None, next_weight=None, eps=1
 
 def block_output_backward(d_new, d_u, x, y, gate, weight, scale, next_weight, stats, d_gate_out=None):
     """Gradients from those of new and u (each may be None) -> (d_x, d_y, d_gate, d_weight, d_scale, d_next_weight), None for an operand that
-    is None.  `d_gate_out`: a tensor of the gate's shape to write its gradient into (a slice of a projection's gradient, say)."""
+    is None.  `d_gate_out`: a tensor of the gate's shape to write its gradient into (a slice of a projection's gradient, say; not
+    over an operand)."""
     return ops.block_output_backward(d_new, d_u, x, y, gate, weight, scale, next_weight, stats, d_gate_out)

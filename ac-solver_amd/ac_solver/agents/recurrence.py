@@ -2,7 +2,7 @@
 `acx_scan_backward` (csrc/acx_scan.hip); a block of the agent made of it and its end (block_norm), over a rollout and, in one launch,
 for a single step (`acx_block_step`, csrc/acx_block.hip).  The reference's agent has no memory (ac_solver/agents/ppo_agent.py:11-109).
 
-Arguments that do not fit raise TypeError (types) or ValueError (shapes, places, values) before anything is allocated or launched.
+Arguments that do not fit raise TypeError (types) or ValueError (shapes, places, values) before anything is launched.
 Kernels go to the current stream of the tensors' device."""
 from ac_solver.agents import activation8
 from ac_solver.agents._ops import ops
@@ -28,8 +28,9 @@ def gated_scan_forward(candidate, gate, reset=None, state=None, save=True):
 
 def gated_scan_backward(d_hidden, d_last, candidate, gate, reset, bounds, want_state=True, out=None):
     """Gradients of candidate, gate and initial state from those of hidden and last state (`d_last` may be None).  `out`: two tensors
-    [steps, rows, features] to write the first two into (slices of a projection's gradient, say).  -> (d_candidate, d_gate, d_state or None)"""
-    return ops.gated_scan_backward(d_hidden, d_last, candidate, gate, reset, bounds, want_state, *(out or (None, None)))
+    [steps, rows, features] to write the first two into (slices of a projection's gradient, say; not over an operand).
+    -> (d_candidate, d_gate, d_state or None)"""
+    return ops.gated_scan_backward(d_hidden, d_last, candidate, gate, reset, bounds, want_state, *((None, None) if out is None else out))
 
 
 def recurrent_block(x, projected, state, weight, scale=None, next_weight=None, reset=None, eps=1e-6):

@@ -475,8 +475,18 @@ template <class E, int TO, int TI, int NT> static hipError_t launch(const Args& 
 
 static int check_rows(int64_t M, int64_t K, int dtype, const char* who) {
     if (dtype != ACX_F32 && dtype != ACX_BF16 && dtype != ACX_F16) return fail(ACX_E_INVAL, "%s: activations are ACX_F32, ACX_BF16 or ACX_F16", who);
-    if (M < 0 || K < 0 || K > (1 << 20) || M > ((int64_t)1 << 38)) return fail(ACX_E_INVAL, "%s: bad sizes", who);
+    if (M < 0 || K < 0 || K > (1 << 20) || M > ((int64_t)1 << 38)) return fail(ACX_E_INVAL, "%s: bad sizes (rows of up to 2^20 values)", who);
     return ACX_OK;
+}
+static int check_weights(int64_t M, int64_t O, int64_t I, const char* who) {
+    if (M < 1 || O < 1 || I < 1 || M > ((int64_t)1 << 38)) return fail(ACX_E_INVAL, "%s: no rows, outputs or inputs", who);
+    if (O > (1 << 16) || I > (1 << 16) || O * I > (1 << 29)) return fail(ACX_E_INVAL, "%s: up to 65536 outputs and inputs, 2^29 weights", who);
+    return ACX_OK;
+}
+// fn(first row, rows) over launches of fewer than 2^32 lanes, `lpr` lanes a row
+template <class F> static void launches(int64_t M, int64_t lpr, F&& fn) {
+    const int64_t most = (((int64_t)1 << 32) - 256) / lpr;
+    for (int64_t m = 0; m < M; m += most) fn(m, M - m < most ? M - m : most);
 }
 
 }  // namespace act8
@@ -490,12 +500,14 @@ extern "C" int acx_act8_pack(const void* d_x, int64_t x_row, int dtype, int64_t 
     if (rc) return rc;
     if (M == 0 || K == 0) return ACX_OK;
     if (!d_x || !d_q || !d_exponent) return fail(ACX_E_INVAL, "acx_act8_pack: null pointer");
-    const int64_t nb = (K + act8::kBlock - 1) / act8::kBlock, lpr = nb * (dtype == ACX_F32 ? 8 : 4), grid = (M * lpr + 255) / 256;
-    if (grid >= ((int64_t)1 << 31)) return fail(ACX_E_INVAL, "acx_act8_pack: too many values");
+    const int64_t nb = (K + act8::kBlock - 1) / act8::kBlock, lpr = nb * (dtype == ACX_F32 ? 8 : 4);
     elem::with_element(dtype, [&](auto* e) {
         using E = std::remove_pointer_t<decltype(e)>;
         auto* kernel = M * K * (int64_t)sizeof(E) > elem::kStreamBytes ? act8::k_pack8<E, sizeof(E) == 4 ? 4 : 8, true> : act8::k_pack8<E, sizeof(E) == 4 ? 4 : 8, false>;
-        hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(256), 0, (hipStream_t)stream, (const E*)d_x, x_row, M, (int)K, (int)lpr, d_q, d_exponent);
+        act8::launches(M, lpr, [&](int64_t m, int64_t rows) {
+            hipLaunchKernelGGL(kernel, dim3((unsigned)((rows * lpr + 255) / 256)), dim3(256), 0, (hipStream_t)stream, (const E*)d_x + m * x_row, x_row, rows, (int)K, (int)lpr, d_q + m * K,
+                               d_exponent + m * nb);
+        });
     });
     ACX_HIP_TRY(hipGetLastError());
     return ACX_OK;
@@ -507,28 +519,27 @@ extern "C" int acx_act8_unpack(const int8_t* d_q, const uint8_t* d_exponent, int
     if (M == 0 || K == 0) return ACX_OK;
     if (!d_x || !d_q || !d_exponent) return fail(ACX_E_INVAL, "acx_act8_unpack: null pointer");
     const int v = dtype == ACX_F32 ? 4 : 8;
-    const int64_t lpr = (K + v - 1) / v, grid = (M * lpr + 255) / 256;
-    if (grid >= ((int64_t)1 << 31)) return fail(ACX_E_INVAL, "acx_act8_unpack: too many values");
+    const int64_t nb = (K + act8::kBlock - 1) / act8::kBlock, lpr = (K + v - 1) / v;
     elem::with_element(dtype, [&](auto* e) {
         using E = std::remove_pointer_t<decltype(e)>;
         auto* kernel = M * K * (int64_t)sizeof(E) > elem::kStreamBytes ? act8::k_unpack8<E, sizeof(E) == 4 ? 4 : 8, true> : act8::k_unpack8<E, sizeof(E) == 4 ? 4 : 8, false>;
-        hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(256), 0, (hipStream_t)stream, d_q, d_exponent, M, (int)K, (int)lpr, (E*)d_x);
+        act8::launches(M, lpr, [&](int64_t m, int64_t rows) {
+            hipLaunchKernelGGL(kernel, dim3((unsigned)((rows * lpr + 255) / 256)), dim3(256), 0, (hipStream_t)stream, d_q + m * K, d_exponent + m * nb, rows, (int)K, (int)lpr, (E*)d_x + m * K);
+        });
     });
     ACX_HIP_TRY(hipGetLastError());
     return ACX_OK;
 }
 extern "C" int64_t acx_act8_workspace_bytes(int64_t M, int64_t O, int64_t I) {
-    if (M <= 0 || O <= 0 || I <= 0) return 0;
+    if (act8::check_weights(M, O, I, "acx_act8_workspace_bytes")) return 0;
     return act8::work_floats(act8::plan_of(M, O, I), O, I) * 4;
 }
 extern "C" int acx_act8_weight_grad(const void* d_out_grad, int64_t o_row, int dtype, const int8_t* d_q, const uint8_t* d_exponent, int64_t M, int64_t O, int64_t I, float* d_weight_grad,
                                     float* d_bias_grad, void* d_work, int64_t work_bytes, void* stream) {
     if (!have_device()) return ACX_E_NODEVICE;
     int rc = act8::check_rows(M, O, dtype, "acx_act8_weight_grad");
-    if (!rc) rc = act8::check_rows(M, I, dtype, "acx_act8_weight_grad");
+    if (!rc) rc = act8::check_weights(M, O, I, "acx_act8_weight_grad");
     if (rc) return rc;
-    if (O == 0 || I == 0 || M == 0) return fail(ACX_E_INVAL, "acx_act8_weight_grad: no rows, outputs or inputs");
-    if (O > (1 << 16) || I > (1 << 16)) return fail(ACX_E_INVAL, "acx_act8_weight_grad: up to 65536 outputs and inputs");
     if (o_row < O || o_row >= ((int64_t)1 << 24)) return fail(ACX_E_INVAL, "acx_act8_weight_grad: rows of d_out_grad overlap or lie too far apart (2^24 elements)");
     if (!d_out_grad || !d_q || !d_exponent || !d_weight_grad) return fail(ACX_E_INVAL, "acx_act8_weight_grad: null pointer");
     const act8::Plan p = act8::plan_of(M, O, I);

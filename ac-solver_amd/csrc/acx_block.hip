@@ -334,7 +334,7 @@ static int check_sizes(int64_t M, int64_t D, int dtype, float eps, const char* w
 using namespace acx;
 
 extern "C" int64_t acx_block_workspace_bytes(int64_t M, int64_t D, int dtype) {
-    if (M <= 0 || D <= 0 || D > block::kMaxWidth) return 0;
+    if (block::check_sizes(M, D, dtype, 0.0f, "acx_block_workspace_bytes") || M == 0 || D == 0) return 0;
     return block::partial_floats(M, D, dtype) * 4;
 }
 extern "C" int acx_block_forward(const void* d_x, int64_t x_row, const void* d_y, int64_t y_row, const void* d_gate, int64_t g_row, int dtype, const float* d_weight,

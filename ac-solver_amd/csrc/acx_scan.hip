@@ -28,6 +28,7 @@ namespace scan {
 using namespace elem;
 
 constexpr int kSeg = 16;  // steps of a segment
+template <int V, int W> constexpr bool kCut = V == 1 && W == 8;  // variants that the steps are cut into chunks for (plan_of)
 
 struct Args {
     const void *c, *z, *dh;       // candidate, gate, gradient of hidden
@@ -214,7 +215,8 @@ template <class E, int V, int W, bool FINAL, bool STREAM> __global__ void __laun
     if constexpr (FINAL) {
         float h[V] = {};
         if (p.state) load<float, V>(p.state + ch, h);
-        if (gridDim.y > 1) fold_chunks<V, W, true>(p, ch, nd, lane, w, s_map[1], h);
+        if constexpr (kCut<V, W>)
+            if (gridDim.y > 1) fold_chunks<V, W, true>(p, ch, nd, lane, w, s_map[1], h);
 #pragma unroll
         for (int i = 0; i < V; i++) carry[i].b = h[i];
     }
@@ -249,7 +251,7 @@ template <class E, int V, int W, bool FINAL, bool STREAM> __global__ void __laun
         float h[V];
 #pragma unroll
         for (int i = 0; i < V; i++) h[i] = carry[i].b;
-        if constexpr (W > 1 || !FINAL) {
+        if constexpr (W > 1) {
             Affine m[V];
 #pragma unroll
             for (int i = 0; i < V; i++) {
@@ -261,12 +263,7 @@ template <class E, int V, int W, bool FINAL, bool STREAM> __global__ void __laun
                 }
                 m[i] = {starts ? -1.0f : a, x};
             }
-            if constexpr (W == 1) {
-#pragma unroll
-                for (int i = 0; i < V; i++) carry[i] = join(m[i], carry[i]);
-            } else {
-                meet<V, W, true>(s_map[buf], lane, w, m, carry, h);
-            }
+            meet<V, W, true>(s_map[buf], lane, w, m, carry, h);
         }
         if constexpr (FINAL) {
             if (t0 < end) {
@@ -316,7 +313,8 @@ template <class E, int V, int W, bool FINAL, bool STREAM> __global__ void __laun
     if constexpr (FINAL) {
         float x[V] = {};
         if (p.dlast) load<float, V>(p.dlast + ch, x);
-        if (gridDim.y > 1) fold_chunks<V, W, false>(p, ch, nd, lane, w, s_map[1], x);
+        if constexpr (kCut<V, W>)
+            if (gridDim.y > 1) fold_chunks<V, W, false>(p, ch, nd, lane, w, s_map[1], x);
 #pragma unroll
         for (int i = 0; i < V; i++) carry[i].b = x[i];
     }
@@ -364,7 +362,7 @@ template <class E, int V, int W, bool FINAL, bool STREAM> __global__ void __laun
         float x[V];  // X behind this segment
 #pragma unroll
         for (int i = 0; i < V; i++) x[i] = carry[i].b;
-        if constexpr (W > 1 || !FINAL) {
+        if constexpr (W > 1) {
             Affine m[V];
 #pragma unroll
             for (int i = 0; i < V; i++) {
@@ -377,13 +375,8 @@ template <class E, int V, int W, bool FINAL, bool STREAM> __global__ void __laun
                 }
                 m[i] = {starts ? -1.0f : a, b};
             }
-            if constexpr (W == 1) {
-#pragma unroll
-                for (int i = 0; i < V; i++) carry[i] = join(m[i], carry[i]);
-            } else {
-                meet<V, W, false>(s_map[buf], lane, w, m, carry, x);
-                gate.forget();
-            }
+            meet<V, W, false>(s_map[buf], lane, w, m, carry, x);
+            gate.forget();
         }
         if constexpr (FINAL) {
             if (t0 < end) {
@@ -461,10 +454,11 @@ static Plan plan_of(int64_t T, int64_t N, int64_t D) {
 
 template <class E, int V, int W> static void launch(bool forward, const Args& a, const Plan& p, hipStream_t st) {
     const dim3 block(64 * W), grid((unsigned)p.groups, (unsigned)p.chunks);
-    if (p.chunks > 1) {  // (the last chunk's own map is not asked for by anyone, the first one's in the gradient neither; they cost nothing beside the others)
-        if (forward) hipLaunchKernelGGL((k_scan_fwd<E, V, W, false, false>), grid, block, 0, st, a);
-        else hipLaunchKernelGGL((k_scan_bwd<E, V, W, false, false>), grid, block, 0, st, a);
-    }
+    if constexpr (kCut<V, W>)
+        if (p.chunks > 1) {  // (the last chunk's own map is not asked for by anyone, the first one's in the gradient neither; they cost nothing beside the others)
+            if (forward) hipLaunchKernelGGL((k_scan_fwd<E, V, W, false, false>), grid, block, 0, st, a);
+            else hipLaunchKernelGGL((k_scan_bwd<E, V, W, false, false>), grid, block, 0, st, a);
+        }
     if (W == 1 && a.T * a.N * a.D * (int64_t)sizeof(E) > kStreamBytes) {
         if (forward) hipLaunchKernelGGL((k_scan_fwd<E, V, W, true, W == 1>), grid, block, 0, st, a);
         else hipLaunchKernelGGL((k_scan_bwd<E, V, W, true, W == 1>), grid, block, 0, st, a);
@@ -506,7 +500,8 @@ static bool strides_ok(int64_t D, int dtype, std::initializer_list<int64_t> rows
 static int check_sizes(int64_t T, int64_t N, int64_t D, int dtype, const char* who) {
     if (dtype != ACX_F32 && dtype != ACX_BF16 && dtype != ACX_F16) return fail(ACX_E_INVAL, "%s: activations are ACX_F32, ACX_BF16 or ACX_F16", who);
     if (T < 0 || N < 0 || D < 0 || D > (1 << 20) || T > ((int64_t)1 << 40) || N > ((int64_t)1 << 31)) return fail(ACX_E_INVAL, "%s: bad sizes", who);
-    if ((N * D) / 64 >= ((int64_t)1 << 31) || (T > 0 && N * D > ((int64_t)1 << 60) / T)) return fail(ACX_E_INVAL, "%s: too many channels", who);
+    // (a launch has fewer than 2^32 lanes; so many channels have two of them each)
+    if (N * ((D + 1) / 2) > ((int64_t)1 << 32) - 64 || (T > 0 && N * D > ((int64_t)1 << 60) / T)) return fail(ACX_E_INVAL, "%s: too many channels", who);
     return ACX_OK;
 }
 
@@ -516,11 +511,11 @@ static int check_sizes(int64_t T, int64_t N, int64_t D, int dtype, const char* w
 using namespace acx;
 
 extern "C" int64_t acx_scan_bounds_bytes(int64_t T, int64_t N, int64_t D) {
-    if (T < 0 || N < 0 || D < 0) return 0;
+    if (scan::check_sizes(T, N, D, ACX_F32, "acx_scan_bounds_bytes")) return 0;
     return (T + scan::kSeg - 1) / scan::kSeg * N * D * 4;
 }
 extern "C" int64_t acx_scan_workspace_bytes(int64_t T, int64_t N, int64_t D, int dtype) {
-    if (T <= 0 || N <= 0 || D <= 0) return 0;
+    if (scan::check_sizes(T, N, D, dtype, "acx_scan_workspace_bytes") || T == 0 || N == 0 || D == 0) return 0;
     const scan::Plan p = scan::plan_of(T, N, D);
     return p.chunks > 1 ? p.chunks * 2 * N * D * 4 : 0;
 }

@@ -43,6 +43,7 @@ struct AcxFailure : std::runtime_error {
     using std::runtime_error::runtime_error;
 };
 void check(int rc, const char* what) {
+    if (rc == ACX_E_INVAL) throw py::value_error(api.acx_last_error());
     if (rc != ACX_OK) throw AcxFailure(std::string(what) + " failed (code " + std::to_string(rc) + "): " + api.acx_last_error());
 }
 
@@ -104,11 +105,46 @@ void require_gpu(const Tensor& t) {
     if (!t.is_cuda()) value_error("the activations have to live on a GPU, not on " + t.device().str() + ": there is no CPU path");
 }
 
-// a caller's tensor that results are written into: contiguous last axis, no element named twice
-void require_target(const Tensor& t, const char* name, const Tensor& like) {
+// whether two tensors have no element in common, as far as it is told easily: memory apart, or other columns of the same rows
+bool apart(const Tensor& a, const Tensor& b) {
+    if (!a.numel() || !b.numel()) return true;
+    auto bytes = [](const Tensor& t) {
+        int64_t n = 1;
+        for (int64_t k = 0; k < t.dim(); k++) n += (t.size(k) - 1) * t.stride(k);
+        return n * (int64_t)t.element_size();
+    };
+    const int64_t between = static_cast<const char*>(b.data_ptr()) - static_cast<const char*>(a.data_ptr());
+    if (between >= bytes(a) || -between >= bytes(b)) return true;
+    if (a.scalar_type() != b.scalar_type() || a.sizes() != b.sizes()) return false;
+    int64_t row = 0;
+    for (int64_t k = 0; k + 1 < a.dim(); k++) {
+        if (a.size(k) == 1) continue;
+        if (a.stride(k) != b.stride(k)) return false;
+        row = row && row < a.stride(k) ? row : a.stride(k);
+    }
+    const int64_t columns = (between < 0 ? -between : between) / (int64_t)a.element_size();
+    return columns >= a.size(-1) && columns + a.size(-1) <= row;
+}
+void require_apart(const Tensor& t, const char* name, std::initializer_list<const Maybe*> others) {
+    for (const Maybe* o : others)
+        if (*o && !apart(t, **o)) value_error(std::string(name) + " lies in the memory of another operand");
+}
+// a caller's tensor that results are written into: contiguous last axis, no element named twice, nothing that is still read
+void require_target(const Tensor& t, const char* name, const Tensor& like, std::initializer_list<const Maybe*> others) {
     if (!activation(t, name, &like, like.sizes()).is_same(t)) value_error(std::string(name) + " has to have a contiguous last axis");
-    for (int64_t k = 0; k + 1 < t.dim(); k++)
-        if (t.size(k) > 1 && t.stride(k) < t.size(-1)) value_error(std::string(name) + " has rows that overlap");
+    int64_t extent = t.size(-1), before = 0;  // of the axes so far, from the narrowest stride to the widest
+    for (int64_t n = 0; n + 1 < t.dim(); n++) {
+        int64_t axis = -1;
+        for (int64_t k = 0; k + 1 < t.dim(); k++)
+            if (t.size(k) > 1 && t.stride(k) > before && (axis < 0 || t.stride(k) < t.stride(axis))) axis = k;
+        for (int64_t k = 0; k + 1 < t.dim(); k++)
+            if (t.size(k) > 1 && (t.stride(k) < t.size(-1) || (axis >= 0 && k != axis && t.stride(k) == t.stride(axis)))) value_error(std::string(name) + " has rows that overlap");
+        if (axis < 0) break;
+        if (t.stride(axis) < extent) value_error(std::string(name) + " has rows that overlap");
+        before = t.stride(axis);
+        extent += before * (t.size(axis) - 1);
+    }
+    require_apart(t, name, others);
 }
 
 void* ptr(const Tensor& t) { return t.data_ptr(); }
@@ -184,11 +220,12 @@ std::tuple<Tensor, Tensor, Maybe> scan_backward(const Tensor& d_hidden, const Ma
     if (d_last) dl = plain(*d_last, "d_last", {o.rows, o.width}, o.c.device());
     const Tensor b = plain(bounds, "bounds", {api.acx_scan_bounds_bytes(o.steps, o.rows, o.width) / 4}, o.c.device());
     const c10::OptionalDeviceGuard guard(o.c.device());
-    auto target = [&](Maybe& t, const char* name) {
-        if (t) require_target(*t, name, o.c);
+    const Maybe operands[] = {o.c, o.z, dh, b};
+    auto target = [&](Maybe& t, const char* name, const Maybe* other) {
+        if (t) require_target(*t, name, o.c, {&operands[0], &operands[1], &operands[2], &operands[3], &dl, &o.reset, other});
         else t = same(o.c, o.c.sizes());
     };
-    target(dc, "out[0]"), target(dz, "out[1]");
+    target(dc, "out[0]", &dz), target(dz, "out[1]", &dc);
     const int code = code_of(o.c.scalar_type());
     Maybe ds, work = scratch(api.acx_scan_workspace_bytes(o.steps, o.rows, o.width, code), o.c);
     if (want_state) ds = floats({o.rows, o.width}, o.c);
@@ -295,7 +332,8 @@ std::tuple<Tensor, Maybe, Maybe, Maybe, Maybe, Maybe> block_backward(const Maybe
     Maybe dy, dg_rows;
     if (o.y) dy = same(o.x, o.x.sizes());
     if (o.g) {
-        if (dg) require_target(*dg, "d_gate_out", o.x);
+        const Maybe operands[] = {o.x, st};
+        if (dg) require_target(*dg, "d_gate_out", o.x, {&operands[0], &operands[1], &o.y, &o.g, &gn, &gu, &o.w, &o.s, &o.n});
         else dg = same(o.x, o.x.sizes());
     } else {
         dg = std::nullopt;
@@ -389,7 +427,7 @@ std::tuple<Tensor, Tensor> weight_grad8(const Tensor& d_out_, const Tensor& q_, 
     if (d_out.dim() < 1 || d_out.dim() != q.dim() || d_out.sizes().slice(0, d_out.dim() - 1) != q.sizes().slice(0, q.dim() - 1) || d_out.device() != q.device())
         value_error("d_out " + shape_text(d_out.sizes()) + " on " + d_out.device().str() + " and q " + shape_text(q.sizes()) + " on " + q.device().str() + " do not have their rows in common");
     const int64_t outputs = d_out.size(-1), inputs = q.size(-1);
-    if (outputs > 65536 || inputs > 65536) value_error("up to 65536 outputs and inputs");
+    if (outputs > 65536 || inputs > 65536 || outputs * inputs > (1 << 29)) value_error("up to 65536 outputs and inputs, 2^29 weights");
     require_gpu(d_out);
     const c10::OptionalDeviceGuard guard(d_out.device());
     const int64_t rows = inputs ? q.numel() / inputs : 0;
@@ -452,12 +490,17 @@ std::tuple<Tensor, Maybe, Tensor> recurrent_step(const Tensor& x_, const Tensor&
     const int64_t wide[2] = {rows, 3 * width};
     const Tensor projected = activation(projected_, "projected", &x, at::IntArrayRef(wide, 2)), state = plain(state_, "state", {rows, width}, dev);
     if (!weight) type_error("weight has to be a tensor, not NoneType");
-    const Tensor w = plain(*weight, "weight", {width}, dev);
+    const Maybe w = plain(*weight, "weight", {width}, dev);
     Maybe s, n, reset;
     if (scale) s = plain(*scale, "scale", {width}, dev);
     if (next_weight) n = plain(*next_weight, "next_weight", {width}, dev);
     if (reset_) reset = flags(*reset_, "reset", {rows}, dev);
     if (next_state && !plain(*next_state, "next_state", {rows, width}, dev).is_same(*next_state)) value_error("next_state has to be contiguous");
+    if (next_state) {
+        const Maybe operands[] = {x, projected, state};
+        require_apart(*next_state, "next_state", {&operands[0], &operands[1], &w, &s, &n, &reset});
+        if (ptr(*next_state) != ptr(state)) require_apart(*next_state, "next_state", {&operands[2]});
+    }
     require_gpu(x);
     const c10::OptionalDeviceGuard guard(dev);
     const Tensor next = next_state ? *next_state : floats({rows, width}, x);

@@ -395,7 +395,7 @@ int acx_block_step(const void *d_x, int64_t x_row, const void *d_projected, int6
  * value it stands for is q * 2^(exponent - 127).  The exponent is the smallest for which the block's largest magnitude rounds to at most
  * 127 (at least 1); 255 marks a block that held an infinity or a NaN, and stands for NaN.  x has a stride between rows in elements.
  * acx_act8_weight_grad: d_weight_grad [O, I] = d_out_grad^T (q 2^e) and d_bias_grad [O] (nullable) = column sums of d_out_grad, float32, for
- * d_out_grad [M, O] of type dtype; M, O, I >= 1, O and I <= 65536; d_work: acx_act8_workspace_bytes for the duration of the call's kernels. */
+ * d_out_grad [M, O] of type dtype; M, O, I >= 1, O and I <= 65536, O * I <= 2^29; d_work: acx_act8_workspace_bytes for the duration of the call's kernels. */
 int acx_act8_pack(const void *d_x, int64_t x_row, int dtype, int64_t M, int64_t K, int8_t *d_q, uint8_t *d_exponent, void *stream);
 int acx_act8_unpack(const int8_t *d_q, const uint8_t *d_exponent, int64_t M, int64_t K, void *d_x, int dtype, void *stream);
 int64_t acx_act8_workspace_bytes(int64_t M, int64_t O, int64_t I);

@@ -258,6 +258,46 @@ def test_repeated_calls_side_streams_and_graph_replays_agree():
         assert all(torch.equal(a, b) for a, b in zip(out, work()))
 
 
+def test_limits():
+    import torch
+
+    from ac_solver.agents import activation8 as A
+
+    wide = torch.randn(2, (1 << 20) + 1, device="cuda")
+    with pytest.raises(ValueError, match="2\\^20"):
+        A.pack8(wide)
+    x = wide.requires_grad_(True)
+    with A.checkpoint8():  # rows that wide stay as they are
+        out = ((x * 2.0) ** 2).sum()
+    out.backward()
+    assert torch.equal(x.grad, 8.0 * x.detach())  # (powers of two: nothing is rounded that was not before)
+    narrow = torch.zeros(1, 1, device="cuda")
+    with pytest.raises(ValueError, match="2\\^29"):
+        A.weight_grad8(narrow.expand(1, 1 << 16), torch.zeros(1, 1 << 14, device="cuda", dtype=torch.int8), torch.zeros(1, 1 << 9, device="cuda", dtype=torch.uint8))
+
+
+def test_more_lanes_than_a_launch_has():
+    """2^30 + 9 rows of 5 values: four lanes a row and more than 2^32 of them, two launches"""
+    import torch
+
+    from ac_solver.agents import activation8 as A
+
+    rows = (1 << 30) + 9
+    x = torch.empty(rows, 5, device="cuda", dtype=torch.bfloat16)
+    x.view(-1)[:] = 0
+    places = torch.tensor([0, 1, (1 << 30) - 70, (1 << 30) - 65, (1 << 30) - 64, (1 << 30) - 63, 1 << 30, rows - 1], device="cuda")
+    values = torch.randint(-127, 128, (len(places), 5), device="cuda").to(torch.bfloat16)
+    values[:, 0] = 127  # (an exponent of 0)
+    x[places] = values
+    q, e = A.pack8(x)
+    assert torch.equal(q[places], values.to(torch.int8)) and bool((e[places] == 127).all())
+    x.fill_(1.0)
+    del x
+    back = A.unpack8(q, e, torch.bfloat16)
+    assert torch.equal(back[places], values)
+    assert int((q[:, 0] != 0).sum()) == len(places) and int((back[:, 0] != 0).sum()) == len(places)
+
+
 def test_tensors_larger_than_the_caches():
     import torch
 

@@ -333,6 +333,22 @@ def test_targets_of_gradients_are_checked():
     _, _, stats = block_output_forward(c, z, dh, w, w, w)
     with pytest.raises(ValueError, match="overlap"):
         block_output_backward(c, c, c, z, dh, w, w, w, stats, d_gate_out=one)
+    wanted = gated_scan_backward(dh, dl, c, z, r, bounds)
+    buffer = torch.zeros(6, 3, 25, device="cuda")
+    ok = (buffer[..., :8], buffer[..., 8:16])
+    for a, b in zip(gated_scan_backward(dh, dl, c, z, r, bounds, out=ok), wanted):
+        assert torch.equal(a, b)
+    assert torch.equal(ok[0], wanted[0]) and torch.equal(ok[1], wanted[1]) and not buffer[..., 16:].any()
+    crossed = torch.empty(400, device="cuda").as_strided((6, 3, 8), (16, 16, 1))  # (steps and rows that meet)
+    woven = torch.empty(400, device="cuda").as_strided((6, 3, 8), (16, 8, 1))
+    for bad in (crossed, woven):
+        with pytest.raises(ValueError, match="overlap"):
+            gated_scan_backward(dh, dl, c, z, r, bounds, out=(torch.empty_like(c), bad))
+    for bad in ((c, torch.empty_like(c)), (torch.empty_like(c), dh), (buffer[..., :8], buffer[..., 7:15]), (buffer[..., :8], buffer[..., :8])):
+        with pytest.raises(ValueError, match="in the memory of another operand"):
+            gated_scan_backward(dh, dl, c, z, r, bounds, out=bad)
+    with pytest.raises(ValueError, match="in the memory of another operand"):
+        block_output_backward(c, c, c, z, dh, w, w, w, stats, d_gate_out=dh)
     with pytest.raises(ValueError, match="bounds has the shape"):
         gated_scan_backward(dh, dl, c, z, r, bounds[1:])
     with pytest.raises(ValueError, match="stats has the shape"):

@@ -51,6 +51,21 @@ def test_scan_buffer_sizes():
     assert _acx.lib.acx_scan_workspace_bytes(32, 131072, 256, _acx.F32) == 0
 
 
+def test_sizes_that_no_memory_holds_are_no_division_by_zero():
+    from ac_solver import _acx
+
+    lib, huge = _acx.lib, 1 << 62
+    for T, N, D in ((1000, huge, 64), (1000, 1 << 31, 1 << 20), (huge, 64, 64), (1000, 64, huge), (-1, 4, 4), (1000, -4, 4)):
+        assert lib.acx_scan_workspace_bytes(T, N, D, _acx.F32) == 0
+        assert lib.acx_scan_bounds_bytes(T, N, D) == 0
+    assert lib.acx_scan_workspace_bytes(1000, 4, 64, _acx.I64) == 0
+    for M, D in ((huge, 64), (64, huge), (-1, 64), (64, 4097)):
+        assert lib.acx_block_workspace_bytes(M, D, _acx.F32) == 0
+    for M, O, I in ((1000, huge, 64), (1000, 1 << 32, 1 << 32), (1000, 64, huge), (huge, 64, 64), (1000, 1 << 16, 1 << 16), (0, 64, 64)):
+        assert lib.acx_act8_workspace_bytes(M, O, I) == 0
+    assert lib.acx_act8_workspace_bytes(1000, 1 << 16, 1 << 13) > 0
+
+
 def test_the_block_end_refuses_what_it_cannot_read():
     from ac_solver.agents import block_norm as B
 
@@ -91,6 +106,10 @@ def test_a_step_refuses_what_it_cannot_read():
         R.recurrent_step(x.half(), p.half(), h.half(), w)
     with pytest.raises(ValueError, match="next_state has to be contiguous"):
         R.recurrent_step(x, p, h, w, next_state=torch.zeros(8, 5).t())
+    both = torch.zeros(6, 8)  # (the state itself may be the target, not a part of it, nor anything else that is read)
+    for state, target, inputs in ((both[:5], both[1:], x), (h, x, x)):
+        with pytest.raises(ValueError, match="next_state lies in the memory"):
+            R.recurrent_step(inputs, p, state, w, next_state=target)
     with pytest.raises(TypeError, match="reset"):
         R.recurrent_step(x, p, h, w, reset=torch.zeros(5))
     with pytest.raises(ValueError, match="4096"):
