@@ -10,7 +10,7 @@
 // the accuracy of a float32 product, at one to three times the matrix work of a bf16 one and 1 byte instead of 4 read per x.
 // A block with an infinity or a NaN is marked with the exponent byte 255 and restores to NaN: it is not hidden.
 // Measured: 1 Mi x 256 f32 packed in 0.273 ms and restored in 0.273 ms (4.95 TB/s).  Weight gradient of 1 Mi rows, 768 x 256: dy bf16 0.53 ms (4.5 TB/s,
-// memory), dy f32 1.23 ms: 1.24 PFLOP of bf16 products at 1.0 PFLOP/s, where the chip's clock drops to 1.5 GHz under the matrix units' load
+// memory), dy f32 1.19 ms: 1.24 PFLOP of bf16 products at 1.04 PFLOP/s, where the chip's clock drops to 1.5 GHz under the matrix units' load
 // (a library's bf16 product of 8192^3: 1.16 PFLOP/s).  65537 x 256 x 72 bf16 20 + 5 us: five steps a workgroup, their latency and the join.
 #include <type_traits>
 

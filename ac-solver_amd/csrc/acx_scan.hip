@@ -13,7 +13,7 @@
 //   - Few channels and many steps: the steps are also cut into chunks over the grid; a first launch composes each chunk, and the second
 //     one (the same kernel) folds the chunks before its own.  That reads the operands twice, from the caches mostly.
 // Measured: 32 x 32768 x 256 f32 forward 0.59 ms, backward 1.01 ms, 5.6 and 5.4 TB/s of what they move (a copy kernel of torch: 4.8);
-// 2000 x 4 x 256 f32 33 us and 32769 x 3 x 130 bf16 122 us for both together, where the vector pipe (25 instructions an element in a composed
+// 2000 x 4 x 256 f32 35 us and 32769 x 3 x 130 bf16 126 us for both together, where the vector pipe (25 instructions an element in a composed
 // chunk, 37 forward, 58 backward, two of them transcendental) and the second reading share the time with the memory.
 // The state is float32 all the way.  The gradient needs h_(t-1) unrounded: the forward pass leaves the state in front of every segment
 // (4 bytes for 16 steps) and the backward pass runs the segment again from it in registers, which also saves it reading h.
@@ -439,8 +439,8 @@ static Plan plan_of(int64_t T, int64_t N, int64_t D) {
     p.w = p.groups >= 2048 || segments == 1 ? 1 : p.v == 2 || segments <= 4 ? 4 : p.groups >= 128 && p.groups < 512 && segments > 8 ? 16 : 8;
     p.chunks = 1;
     p.chunk = T;
-    // ... and where there are fewer, by the workgroups of a grid as well, though that reads the operands twice (2000 x 4 x 256 f32, 16 groups: 33 us, 147
-    // in one chunk; 32769 x 3 x 130 bf16, 7 groups: 129 us, 2275 in one).  512 workgroups: that last one takes 149 us with 256 and 144 with 1024.
+    // ... and where there are fewer, by the workgroups of a grid as well, though that reads the operands twice (2000 x 4 x 256 f32, 16 groups: 35 us, 147
+    // in one chunk; 32769 x 3 x 130 bf16, 7 groups: 126 us, 2275 in one).  512 workgroups: that last one takes 149 us with 256 and 144 with 1024.
     const int64_t tile = (int64_t)p.w * kSeg, tiles = (T + tile - 1) / tile;
     if (p.groups < 128 && tiles >= 4) {
         int64_t want = 512 / p.groups;
