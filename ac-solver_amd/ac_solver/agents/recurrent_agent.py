@@ -20,6 +20,7 @@ from ac_solver.agents.block_norm import block_input
 from ac_solver.agents.ppo_agent import Linear, initialize_layer
 from ac_solver.agents.recurrence import recurrent_block, recurrent_step
 
+MAX_WIDTH = 4096  # of block_norm
 DTYPES = {"float32": torch.float32, "bfloat16": torch.bfloat16}
 
 
@@ -44,6 +45,8 @@ class RecurrentAgent(nn.Module):
         super().__init__()
         if width < 1 or blocks < 1:
             raise ValueError("a recurrent agent has at least one block of at least one feature")
+        if width > MAX_WIDTH:
+            raise ValueError(f"blocks of up to {MAX_WIDTH} features are handled, not {width}")
         self.width, self.dtype, self.checkpoint_8bit = int(width), DTYPES[dtype], bool(checkpoint_8bit)
         input_dim = int(np.prod(envs.single_observation_space.shape))
         self.encoder = initialize_layer(Linear(input_dim, self.width))

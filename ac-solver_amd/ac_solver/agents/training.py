@@ -587,9 +587,12 @@ def ppo_training_loop(envs, args, device, optimizer, agent, curr_states, success
             ph.lap("behaviour stats (f32)")
         if recurrent and agent.dtype != torch.float32:
             # the rollout's steps keep the memory in float32 where a whole pass rounds it to the activations' type: the importance ratio is formed
-            # against what the update's own pass gives for the unchanged weights
+            # against what the update's own pass gives for the unchanged weights (as many environments at a time as a minibatch has)
             with torch.no_grad():
-                logprobs, _, values = (t.view(T, N) for t in agent.evaluate(obs[:T], actions, starts[:T], memory_before))
+                for first in range(0, N, N // args.num_minibatches):
+                    some = slice(first, first + N // args.num_minibatches)
+                    logprob, _, value = agent.evaluate(obs[:T, some], actions[:, some], starts[:T, some], memory_before[:, some])
+                    logprobs[:, some], values[:, some] = logprob.view(T, -1), value.view(T, -1)
         with torch.no_grad():
             next_value = (agent.get_value(obs[T].float(), starts[T], memory) if recurrent else agent.get_value(obs[T].float())).reshape(-1)
             advantages, returns = compute_gae(rewards, values, dones[:T], next_value, dones[T], args.gamma, args.gae_lambda)

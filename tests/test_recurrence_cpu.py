@@ -173,6 +173,8 @@ def test_the_recurrent_agent_needs_a_gpu_and_says_so():
         agent.act(torch.zeros(4, 50), torch.zeros(4, dtype=torch.bool), agent.initial_state(4))
     with pytest.raises(ValueError, match="at least one"):
         RecurrentAgent(spaces, 32, 0)
+    with pytest.raises(ValueError, match="4096"):
+        RecurrentAgent(spaces, 4097, 1)
     with pytest.raises(ValueError, match="steps, rows, features"):
         R.recurrent_block(torch.zeros(4, 8), torch.zeros(4, 24), None, torch.ones(8))
     with pytest.raises(ValueError, match="projected has the shape"):
