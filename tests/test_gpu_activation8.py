@@ -309,3 +309,27 @@ def test_tensors_larger_than_the_caches():
     for part in (slice(0, 30000), slice(30000, 70001)):
         qh, eh = pack8(x[part])
         assert torch.equal(q[part], qh) and torch.equal(e[part], eh) and torch.equal(back[part], unpack8(qh, eh))
+
+
+@pytest.mark.parametrize("M,O,I", [(2900003, 768, 32), (4300003, 12, 1024)])
+def test_weight_grad_offsets_past_32_bits(M, O, I):
+    """gradients (or checkpoints) of more than 2^31 values (2^32 bytes), all zero but for the first and the last 200 rows: the product of these 400 (zeros
+    add nothing and round nothing; the tolerance of check_weight_grad with 400 terms)"""
+    import torch
+
+    from ac_solver.agents.activation8 import pack8, unpack8, weight_grad8
+
+    assert max(2 * M * O, M * I) > 1 << 32
+    q = torch.zeros((M, I), device="cuda", dtype=torch.int8)
+    e = torch.full((M, I // 32), 127, device="cuda", dtype=torch.uint8)
+    dy = torch.zeros((M, O), device="cuda", dtype=torch.bfloat16)
+    rows = torch.cat([torch.arange(200), torch.arange(M - 200, M)]).cuda()
+    q[rows], e[rows] = pack8(values(400, I, "float32", 8))
+    dy[rows] = torch.randn((400, O), device="cuda", generator=torch.Generator(device="cuda").manual_seed(9)).to(torch.bfloat16)
+    dw, db = weight_grad8(dy, q, e)
+    xd, yd = unpack8(q[rows], e[rows]).double(), dy[rows].double()
+    adds = 8 * 400 ** 0.5 + 16 + 300
+    err, lim = (dw.double() - yd.t() @ xd).abs(), adds * 2.0 ** -24 * (yd.abs().t() @ xd.abs()) + 1e-37
+    assert not bool((err > lim).any())
+    err, lim = (db.double() - yd.sum(0)).abs(), adds * 2.0 ** -24 * yd.abs().sum(0) + 1e-37
+    assert not bool((err > lim).any())

@@ -282,3 +282,47 @@ def test_a_step_starts_episodes_from_zero_whatever_the_state():
     new, u, ns = recurrent_step(x, p, h, w, s, v, reset=torch.ones(4, dtype=torch.bool, device="cuda"))
     want = recurrent_step(x, p, torch.zeros_like(h), w, s, v)
     assert all(torch.equal(a, b) for a, b in zip((new, u, ns), want))
+
+
+def test_offsets_past_32_bits():
+    """2.16e9 values a tensor: rows do not depend on each other, so the last ones have the bits they have alone; gradients only behind the last 100
+    rows make the sums over the rows theirs"""
+    import torch
+
+    from ac_solver.agents.block_norm import block_output_backward, block_output_forward
+
+    M, D, some = (1 << 21) + 5, 1030, slice(-100, None)
+    x, y, g, w, s, v, dx, du = make(M, D, "bfloat16", 3, "contiguous")
+    assert x.numel() > 1 << 31
+    dx[:-100], du[:-100] = 0, 0
+    new, u, stats = block_output_forward(x, y, g, w, s, v, EPS)
+    grads = block_output_backward(dx, du, x, y, g, w, s, v, stats)
+    last = [t[some] for t in (x, y, g)]
+    new1, u1, stats1 = block_output_forward(*last, w, s, v, EPS)
+    grads1 = block_output_backward(dx[some], du[some], *last, w, s, v, stats1)
+    assert torch.equal(new[some], new1) and torch.equal(u[some], u1) and torch.equal(stats[some], stats1)
+    assert all(torch.equal(a[some], b) for a, b in zip(grads[:3], grads1[:3]))
+    assert not any(bool(a[:-100].any()) for a in grads[:3])
+    ops = [*last, w, s, v]
+    wn, _, wg = definition(*ops, dx[some], du[some])
+    for name, got, want, sums in zip(("weight", "scale", "next_weight"), grads[3:], wg[3:], magnitudes(wn, *ops, dx[some], du[some])):
+        assert_close(got, want, "float32", "d " + name, sums=sums)
+
+
+def test_a_step_past_32_bits_of_offset():
+    import torch
+
+    from ac_solver.agents.recurrence import recurrent_step
+
+    N, D = 2900000, 256
+    g = torch.Generator(device="cuda").manual_seed(4)
+    x = torch.randn((N, D), device="cuda", generator=g, dtype=torch.bfloat16)
+    p = torch.randn((N, 3 * D), device="cuda", generator=g, dtype=torch.bfloat16)
+    h = torch.randn((N, D), device="cuda", generator=g)
+    r = torch.rand(N, device="cuda", generator=g) < 0.1
+    w = torch.rand(D, device="cuda", generator=g)
+    assert p.numel() > 1 << 31
+    out = recurrent_step(x, p, h, w, w, w, reset=r)
+    for part in (slice(0, 1000), slice(-1000, None)):
+        for a, b in zip(out, recurrent_step(x[part], p[part], h[part], w, w, w, reset=r[part])):
+            assert torch.equal(a[part], b)

@@ -401,3 +401,50 @@ def test_tensors_larger_than_the_caches():
         g = gated_scan_backward(cut(dh), cut(dl).contiguous(), args[0], args[1], args[2], half[2])
         assert torch.equal(cut(whole[0]), half[0]) and torch.equal(cut(whole[1]), half[1])
         assert all(torch.equal(cut(a), b) for a, b in zip(grads, g))
+
+
+def test_offsets_past_32_bits():
+    """slices of a projection of 2.15e9 values; the same bits as in halves (a lane walks all steps in either)"""
+    import torch
+
+    from ac_solver.agents.recurrence import gated_scan_backward, gated_scan_forward
+
+    T, N, D = 20, 140000, 256
+    c, z, r, s, dh, dl = inputs(T, N, D, "bfloat16", 6, layout="slices")
+    assert T * c.stride(0) > 1 << 31
+    d_projected = torch.zeros(T, N, 3 * D, device="cuda", dtype=torch.bfloat16)
+    whole = gated_scan_forward(c, z, r, s)
+    grads = gated_scan_backward(dh, dl, c, z, r, whole[2], out=(d_projected[..., :D], d_projected[..., D:2 * D]))
+    assert not bool(d_projected[..., 2 * D:].any())
+    for part in (slice(0, 70000), slice(70000, N)):
+        args = [c[:, part], z[:, part], r[:, part].contiguous(), s[part].contiguous()]
+        half = gated_scan_forward(*args)
+        g = gated_scan_backward(dh[:, part], dl[part].contiguous(), args[0], args[1], args[2], half[2])
+        assert torch.equal(whole[0][:, part], half[0]) and torch.equal(whole[1][part], half[1])
+        assert torch.equal(grads[0][:, part], g[0]) and torch.equal(grads[1][:, part], g[1]) and torch.equal(grads[2][part], g[2])
+
+
+def test_steps_past_32_bits_of_offset():
+    """8.4e6 steps of 280 channels, cut into chunks: the first and the last steps against the definition of 1000 of them.  What 600 steps hand on is the
+    product of 600 gates: sigmoid of normal numbers around 2 with a deviation of 1.5 has a mean logarithm below -0.2 (at the mean it is -0.127, and the
+    logarithm of the sigmoid is concave, with variance 2.25 taking it to about -0.25), so e^-120, far below float32's 2^-24."""
+    import torch
+
+    from ac_solver.agents.recurrence import gated_scan_backward, gated_scan_forward
+
+    T, N, D = (1 << 23) + 3, 4, 70
+    c, z, _, s, dh, dl = inputs(T, N, D, "bfloat16", 7, reset=False)
+    assert c.numel() > 1 << 31
+    hidden, last, bounds = gated_scan_forward(c, z, None, s)
+    dc, dz, ds = gated_scan_backward(dh, dl, c, z, None, bounds)
+    want = definition(c[:1000], z[:1000], None, s, dh[:1000], None)
+    gtop = float(want[2].abs().max()) + float(dh[:1000].abs().max()) * 4
+    assert_close(hidden[:1000], want[0], "bfloat16", "first hidden")
+    assert_close(dc[:400], want[2][:400], "bfloat16", "first d candidate", gtop)
+    assert_close(dz[:400], want[3][:400], "bfloat16", "first d gate", gtop * 4)
+    assert_close(ds, want[4], "float32", "d state", gtop)
+    want = definition(c[-1000:], z[-1000:], None, None, dh[-1000:], dl)
+    assert_close(hidden[-400:], want[0][-400:], "bfloat16", "last hidden")
+    assert_close(last, want[1], "float32", "last")
+    assert_close(dc[-400:], want[2][-400:], "bfloat16", "last d candidate", gtop)
+    assert_close(dz[-400:], want[3][-400:], "bfloat16", "last d gate", gtop * 4)
