@@ -12,7 +12,7 @@
 // Measured: 1 Mi x 256 bf16 forward 0.565 ms (4.75 TB/s of what it moves), backward 0.91 ms (4.7 TB/s), the sums over rows 8 us; 4099 x 2048 f32
 // 30 + 50 + 4 us; one step of 131072 x 256 bf16 0.133 ms (5.0 TB/s).  The backward pass without the next row's operands on the way: 1.28 ms; the
 // forward pass has the waves to hide its loads and loses by it (0.584 ms).
-//   - Sums over rows: every lane adds its features over the rows that its workgroup walks, the workgroup's row groups join in LDS, and a second
+//   - Sums over rows: every lane adds its features over the rows that its workgroup walks, the workgroup's row groups join through the lanes of a wave and LDS, and a second
 //     launch adds the workgroups' partial sums in a fixed order: the result does not depend on which workgroup came first.
 #include <type_traits>
 
@@ -146,7 +146,7 @@ template <class E, int V, int LR, bool STEP> __global__ void __launch_bounds__(k
 template <class E, int V, int LR> __global__ void __launch_bounds__(kThreads<LR>) k_block_bwd(const Args p) {
     constexpr bool kPrecise = sizeof(E) == 4;
     __shared__ float s_red[kThreads<LR> / 64];
-    __shared__ float s_join[kRows<LR> > 1 ? 256 * V : 1];
+    __shared__ float s_join[kRows<LR> > 1 ? 4 * LR * V : 1];
     const int j = LR > 64 ? threadIdx.x : threadIdx.x % LR, d = j * V;
     float w[V], scale[V], next[V], dw[V] = {}, dscale[V] = {}, dnext[V] = {};
     load_weight<V>(p.w, d, p.D, 0.0f, w);
@@ -231,19 +231,20 @@ template <class E, int V, int LR> __global__ void __launch_bounds__(kThreads<LR>
 #pragma unroll
     for (int q = 0; q < 3; q++) {
         float(&acc)[V] = q == 0 ? dw : q == 1 ? dscale : dnext;
-        if constexpr (kRows<LR> > 1) {
-            __syncthreads();
+        if constexpr (kRows<LR> > 1) {  // the row groups of a wave among themselves, then the four waves
 #pragma unroll
-            for (int i = 0; i < V; i++) s_join[(threadIdx.x / LR * V + i) * LR + j] = acc[i];
+            for (int i = 0; i < V; i++)
+#pragma unroll
+                for (int m = LR; m < 64; m *= 2) acc[i] += __shfl_xor(acc[i], m);
+            __syncthreads();
+            if ((threadIdx.x & 63) < LR) {
+#pragma unroll
+                for (int i = 0; i < V; i++) s_join[((threadIdx.x >> 6) * V + i) * LR + j] = acc[i];
+            }
             __syncthreads();
             if (threadIdx.x < LR) {
 #pragma unroll
-                for (int i = 0; i < V; i++) {
-                    float v = 0.0f;
-#pragma unroll
-                    for (int k = 0; k < kRows<LR>; k++) v += s_join[(k * V + i) * LR + j];
-                    acc[i] = v;
-                }
+                for (int i = 0; i < V; i++) acc[i] = (s_join[i * LR + j] + s_join[(V + i) * LR + j]) + (s_join[(2 * V + i) * LR + j] + s_join[(3 * V + i) * LR + j]);
             }
         }
         if (LR > 64 || threadIdx.x < LR) {
@@ -286,12 +287,13 @@ __global__ void __launch_bounds__(1024) k_block_sum(const float* __restrict__ pa
 constexpr int kMaxWidth = 4096;  // 1024 lanes with a vector of 4 each; with two they would spill
 
 // lanes of a row, by its vectors: fn(V, LR, workgroup).  16-byte loads, but for 16-bit rows of more than 2048 (a vector of 8 in each
-// of 1024 lanes would spill).
+// of 1024 lanes would spill).  Rows of one or two vectors take two lanes: 487495 x 2 f16 12 + 40 us (forward, backward), 41 + 108 with eight.
 template <class E, class F> static void with_shape(int64_t D, F&& fn) {
     using std::integral_constant;
     auto narrow = [&](auto v) {
         const int n = (int)((D + decltype(v)::value - 1) / decltype(v)::value);
-        if (n <= 8) fn(v, integral_constant<int, 8>{}, 256);
+        if (n <= 2) fn(v, integral_constant<int, 2>{}, 256);
+        else if (n <= 8) fn(v, integral_constant<int, 8>{}, 256);
         else if (n <= 16) fn(v, integral_constant<int, 16>{}, 256);
         else if (n <= 32) fn(v, integral_constant<int, 32>{}, 256);
         else if (n <= 64) fn(v, integral_constant<int, 64>{}, 256);

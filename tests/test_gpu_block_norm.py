@@ -284,6 +284,12 @@ def test_a_step_starts_episodes_from_zero_whatever_the_state():
     assert all(torch.equal(a, b) for a, b in zip((new, u, ns), want))
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("D", [2, 8, 13, 17])
+def test_many_narrow_rows(D, dtype):
+    check(140001, D, dtype)
+
+
 def test_offsets_past_32_bits():
     """2.16e9 values a tensor: rows do not depend on each other, so the last ones have the bits they have alone; gradients only behind the last 100
     rows make the sums over the rows theirs"""
