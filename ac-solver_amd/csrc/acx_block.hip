@@ -284,10 +284,12 @@ __global__ void __launch_bounds__(1024) k_block_sum(const float* __restrict__ pa
     }
 }
 
-constexpr int kMaxWidth = 4096;  // 1024 lanes with a vector of 4 each; with two they would spill
+constexpr int kMaxWidth = 4096;  // a workgroup's lanes with a vector each
 
-// lanes of a row, by its vectors: fn(V, LR, workgroup).  16-byte loads, but for 16-bit rows of more than 2048 (a vector of 8 in each
-// of 1024 lanes would spill).  Rows of one or two vectors take two lanes: 487495 x 2 f16 12 + 40 us (forward, backward), 41 + 108 with eight.
+// lanes of a row, by its vectors: fn(V, LR, workgroup).  16-byte loads.  (16-bit rows of more than 2048 with 8-byte ones in up to 1024
+// lanes, which have no registers left for the next row: 56005 x 3302 bf16 632 + 1354 us forward and backward, 396 + 860 like this; float32
+// ones keep to 1024 lanes, 16001 x 2050 takes 183 + 357 us with 32 bytes a lane and 136 + 297 with 16.)  Rows of one or two vectors take
+// two lanes: 487495 x 2 f16 12 + 40 us, 41 + 108 with eight.
 template <class E, class F> static void with_shape(int64_t D, F&& fn) {
     using std::integral_constant;
     auto narrow = [&](auto v) {
@@ -301,19 +303,24 @@ template <class E, class F> static void with_shape(int64_t D, F&& fn) {
     };
     if constexpr (sizeof(E) == 2) {
         if (D <= 2048) narrow(integral_constant<int, 8>{});
-        else fn(integral_constant<int, 4>{}, integral_constant<int, 1024>{}, (int)(D + 255) / 256 * 64);
+        else fn(integral_constant<int, 8>{}, integral_constant<int, 512>{}, (int)(D + 511) / 512 * 64);
     } else {
         if (D <= 1024) narrow(integral_constant<int, 4>{});
         else if (D <= 2048) fn(integral_constant<int, 4>{}, integral_constant<int, 512>{}, (int)(D + 255) / 256 * 64);
         else fn(integral_constant<int, 4>{}, integral_constant<int, 1024>{}, (int)(D + 255) / 256 * 64);
     }
 }
-// as many workgroups as stay resident: what is gained by more is less than their partial sums cost
-static int64_t workgroups(int64_t M, int lr, int threads) {
+// About as many workgroups as stay resident (what is gained by more is less than their partial sums cost), the same number for each of the 256
+// compute units: 819 of 320 lanes on 49016 x 1104 f32, the backward pass takes 592 us and 484 with 768, because 51 of them start
+// when the others end.
+static int64_t workgroups(int64_t M, int lr, int threads, int lanes = 1024) {
     const int rows = lr > 64 ? 1 : 256 / lr;
-    const int64_t n = (M + rows - 1) / rows, most = 262144 / threads;
+    const int64_t n = (M + rows - 1) / rows, most = lanes / threads * 256;
     return n < most ? n : most;
 }
+// (the forward pass has no partial sums and fewer registers: with 1024 lanes a compute unit workgroups of 576 to 960 would be alone on one; 16001 x 2050
+// f32 136 us, 162 with one each; 56005 x 3302 bf16, 448 lanes, 396 us with two each, 458 with four)
+static int forward_lanes(int threads) { return threads > 512 ? 1920 : 1024; }
 static int64_t partial_floats(int64_t M, int64_t D, int dtype) {
     int64_t n = 0;
     with_element(dtype, [&](auto* e) {
@@ -354,7 +361,7 @@ extern "C" int acx_block_forward(const void* d_x, int64_t x_row, const void* d_y
         using E = std::remove_pointer_t<decltype(e)>;
         block::with_shape<E>(D, [&](auto v, auto lr, int threads) {
             constexpr int LR = decltype(lr)::value;
-            hipLaunchKernelGGL((block::k_block_fwd<E, decltype(v)::value, LR, false>), dim3((unsigned)block::workgroups(M, LR, threads)), dim3(threads), 0, (hipStream_t)stream, a);
+            hipLaunchKernelGGL((block::k_block_fwd<E, decltype(v)::value, LR, false>), dim3((unsigned)block::workgroups(M, LR, threads, block::forward_lanes(threads))), dim3(threads), 0, (hipStream_t)stream, a);
         });
     });
     ACX_HIP_TRY(hipGetLastError());
@@ -375,7 +382,7 @@ extern "C" int acx_block_step(const void* d_x, int64_t x_row, const void* d_proj
         using E = std::remove_pointer_t<decltype(e)>;
         block::with_shape<E>(D, [&](auto v, auto lr, int threads) {
             constexpr int LR = decltype(lr)::value;
-            hipLaunchKernelGGL((block::k_block_fwd<E, decltype(v)::value, LR, true>), dim3((unsigned)block::workgroups(M, LR, threads)), dim3(threads), 0, (hipStream_t)stream, a);
+            hipLaunchKernelGGL((block::k_block_fwd<E, decltype(v)::value, LR, true>), dim3((unsigned)block::workgroups(M, LR, threads, block::forward_lanes(threads))), dim3(threads), 0, (hipStream_t)stream, a);
         });
     });
     ACX_HIP_TRY(hipGetLastError());

@@ -332,3 +332,10 @@ def test_a_step_past_32_bits_of_offset():
     for part in (slice(0, 1000), slice(-1000, None)):
         for a, b in zip(out, recurrent_step(x[part], p[part], h[part], w, w, w, reset=r[part])):
             assert torch.equal(a[part], b)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("D", [1104, 2050, 2712, 3302, 4096])
+def test_wide_rows_walk_the_grid(D, dtype):
+    """more rows than workgroups, of every size that a wide row takes"""
+    check(3001, D, dtype)
