@@ -86,11 +86,17 @@ def packing():
     return getattr(_inside, "depth", 0) > 0
 
 
+def _is_leaf(t):
+    """whether t is a leaf (a parameter, an input) or a view of one: torch's linear layer keeps the transpose of its weight.  (A view that a function made
+    without recording it has a base without a gradient of its own: the function's result, not a leaf.)"""
+    return t.grad_fn is None or (t._base is not None and t._base.is_leaf and t._base.requires_grad)
+
+
 class checkpoint8(torch.autograd.graph.saved_tensors_hooks):
     """`with checkpoint8(): ...` -- what autograd keeps of the activations computed inside the block is kept in 8 bits (pack8) and restored
     in the backward pass: a quarter (float32) or half (16 bits) of the memory; the gradients are those of the restored values (row
-    statistics and states that an operator kept beside them stay what they were).  Kept as they are: leaves (parameters, inputs),
-    vectors, tensors of fewer than 4096 values or with rows of more than 2^20, whole numbers, tensors on the CPU."""
+    statistics and states that an operator kept beside them stay what they were).  Kept as they are: leaves (parameters, inputs) and
+    their views, vectors, tensors of fewer than 4096 values or with rows of more than 2^20, whole numbers, tensors on the CPU."""
 
     def __init__(self):
         super().__init__(self._keep, self._restore)
@@ -105,7 +111,7 @@ class checkpoint8(torch.autograd.graph.saved_tensors_hooks):
 
     @staticmethod
     def _keep(t):
-        if t.dtype not in DTYPES or not t.is_cuda or t.dim() < 2 or t.numel() < MIN_VALUES or t.shape[-1] > MAX_WIDTH or t.grad_fn is None:
+        if t.dtype not in DTYPES or not t.is_cuda or t.dim() < 2 or t.numel() < MIN_VALUES or t.shape[-1] > MAX_WIDTH or _is_leaf(t):
             return t
         return _Packed(t)
 

@@ -333,3 +333,55 @@ def test_weight_grad_offsets_past_32_bits(M, O, I):
     assert not bool((err > lim).any())
     err, lim = (db.double() - yd.sum(0)).abs(), adds * 2.0 ** -24 * yd.abs().sum(0) + 1e-37
     assert not bool((err > lim).any())
+
+
+FORMS_OF_A_LEAF = {
+    "view": lambda a: a.view(5, 60, 256),
+    "transpose": lambda a: a.t(),
+    "slice": lambda a: a[:, 3:131],
+    "select": lambda a: a.view(5, 60, 256)[2],
+    "split": lambda a: a.split(128, 1)[1],
+    "unbind": lambda a: a.view(2, 150, 256).unbind(0)[1],
+    "expand": lambda a: a.unsqueeze(0).expand(2, 300, 256),
+    "view of a view": lambda a: a.t()[:100].unsqueeze(1),
+}
+
+
+@pytest.mark.parametrize("form", sorted(FORMS_OF_A_LEAF))
+def test_checkpoint8_keeps_views_of_leaves(form):
+    """a leaf in another shape is still the leaf: the gradient is the one outside the block, bit by bit"""
+    import torch
+
+    from ac_solver.agents.activation8 import checkpoint8
+
+    a = torch.randn(300, 256, device="cuda", requires_grad=True)
+    with checkpoint8():
+        out = FORMS_OF_A_LEAF[form](a).square()
+    d = torch.randn_like(out)
+    (got,) = torch.autograd.grad(out, a, d)
+    (want,) = torch.autograd.grad(FORMS_OF_A_LEAF[form](a).square(), a, d)
+    assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("shape", [(300, 256), (3, 100, 256)])
+def test_checkpoint8_around_a_plain_layer(shape):
+    """torch's own linear layer keeps a transposed view of its weight: that one stays exact, its input is kept in 8 bits.  The gradient of the weight is a sum of
+    300 products in float32, in whatever order the library takes: at most 300 roundings of 2^-24 of the magnitudes."""
+    import torch
+
+    from ac_solver.agents.activation8 import checkpoint8, pack8, unpack8
+
+    torch.manual_seed(3)
+    layer = torch.nn.Linear(256, 192).cuda()
+    x = torch.randn(*shape, device="cuda", requires_grad=True)
+    u = x * 1.0
+    with checkpoint8():
+        out = layer(u)
+    plain = layer(u)
+    d = torch.randn_like(out)
+    dx, dw, db = torch.autograd.grad(out, (x, layer.weight, layer.bias), d, retain_graph=True)
+    wx, ww, wb = torch.autograd.grad(plain, (x, layer.weight, layer.bias), d)
+    assert torch.equal(dx, wx) and torch.equal(db, wb)
+    kept, d2 = unpack8(*pack8(u.detach())).double().view(-1, 256), d.double().view(-1, 192)
+    assert bool(((dw.double() - d2.t() @ kept).abs() <= 300 * 2.0 ** -24 * (d2.abs().t() @ kept.abs())).all())
+    assert not torch.equal(dw, ww)  # (the input is an activation: it is in 8 bits)
