@@ -86,17 +86,31 @@ def packing():
     return getattr(_inside, "depth", 0) > 0
 
 
+# nodes of autograd that hand a tensor on with the same values, up to a rounding to another type (their names without the number behind them)
+_SAME_VALUES = frozenset(n + "Backward" for n in ("Alias AsStrided Clone Diagonal Expand Movedim Permute ReshapeAlias Select Slice Split SplitWithSizes Squeeze T ToCopy Transpose Unbind "
+                                                  "Unfold UnsafeSplit UnsafeView Unsqueeze View").split())
+
+
 def _is_leaf(t):
-    """whether t is a leaf (a parameter, an input) or a view of one: torch's linear layer keeps the transpose of its weight.  (A view that a function made
-    without recording it has a base without a gradient of its own: the function's result, not a leaf.)"""
-    return t.grad_fn is None or (t._base is not None and t._base.is_leaf and t._base.requires_grad)
+    """whether t is a leaf (a parameter, an input), a view of one, or a copy of one in another type or layout: torch's linear layer keeps the transpose of
+    its weight, in bfloat16 that of a copy which autocast made.  (A view that a function made without recording it has a base without a
+    gradient of its own: the function's result, not a leaf.)"""
+    if t.grad_fn is None or (t._base is not None and t._base.is_leaf and t._base.requires_grad):
+        return True
+    node = t.grad_fn
+    while node.name().rstrip("0123456789") in _SAME_VALUES:
+        node = node.next_functions[0][0]
+        if node is None:
+            return True
+    return node.name().endswith("AccumulateGrad")
 
 
 class checkpoint8(torch.autograd.graph.saved_tensors_hooks):
     """`with checkpoint8(): ...` -- what autograd keeps of the activations computed inside the block is kept in 8 bits (pack8) and restored
     in the backward pass: a quarter (float32) or half (16 bits) of the memory; the gradients are those of the restored values (row
-    statistics and states that an operator kept beside them stay what they were).  Kept as they are: leaves (parameters, inputs) and
-    their views, vectors, tensors of fewer than 4096 values or with rows of more than 2^20, whole numbers, tensors on the CPU."""
+    statistics and states that an operator kept beside them stay what they were).  Kept as they are: leaves (parameters, inputs), their
+    views and their copies in other types, vectors, tensors of fewer than 4096 values or with rows of more than 2^20, whole numbers, tensors
+    on the CPU."""
 
     def __init__(self):
         super().__init__(self._keep, self._restore)

@@ -385,3 +385,40 @@ def test_checkpoint8_around_a_plain_layer(shape):
     kept, d2 = unpack8(*pack8(u.detach())).double().view(-1, 256), d.double().view(-1, 192)
     assert bool(((dw.double() - d2.t() @ kept).abs() <= 300 * 2.0 ** -24 * (d2.abs().t() @ kept.abs())).all())
     assert not torch.equal(dw, ww)  # (the input is an activation: it is in 8 bits)
+
+
+def test_checkpoint8_keeps_copies_of_leaves_in_other_types():
+    """a layer in bfloat16 reads a bfloat16 copy of its float32 weight, autocast makes that copy itself: the gradient of the input is the one outside the
+    block, bit by bit; a clone and a contiguous transpose of a leaf are kept, too"""
+    import contextlib
+
+    import torch
+    from torch.nn import functional as F
+
+    from ac_solver.agents.activation8 import checkpoint8
+
+    torch.manual_seed(4)
+    w = torch.randn(192, 256, device="cuda", requires_grad=True)
+    x = torch.randn(300, 256, device="cuda", requires_grad=True)
+
+    def cast(block):
+        with block:
+            return F.linear((x * 1.0).bfloat16(), w.bfloat16())
+
+    def cast_of_a_view(block):
+        with block:
+            return (x * 1.0).bfloat16() @ w.t().bfloat16()
+
+    def autocast(block):
+        with block, torch.autocast("cuda", torch.bfloat16):
+            return F.linear(x * 1.0, w)
+
+    for f in (cast, cast_of_a_view, autocast):
+        got, want = f(checkpoint8()), f(contextlib.nullcontext())
+        d = torch.randn_like(got)
+        assert torch.equal(torch.autograd.grad(got, x, d)[0], torch.autograd.grad(want, x, d)[0]), f.__name__
+    for f in (lambda: w.clone().square(), lambda: w.t().contiguous().square(), lambda: w.double().float().square()):
+        with checkpoint8():
+            got = f()
+        d = torch.randn_like(got)
+        assert torch.equal(torch.autograd.grad(got, w, d)[0], torch.autograd.grad(f(), w, d)[0])
