@@ -109,8 +109,8 @@ class checkpoint8(torch.autograd.graph.saved_tensors_hooks):
     """`with checkpoint8(): ...` -- what autograd keeps of the activations computed inside the block is kept in 8 bits (pack8) and restored
     in the backward pass: a quarter (float32) or half (16 bits) of the memory; the gradients are those of the restored values (row
     statistics and states that an operator kept beside them stay what they were).  Kept as they are: leaves (parameters, inputs), their
-    views and their copies in other types, vectors, tensors of fewer than 4096 values or with rows of more than 2^20, whole numbers, tensors
-    on the CPU."""
+    views and their copies in other types, vectors, tensors with one value a row (row statistics), of fewer than 4096 values or with rows of more
+    than 2^20, whole numbers, tensors on the CPU."""
 
     def __init__(self):
         super().__init__(self._keep, self._restore)
@@ -125,7 +125,7 @@ class checkpoint8(torch.autograd.graph.saved_tensors_hooks):
 
     @staticmethod
     def _keep(t):
-        if t.dtype not in DTYPES or not t.is_cuda or t.dim() < 2 or t.numel() < MIN_VALUES or t.shape[-1] > MAX_WIDTH or _is_leaf(t):
+        if t.dtype not in DTYPES or not t.is_cuda or t.dim() < 2 or t.numel() < MIN_VALUES or not 1 < t.shape[-1] <= MAX_WIDTH or _is_leaf(t):
             return t
         return _Packed(t)
 

@@ -422,3 +422,20 @@ def test_checkpoint8_keeps_copies_of_leaves_in_other_types():
             got = f()
         d = torch.randn_like(got)
         assert torch.equal(torch.autograd.grad(got, w, d)[0], torch.autograd.grad(f(), w, d)[0])
+
+
+def test_checkpoint8_keeps_one_value_a_row():
+    """a column of row statistics (the reciprocal root of a norm) would take two bytes a value, and every value of its row hangs on it: kept as it is"""
+    import torch
+
+    from ac_solver.agents.activation8 import checkpoint8
+
+    a = torch.randn(8192, 8, device="cuda", requires_grad=True)
+
+    def f():
+        return torch.rsqrt(a.square().mean(-1, keepdim=True) + 1e-6)
+
+    with checkpoint8():
+        out = f()
+    d = torch.randn_like(out)
+    assert out.numel() == 8192 and torch.equal(torch.autograd.grad(out, a, d)[0], torch.autograd.grad(f(), a, d)[0])
