@@ -126,7 +126,7 @@ class checkpoint8(torch.autograd.graph.saved_tensors_hooks):
     @staticmethod
     def _keep(t):
         if t.dtype not in DTYPES or not t.is_cuda or t.dim() < 2 or t.numel() < MIN_VALUES or not 1 < t.shape[-1] <= MAX_WIDTH or _is_leaf(t):
-            return t
+            return t.detach()  # (autograd hangs it back into its graph; t itself, if its own node keeps it, would hold that node, and the graph behind it, for good)
         return _Packed(t)
 
     @staticmethod

@@ -179,3 +179,26 @@ def test_the_recurrent_agent_needs_a_gpu_and_says_so():
         R.recurrent_block(torch.zeros(4, 8), torch.zeros(4, 24), None, torch.ones(8))
     with pytest.raises(ValueError, match="projected has the shape"):
         R.recurrent_block(torch.zeros(2, 4, 8), torch.zeros(2, 4, 16), None, torch.ones(8))
+
+
+def test_checkpoint8_holds_no_graph_that_nobody_else_holds():
+    """an output that its own node keeps (tanh) goes with the last reference to it, also where no backward pass runs; second derivatives pass through"""
+    import gc
+    import weakref
+
+    from ac_solver.agents.activation8 import checkpoint8
+
+    a = torch.randn(64, 4, requires_grad=True)
+    with checkpoint8():
+        y = torch.tanh(a * 1.0)
+    gone = weakref.ref(y)
+    del y
+    gc.collect()
+    assert gone() is None
+    with checkpoint8():
+        y = torch.tanh(a * 1.0)
+    (g,) = torch.autograd.grad(y.sum(), a, create_graph=True)
+    (h,) = torch.autograd.grad(g.sum(), a)
+    t = torch.tanh(a.detach().double())
+    # 1 - t^2 and 2 t: at most eight roundings of values of at most 2
+    assert float((h.double() + 2 * t * (1 - t * t)).abs().max()) <= 16 * 2.0 ** -24
