@@ -75,6 +75,27 @@ class _Packed:
         self.q, self.exponent = pack8(t)
         self.dtype = t.dtype
 
+    def restore(self):
+        return unpack8(self.q, self.exponent, self.dtype)
+
+
+class _Kept:
+    """a tensor that autograd saved, as it is.  (Detached: autograd hangs it back into its graph; the tensor itself, if its own node keeps it, would hold that
+    node, and the graph behind it, for good.)  Autograd leaves it to the hooks to notice that it has been changed in place since."""
+
+    __slots__ = ("tensor", "version")
+
+    def __init__(self, t):
+        self.tensor = t.detach()
+        self.version = None if t.is_inference() else t._version
+
+    def restore(self):
+        t = self.tensor
+        if self.version is not None and t._version != self.version:
+            raise RuntimeError(f"one of the variables needed for gradient computation has been modified by an inplace operation: {tuple(t.shape)} of {t.dtype} is at version "
+                               f"{t._version}, expected version {self.version}")
+        return t
+
 
 MIN_VALUES = 1 << 12  # a tensor worth a launch
 MAX_WIDTH = 1 << 20  # of pack8
@@ -126,9 +147,9 @@ class checkpoint8(torch.autograd.graph.saved_tensors_hooks):
     @staticmethod
     def _keep(t):
         if t.dtype not in DTYPES or not t.is_cuda or t.dim() < 2 or t.numel() < MIN_VALUES or not 1 < t.shape[-1] <= MAX_WIDTH or _is_leaf(t):
-            return t.detach()  # (autograd hangs it back into its graph; t itself, if its own node keeps it, would hold that node, and the graph behind it, for good)
+            return _Kept(t)
         return _Packed(t)
 
     @staticmethod
     def _restore(kept):
-        return unpack8(kept.q, kept.exponent, kept.dtype) if isinstance(kept, _Packed) else kept
+        return kept.restore()

@@ -202,3 +202,19 @@ def test_checkpoint8_holds_no_graph_that_nobody_else_holds():
     t = torch.tanh(a.detach().double())
     # 1 - t^2 and 2 t: at most eight roundings of values of at most 2
     assert float((h.double() + 2 * t * (1 - t * t)).abs().max()) <= 16 * 2.0 ** -24
+
+
+def test_checkpoint8_notices_in_place_changes_of_what_it_kept_as_it_was():
+    """as autograd itself does: no gradient from a tensor that has changed since"""
+    from ac_solver.agents.activation8 import checkpoint8
+
+    a, b = torch.randn(64, 4, requires_grad=True), torch.randn(64, 4)
+    with checkpoint8():
+        out = a * b
+    b.add_(1.0)
+    with pytest.raises(RuntimeError, match="inplace"):
+        out.sum().backward()
+    with checkpoint8():
+        out = a * b
+    d = torch.randn(64, 4)
+    assert torch.equal(torch.autograd.grad(out, a, d, retain_graph=True)[0], d * b) and torch.equal(torch.autograd.grad(out, a, d)[0], d * b)
