@@ -70,6 +70,15 @@ std::string type_text(at::ScalarType t) {
     }
 }
 
+struct NoForwardMode : std::runtime_error {  // (NotImplementedError, as torch raises for its own functions)
+    using std::runtime_error::runtime_error;
+};
+// Every operand that can carry one passes here: outputs without its tangent would read as a derivative of zero.  (Inside a function of autograd forward
+// mode is off, and there is nothing to be seen: the operands are looked at in front of it, by wants_grad.)
+void require_no_tangent(const Tensor& t, const char* name) {
+    if (t._fw_grad(0).defined()) throw NoForwardMode(std::string(name) + " has a tangent: forward mode derivatives of this operator are not implemented");
+}
+
 Tensor tensor(py::handle o, const char* name) {
     if (!THPVariable_Check(o.ptr())) type_error(std::string(name) + " has to be a tensor, not " + Py_TYPE(o.ptr())->tp_name);
     return THPVariable_Unpack(o.ptr());
@@ -85,6 +94,7 @@ int code_of(at::ScalarType t) { return t == at::kFloat ? ACX_F32 : t == at::kBFl
 // of a sum).
 Tensor activation(Tensor t, const char* name, const Tensor* like = nullptr, std::optional<at::IntArrayRef> shape = std::nullopt) {
     if (code_of(t.scalar_type()) < 0) type_error(std::string(name) + " has to be float32, bfloat16 or float16, not " + type_text(t.scalar_type()));
+    require_no_tangent(t, name);
     if (like && (t.scalar_type() != like->scalar_type() || t.device() != like->device()))
         value_error(std::string(name) + " is " + type_text(t.scalar_type()) + " on " + t.device().str() + ", the other activations are " + type_text(like->scalar_type()) + " on " +
                     like->device().str());
@@ -95,6 +105,7 @@ Tensor activation(Tensor t, const char* name, const Tensor* like = nullptr, std:
 // a contiguous tensor of exactly this type, shape and device (parameters, states)
 Tensor plain(Tensor t, const char* name, at::IntArrayRef shape, at::Device device, at::ScalarType type = at::kFloat) {
     if (t.scalar_type() != type) type_error(std::string(name) + " has to be " + type_text(type) + ", not " + type_text(t.scalar_type()));
+    require_no_tangent(t, name);
     if (t.sizes() != shape) value_error(std::string(name) + " has the shape " + shape_text(t.sizes()) + ", expected " + shape_text(shape));
     if (t.device() != device) value_error(std::string(name) + " lives on " + t.device().str() + ", the activations on " + device.str());
     return t.is_contiguous() ? t : t.contiguous();
@@ -160,6 +171,8 @@ Maybe scratch(int64_t bytes, const Tensor& like) {
 }
 int64_t bytes_of(const Maybe& t) { return t ? t->numel() : 0; }
 bool wants_grad(std::initializer_list<const Maybe*> ts) {
+    for (const Maybe* t : ts)
+        if (*t) require_no_tangent(**t, "an operand");
     if (!at::GradMode::is_enabled()) return false;
     for (const Maybe* t : ts)
         if (*t && (*t)->requires_grad()) return true;
@@ -539,6 +552,8 @@ PYBIND11_MODULE(acx_torch, m) {
                 if (p) std::rethrow_exception(p);
             } catch (const AcxFailure& e) {
                 PyErr_SetString(error, e.what());
+            } catch (const NoForwardMode& e) {
+                PyErr_SetString(PyExc_NotImplementedError, e.what());
             }
         });
     });

@@ -448,3 +448,37 @@ def test_steps_past_32_bits_of_offset():
     assert_close(last, want[1], "float32", "last")
     assert_close(dc[-400:], want[2][-400:], "bfloat16", "last d candidate", gtop)
     assert_close(dz[-400:], want[3][-400:], "bfloat16", "last d gate", gtop * 4)
+
+
+def test_forward_mode_is_refused():
+    """a tangent on an operand, or on the gradient that a backward pass starts from, is not dropped silently"""
+    import torch
+    import torch.autograd.forward_ad as forward_ad
+
+    from ac_solver.agents.activation8 import linear8
+    from ac_solver.agents.block_norm import block_input, block_output, block_output_backward, block_output_forward
+    from ac_solver.agents.recurrence import gated_scan, gated_scan_backward, gated_scan_forward, recurrent_block
+
+    c, z, r, s, dh, dl = inputs(6, 2, 8, "float32", 2)
+    w, p = torch.ones(8, device="cuda"), torch.cat((c, z, dh), dim=-1)
+    calls = ((lambda t: gated_scan(t, z)[0], c), (lambda t: gated_scan(c, z, state=t)[0], s), (lambda t: block_output(c, t, z, w, w, w)[0], dh), (lambda t: block_output(c, z, dh, t)[0], w),
+             (lambda t: block_input(t, w), c), (lambda t: recurrent_block(c, t, None, w)[0], p), (lambda t: linear8(t, torch.ones(3, 8, device="cuda")), c))
+    for f, t in calls:
+        with forward_ad.dual_level():
+            with pytest.raises(NotImplementedError):
+                f(forward_ad.make_dual(t, torch.ones_like(t)))
+            with pytest.raises(NotImplementedError):
+                f(forward_ad.make_dual(t.clone().requires_grad_(), torch.ones_like(t)))
+        leaf = t.clone().requires_grad_()
+        out = f(leaf)
+        with forward_ad.dual_level(), pytest.raises(RuntimeError, match="forward mode"):
+            if t.dim() == 3 and out.shape[-1] == 3:  # (linear8's gradient of x is torch's own, which has a tangent: take the weight's)
+                weight = torch.ones(3, 8, device="cuda", requires_grad=True)
+                out, leaf = linear8(t, weight), weight
+            torch.autograd.grad(out, leaf, forward_ad.make_dual(torch.ones_like(out), torch.ones_like(out)))
+    _, _, bounds = gated_scan_forward(c, z, r, s)
+    _, _, stats = block_output_forward(c, z, dh, w, w, w)
+    for f, args, places in ((gated_scan_backward, [dh, dl, c, z, None, bounds], (0, 1, 5)), (block_output_backward, [dh, dh, c, z, dh, w, w, w, stats], (0, 1, 8))):
+        for k in places:
+            with forward_ad.dual_level(), pytest.raises(NotImplementedError, match="forward mode"):
+                f(*args[:k], forward_ad.make_dual(args[k], torch.ones_like(args[k])), *args[k + 1:])

@@ -218,3 +218,36 @@ def test_checkpoint8_notices_in_place_changes_of_what_it_kept_as_it_was():
         out = a * b
     d = torch.randn(64, 4)
     assert torch.equal(torch.autograd.grad(out, a, d, retain_graph=True)[0], d * b) and torch.equal(torch.autograd.grad(out, a, d)[0], d * b)
+
+
+def test_forward_mode_tangents_are_refused_not_dropped():
+    """an operand with a tangent, with or without a gradient of its own, in every function: the outputs would carry none, which reads as a derivative of zero
+    (what the backward functions look at behind the place of the tensors needs a GPU)"""
+    import torch.autograd.forward_ad as forward_ad
+
+    from ac_solver.agents import activation8 as A
+    from ac_solver.agents import block_norm as B
+
+    c, z = scan_args()
+    x, w, p, h = torch.zeros(5, 8), torch.ones(8), torch.zeros(5, 24), torch.zeros(5, 8)
+    s, bounds, stats = torch.zeros(2, 4), torch.zeros(8), torch.zeros(5, 2)
+    q, e = torch.zeros(5, 8, dtype=torch.int8), torch.zeros(5, 1, dtype=torch.uint8)
+    calls = [(R.gated_scan, [c, z, None, s], (0, 1, 3)), (R.gated_scan_forward, [c, z, None, s], (0, 1, 3)),
+             (R.gated_scan_backward, [c, s, c, z, None, bounds], (2, 3)), (B.block_output, [x, x, x, w, w, w], (0, 1, 2, 3, 4, 5)), (B.block_input, [x, w], (0, 1)),
+             (B.block_output_forward, [x, x, x, w, w, w], (0, 1, 2, 3, 4, 5)), (B.block_output_backward, [x, x, x, x, x, w, w, w, stats], (2, 3, 4, 5, 6, 7)),
+             (R.recurrent_block, [x[None], p[None], h, w, w, w], (0, 1, 2, 3, 4, 5)), (R.recurrent_step, [x, p, h, w, w, w], (0, 1, 2, 3, 4, 5)),
+             (A.pack8, [x], (0,)), (A.weight_grad8, [x, q, e], (0,))]
+    for f, args, places in calls:
+        for k in places:
+            for grad in (False, True):
+                with forward_ad.dual_level():
+                    mine = list(args)
+                    mine[k] = forward_ad.make_dual(args[k].clone().requires_grad_(grad), torch.ones_like(args[k]))
+                    with pytest.raises(NotImplementedError, match="forward mode"):
+                        f(*mine)
+        with pytest.raises(ValueError, match="GPU"):  # without a tangent only the place is wrong
+            f(*args)
+    with forward_ad.dual_level():  # (outside a level, or with forward mode off, there are no tangents)
+        d = forward_ad.make_dual(c, torch.ones_like(c))
+        with forward_ad._set_fwd_grad_enabled(False), pytest.raises(ValueError, match="GPU"):
+            R.gated_scan(d, z)
