@@ -12,13 +12,14 @@ from ac_solver.agents._ops import DTYPES, ops
 def pack8(x):
     """x [..., width] (float32, bfloat16 or float16) -> (q [..., width] int8, exponent [..., ceil(width / 32)] uint8): the value kept for x
     is q * 2^(exponent - 127), with one exponent for 32 neighbouring features -- the smallest for which the largest of them rounds to at
-    most 127, so the error is at most 2^-7 of that largest one (rows of up to 2^20 features).  A block that holds an infinity or a NaN is marked (exponent 255) and
-    restores to NaN."""
+    most 127, so the error is at most 1/127 of that largest one, or 2^-127 (rows of up to 2^20 features).  A block that holds an infinity or a NaN is marked (exponent
+    255) and restores to NaN; finite values restore to finite ones (see unpack8)."""
     return ops.pack8(x)
 
 
 def unpack8(q, exponent, dtype=torch.float32):
-    """the values that a checkpoint of pack8 stands for, rounded to `dtype` (exact in float32 and bfloat16)"""
+    """the values that a checkpoint of pack8 stands for, rounded to `dtype` (exact in float32 and bfloat16); what lies above the largest finite value of `dtype`
+    (float16's 65504 is kept as 64 * 2^10, float32's largest as 64 * 2^122) becomes that largest value"""
     if not isinstance(dtype, torch.dtype):
         raise TypeError(f"dtype has to be a torch type, not {type(dtype).__name__}")
     return ops.unpack8(q, exponent, dtype)
@@ -26,8 +27,8 @@ def unpack8(q, exponent, dtype=torch.float32):
 
 def weight_grad8(d_out, q, exponent):
     """The gradients of weight and bias of a linear layer whose input was kept by pack8: d_out [..., outputs] (float32, bfloat16 or float16),
-    q [..., inputs] -> (d_out^T x [outputs, inputs], sum of d_out [outputs]), both float32, x the values the checkpoint stands for; float32
-    accuracy for every type of d_out.  Up to 65536 outputs and inputs, 2^29 weights."""
+    q [..., inputs] -> (d_out^T x [outputs, inputs], sum of d_out [outputs]), both float32, x the values the checkpoint stands for (unpack8 in
+    bfloat16); float32 accuracy for every type of d_out.  Up to 65536 outputs and inputs, 2^29 weights."""
     return ops.weight_grad8(d_out, q, exponent)
 
 

@@ -8,7 +8,8 @@
 // matrix instructions without rounding the checkpoint again.  dy is brought there without rounding either: a float32 is the sum of three
 // bfloat16 (8 + 8 + 8 bits, each the truncated rest of the last), a float16 of two, a bfloat16 of one; the accumulators are float32.  So dW has
 // the accuracy of a float32 product, at one to three times the matrix work of a bf16 one and 1 byte instead of 4 read per x.
-// A block with an infinity or a NaN is marked with the exponent byte 255 and restores to NaN: it is not hidden.
+// A block with an infinity or a NaN is marked with the exponent byte 255 and restores to NaN: it is not hidden.  Finite values restore to finite ones: where rounding up left
+// the type, to its largest.
 // Measured: 1 Mi x 256 f32 packed in 0.273 ms and restored in 0.273 ms (4.95 TB/s).  Weight gradient of 1 Mi rows, 768 x 256: dy bf16 0.53 ms (4.5 TB/s,
 // memory), dy f32 1.19 ms: 1.24 PFLOP of bf16 products at 1.04 PFLOP/s, where the chip's clock drops to 1.5 GHz under the matrix units' load
 // (a library's bf16 product of 8192^3: 1.16 PFLOP/s).  65537 x 256 x 72 bf16 20 + 5 us: five steps a workgroup, their latency and the join.
@@ -79,18 +80,32 @@ template <class E, int V, bool STREAM> __global__ void __launch_bounds__(256) k_
     const int64_t row = l / lpr;
     if (row >= M) return;
     const int j = (int)(l - row * lpr), d = j * V, valid = K - d;
-    const float factor = exponent_factor(exps[row * ((K + kBlock - 1) / kBlock) + d / kBlock]);
+    const uint32_t e = exps[row * ((K + kBlock - 1) / kBlock) + d / kBlock];
+    const float factor = exponent_factor(e);
+    // Rounding up to the next exponent can carry a finite value past the largest one of its type (65504 in float16: 64 2^10): it restores to that
+    // largest one, and so does what `E` has no room for.  (Up to the exponent looked at 127 2^e fits; the comparison is false for the NaN of a marked block.)
+    constexpr bool kHalf = std::is_same<E, f16_t>::value;
+    constexpr float kLargest = sizeof(E) == 4 ? 0x1.fffffep127f : kHalf ? 65504.0f : 0x1.fep127f;
+    auto saturate = [&](float (&v)[V]) {
+        if (e > (kHalf ? 136u : 248u)) {
+#pragma unroll
+            for (int i = 0; i < V; i++) v[i] = __builtin_fabsf(v[i]) > kLargest ? __builtin_copysignf(kLargest, v[i]) : v[i];
+        }
+    };
     const int8_t* p = q + row * K + d;
     float v[V];
     if (valid >= V) {
         const uint64_t bytes = *(const typename Bytes<V>::type*)p;
 #pragma unroll
         for (int i = 0; i < V; i++) v[i] = (float)(int8_t)(bytes >> (8 * i)) * factor;
+        saturate(v);
+        store<E, V, STREAM>(out + row * K + d, v);
     } else {
 #pragma unroll
         for (int i = 0; i < V; i++) v[i] = i < valid ? (float)p[i] * factor : 0.0f;
+        saturate(v);
+        store_some<E, V, STREAM>(out + row * K + d, valid, v);
     }
-    store_some<E, V, STREAM>(out + row * K + d, valid, v);
 }
 
 // ---- weight gradient ----------------------------------------------------------------------------------------------------------------
@@ -213,19 +228,34 @@ template <class E, int TO, int TI, int NT, int PART> __device__ __forceinline__ 
             }
         }
     };
-    auto write_b = [&](u32x4* sB, int chunk, int g, const uint32_t (&q)[8], const uint32_t (&e)[8]) {
+    // `edge`: some exponent is 249 or above, where 64 2^122, the largest finite activation rounded up, comes out as an infinity: written a second time, with
+    // bfloat16's largest number in its place
+    auto write_b = [&](u32x4* sB, int chunk, int g, const uint32_t (&q)[8], const uint32_t (&e)[8], bool edge) {
         float f[8];
 #pragma unroll
         for (int r = 0; r < 8; r++) f[r] = exponent_factor(e[r]);
-#pragma unroll
-        for (int v = 0; v < VI; v++) {
+        auto column = [&](int v) {
             u32x4 w;
 #pragma unroll
             for (int r = 0; r < 4; r++) w[r] = high_halves((float)(int8_t)(q[2 * r] >> (8 * v)) * f[2 * r], (float)(int8_t)(q[2 * r + 1] >> (8 * v)) * f[2 * r + 1]);
-            sB[chunk * TI + v * (TI / VI) + g] = w;
+            return w;
+        };
+#pragma unroll
+        for (int v = 0; v < VI; v++) {
+            sB[chunk * TI + v * (TI / VI) + g] = column(v);
             __builtin_amdgcn_sched_barrier(0);
         }
+        if (edge) {
+#pragma unroll 1
+            for (int v = 0; v < VI; v++) {
+                u32x4 w = column(v);
+#pragma unroll
+                for (int r = 0; r < 4; r++) w[r] -= ((w[r] & 0x7FFFu) == 0x7F80u ? 1u : 0u) + ((w[r] & 0x7FFF0000u) == 0x7F800000u ? 0x10000u : 0u);
+                sB[chunk * TI + v * (TI / VI) + g] = w;
+            }
+        }
     };
+    auto at_edge = [](uint32_t e) { return e - 249u < 6u; };
     auto stage = [&](u32x4* set, const Rows& from, bool count) {
 #pragma unroll
         for (int k = 0; k < T::kPerA; k++) {
@@ -255,7 +285,7 @@ template <class E, int TO, int TI, int NT, int PART> __device__ __forceinline__ 
                 e[5] = __builtin_amdgcn_ds_swizzle(from.e[k], 0x0018 | 5 << 5);
                 e[6] = __builtin_amdgcn_ds_swizzle(from.e[k], 0x0018 | 6 << 5);
                 e[7] = __builtin_amdgcn_ds_swizzle(from.e[k], 0x0018 | 7 << 5);
-                write_b(set + kP * kChunks * TO, item / (TI / VI), item % (TI / VI), from.b[k], e);
+                write_b(set + kP * kChunks * TO, item / (TI / VI), item % (TI / VI), from.b[k], e, __any(at_edge(from.e[k])));
             }
         }
     };
@@ -281,6 +311,7 @@ template <class E, int TO, int TI, int NT, int PART> __device__ __forceinline__ 
             const int item = tid + k * NT, chunk = item / (TI / VI), g = item % (TI / VI);
             if (item < T::kItemsB) {
                 uint32_t q[8], e[8];
+                bool edge = false;
 #pragma unroll
                 for (int r = 0; r < 8; r++) {
                     const int64_t m = m0 + chunk * 8 + r;
@@ -290,9 +321,10 @@ template <class E, int TO, int TI, int NT, int PART> __device__ __forceinline__ 
 #pragma unroll
                         for (int v = 0; v < VI; v++)
                             if (i0 + g * VI + v < p.I) q[r] |= (uint32_t)(uint8_t)p.q[m * p.I + i0 + g * VI + v] << (8 * v);
+                        edge |= at_edge(e[r]);
                     }
                 }
-                write_b(set + kP * kChunks * TO, chunk, g, q, e);
+                write_b(set + kP * kChunks * TO, chunk, g, q, e, __any(edge));
             }
         }
     };

@@ -393,7 +393,8 @@ int acx_block_step(const void *d_x, int64_t x_row, const void *d_projected, int6
 /* ---- activations kept in 8 bits (csrc/acx_act8.hip) -----------------------------------------------------------------------------
  * A checkpoint of M rows of K values: int8 q [M, K] and one exponent byte per 32 neighbouring values of a row [M, ceil(K / 32)]; the
  * value it stands for is q * 2^(exponent - 127).  The exponent is the smallest for which the block's largest magnitude rounds to at most
- * 127 (at least 1); 255 marks a block that held an infinity or a NaN, and stands for NaN.  x has a stride between rows in elements.
+ * 127 (at least 1); 255 marks a block that held an infinity or a NaN, and stands for NaN.  A value above the largest finite one of the type it is restored
+ * to (bfloat16 in the weight gradient) becomes that one: finite values stay finite.  x has a stride between rows in elements.
  * acx_act8_weight_grad: d_weight_grad [O, I] = d_out_grad^T (q 2^e) and d_bias_grad [O] (nullable) = column sums of d_out_grad, float32, for
  * d_out_grad [M, O] of type dtype; M, O, I >= 1, O and I <= 65536, O * I <= 2^29; d_work: acx_act8_workspace_bytes for the duration of the call's kernels. */
 int acx_act8_pack(const void *d_x, int64_t x_row, int dtype, int64_t M, int64_t K, int8_t *d_q, uint8_t *d_exponent, void *stream);

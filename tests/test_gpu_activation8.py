@@ -439,3 +439,55 @@ def test_checkpoint8_keeps_one_value_a_row():
         out = f()
     d = torch.randn_like(out)
     assert out.numel() == 8192 and torch.equal(torch.autograd.grad(out, a, d)[0], torch.autograd.grad(f(), a, d)[0])
+
+
+def test_finite_values_restore_to_finite_values():
+    """where rounding up to the next exponent carries a block's largest value past the type's largest finite one (float16 from 65280 on, float32 and bfloat16
+    from 1.9921875 * 2^127 on) it restores to that largest one: off by at most 2^-8 of it; the fifths of
+    it beside it lie a quarter of q's unit from a whole number, 2^-8 of the largest again (2^-7 leaves a factor of two); infinities and NaN still restore to NaN"""
+    import torch
+
+    from ac_solver.agents.activation8 import pack8, unpack8
+
+    border = {"float16": [65280.0, 65376.0, 65504.0, 65248.0], "bfloat16": [3.3895313892515355e38, 3.37e38], "float32": [3.3895313892515355e38, 3.4e38, 3.4028234663852886e38, 3.3895311e38]}
+    for name, tops in border.items():
+        dt = getattr(torch, name)
+        for width in (1, 3, 8, 32, 40):
+            rows = [[s * t] + [t / 5] * (width - 1) for t in tops for s in (1.0, -1.0)]
+            x = torch.tensor(rows, device="cuda", dtype=torch.float64).to(dt)
+            back = unpack8(*pack8(x), dt)
+            assert torch.isfinite(x).all() and torch.isfinite(back).all(), (name, width)
+            err, top = (back.double() - x.double()).abs(), x.double().abs()[:, :1]
+            assert bool((err[:, :32] <= 2.0 ** -7 * top).all()), (name, width)
+            for other in DTYPES:
+                assert torch.isfinite(unpack8(*pack8(x), getattr(torch, other))).all(), (name, other, width)
+    x = torch.full((4, 40), 1.0, device="cuda")
+    x[0, 3], x[1, 3], x[2, 35] = float("inf"), -float("inf"), float("nan")
+    for other in DTYPES:
+        bad = torch.isnan(unpack8(*pack8(x), getattr(torch, other)))
+        want = torch.zeros_like(bad)
+        want[0, :32], want[1, :32], want[2, 32:] = True, True, True
+        assert torch.equal(bad, want)
+
+
+@pytest.mark.parametrize("M", [3, 200])
+def test_weight_grad_of_the_largest_finite_values(M):
+    """the largest finite activations count as what they restore to in bfloat16, 1.9921875 * 2^127 (M 3: the rows that are read one by one; 200: whole
+    vectors, too).  Only these rows are not zero, so a product is one term of float32: the two roundings of a term and of its sum."""
+    import torch
+
+    from ac_solver.agents.activation8 import pack8, unpack8, weight_grad8
+
+    for dtype in DTYPES:
+        for O, I in ((3, 5), (70, 40), (65, 129), (300, 260)):
+            x = torch.zeros(M, I, device="cuda")
+            dy = torch.zeros(M, O, device="cuda", dtype=getattr(torch, dtype))
+            for row, sign in ((0, 1.0), (M - 1, -1.0)):
+                x[row, row % I] = sign * 3.4028234663852886e38
+            dy[0], dy[M - 1, :2] = 2.0 ** -9, 2.0 ** -10
+            q, e = pack8(x)
+            dw, db = weight_grad8(dy, q, e)
+            kept = unpack8(q, e, torch.bfloat16).double()
+            want = dy.double().t() @ kept
+            assert torch.isfinite(dw).all() and float(want.abs().max()) > 1e35
+            assert bool(((dw.double() - want).abs() <= 2.0 ** -23 * want.abs()).all()), (dtype, O, I)
