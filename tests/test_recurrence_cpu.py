@@ -251,3 +251,38 @@ def test_forward_mode_tangents_are_refused_not_dropped():
         d = forward_ad.make_dual(c, torch.ones_like(c))
         with forward_ad._set_fwd_grad_enabled(False), pytest.raises(ValueError, match="GPU"):
             R.gated_scan(d, z)
+
+
+def _make(*args):
+    """make in csrc/, the libraries of HIP and plain C++ code taken as up to date"""
+    import os
+    import subprocess
+
+    csrc = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "ac-solver_amd", "csrc")
+    return subprocess.run(["make", "-C", csrc, "-o", "../lib/libacx.so", "-o", "../lib/libacx_trainer.so", *args], capture_output=True, text=True)
+
+
+@pytest.mark.parametrize("where", ["", "nowhere"])
+def test_the_library_builds_without_torch(tmp_path, where):
+    """no torch, or one without its headers: everything but the binding is built, and make says so"""
+    out = _make(f"BINDING={tmp_path}/acx_torch.so", f"BUILD={tmp_path}", f"TORCH_DIR={tmp_path / where if where else ''}")
+    assert out.returncode == 0 and "not built" in out.stderr and not (tmp_path / "acx_torch.so").exists(), out.stderr
+
+
+def test_the_binding_is_built_again_for_another_torch(tmp_path):
+    """(the compiler is replaced by one that only makes the file)"""
+    import os
+
+    (tmp_path / "bin").mkdir()
+    fake = tmp_path / "bin" / "g++"
+    fake.write_text("#!/bin/sh\nwhile [ \"$1\" != -o ]; do shift; done\necho built > \"$2\"\n")
+    fake.chmod(0o755)
+    path = os.environ["PATH"]
+    os.environ["PATH"] = f"{tmp_path / 'bin'}:{path}"
+    try:
+        args = (f"BINDING={tmp_path}/acx_torch.so", f"BUILD={tmp_path}/build")
+        said = [_make(*args, f"TORCH_VERSION={v}") for v in ("1", "1", "2", "2", "1", "1")]
+    finally:
+        os.environ["PATH"] = path
+    assert all(s.returncode == 0 for s in said), [s.stderr for s in said]
+    assert ["acx_torch.cpp" in s.stdout for s in said] == [True, False, True, False, True, False]
