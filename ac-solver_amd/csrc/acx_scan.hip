@@ -497,6 +497,9 @@ static bool strides_ok(int64_t D, int dtype, std::initializer_list<int64_t> rows
         if (r < 0 || r > (((int64_t)1 << 32) / element_bytes(dtype) - D) / apart) return false;
     return true;
 }
+// Whether two states [N, D] have memory in common: one workgroup reads the first where another one, of a later chunk or of the same channels (see Lane), may have
+// written the second already.
+static bool meet_in_memory(const float* a, const float* b, int64_t n) { return a && b && (a < b ? b - a : a - b) < n; }
 static int check_sizes(int64_t T, int64_t N, int64_t D, int dtype, const char* who) {
     if (dtype != ACX_F32 && dtype != ACX_BF16 && dtype != ACX_F16) return fail(ACX_E_INVAL, "%s: activations are ACX_F32, ACX_BF16 or ACX_F16", who);
     if (T < 0 || N < 0 || D < 0 || D > (1 << 20) || T > ((int64_t)1 << 40) || N > ((int64_t)1 << 31)) return fail(ACX_E_INVAL, "%s: bad sizes", who);
@@ -527,7 +530,7 @@ extern "C" int acx_scan_forward(const void* d_candidate, int64_t c_step, int64_t
     if (N == 0 || D == 0) return ACX_OK;
     if (T == 0) return fail(ACX_E_INVAL, "acx_scan_forward: no steps");
     if (!d_candidate || !d_gate || !d_hidden || !d_last) return fail(ACX_E_INVAL, "acx_scan_forward: null pointer");
-    if (d_last == d_state) return fail(ACX_E_INVAL, "acx_scan_forward: the last state does not replace the first in place");
+    if (scan::meet_in_memory(d_last, d_state, N * D)) return fail(ACX_E_INVAL, "acx_scan_forward: the last state does not replace the first in place");
     if (!scan::strides_ok(D, dtype, {c_row, z_row})) return fail(ACX_E_INVAL, "acx_scan_forward: rows too far apart (4 GiB among the rows of 64 lanes)");
     scan::Args a = {};
     a.c = d_candidate, a.c_st = c_step, a.c_sn = c_row;
@@ -546,6 +549,8 @@ extern "C" int acx_scan_backward(const void* d_candidate, int64_t c_step, int64_
     if (N == 0 || D == 0) return ACX_OK;
     if (T == 0) return fail(ACX_E_INVAL, "acx_scan_backward: no steps");
     if (!d_candidate || !d_gate || !d_hidden_grad || !d_bounds || !d_candidate_grad || !d_gate_grad) return fail(ACX_E_INVAL, "acx_scan_backward: null pointer");
+    if (scan::meet_in_memory(d_state_grad, d_last_grad, N * D))
+        return fail(ACX_E_INVAL, "acx_scan_backward: the gradient of the first state does not replace that of the last in place");
     if (!scan::strides_ok(D, dtype, {c_row, z_row, g_row, dc_row, dz_row}))
         return fail(ACX_E_INVAL, "acx_scan_backward: rows too far apart (4 GiB among the rows of 64 lanes)");
     scan::Args a = {};

@@ -355,7 +355,8 @@ int64_t acx_policy_packed_bytes(int in_dim);
  * d_hidden is contiguous [T, N, D], d_reset [T, N] bytes (nullable), d_state and d_last [N, D] (different buffers).
  * d_bounds (nullable: no gradient wanted; acx_scan_bounds_bytes) takes what acx_scan_backward needs besides the operands.
  * d_work: acx_scan_workspace_bytes of scratch for the duration of the call's kernels, not shared with another call in flight.
- * acx_scan_backward: gradients of candidate, gate and state (nullable) from those of hidden and last (nullable). */
+ * acx_scan_backward: gradients of candidate, gate and state (nullable) from those of hidden and last (nullable).  Results lie
+ * apart from operands, here and in the functions of the recurrent agent below (but for acx_block_step's state). */
 int64_t acx_scan_bounds_bytes(int64_t T, int64_t N, int64_t D);
 int64_t acx_scan_workspace_bytes(int64_t T, int64_t N, int64_t D, int dtype);
 int acx_scan_forward(const void *d_candidate, int64_t c_step, int64_t c_row, const void *d_gate, int64_t z_step, int64_t z_row, int dtype,

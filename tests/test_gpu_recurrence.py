@@ -482,3 +482,39 @@ def test_forward_mode_is_refused():
         for k in places:
             with forward_ad.dual_level(), pytest.raises(NotImplementedError, match="forward mode"):
                 f(*args[:k], forward_ad.make_dual(args[k], torch.ones_like(args[k])), *args[k + 1:])
+
+
+def test_the_states_of_a_scan_do_not_replace_each_other_in_place():
+    """of the C functions (from Python the results are new tensors): the last state over the first, the first state's gradient over the last one's, whole or in part,
+    where other workgroups may still have to read; buffers side by side are taken"""
+    import torch
+
+    from ac_solver import _acx
+    from ac_solver.agents.recurrence import gated_scan_backward, gated_scan_forward
+
+    T, N, D = 4100, 2, 66
+    c, z, r, s, dh, dl = inputs(T, N, D, "float32", 8)
+    hidden, last, bounds = gated_scan_forward(c, z, r, s)
+    dc, dz, ds = gated_scan_backward(dh, dl, c, z, r, bounds)
+    work = torch.empty(_acx.lib.acx_scan_workspace_bytes(T, N, D, _acx.F32), dtype=torch.uint8, device="cuda")
+    assert work.numel()
+    both = torch.zeros(2 * N * D, device="cuda")
+    st = N * D, D
+    stream = torch.cuda.current_stream().cuda_stream
+
+    def forward(place):
+        both[:N * D] = s.view(-1)
+        return _acx.lib.acx_scan_forward(c.data_ptr(), *st, z.data_ptr(), *st, _acx.F32, r.data_ptr(), both.data_ptr(), T, N, D, torch.empty_like(hidden).data_ptr(),
+                                         both.data_ptr() + 4 * place, None, work.data_ptr(), work.numel(), stream)
+
+    def backward(place):
+        both[:N * D] = dl.view(-1)
+        return _acx.lib.acx_scan_backward(c.data_ptr(), *st, z.data_ptr(), *st, dh.data_ptr(), *st, _acx.F32, r.data_ptr(), bounds.data_ptr(), both.data_ptr(), T, N, D,
+                                          torch.empty_like(dc).data_ptr(), *st, torch.empty_like(dz).data_ptr(), *st, both.data_ptr() + 4 * place, work.data_ptr(), work.numel(), stream)
+
+    for call, want in ((forward, last), (backward, ds)):
+        for place in (0, 1, N * D - 1):
+            assert call(place) == _acx.E_INVAL and b"in place" in _acx.lib.acx_last_error()
+        assert call(N * D) == _acx.OK
+        torch.cuda.synchronize()
+        assert torch.equal(both[N * D:].view(N, D), want)
