@@ -158,6 +158,11 @@ void require_target(const Tensor& t, const char* name, const Tensor& like, std::
     require_apart(t, name, others);
 }
 
+// a caller's tensor has been written into: what autograd kept of it elsewhere is not what it was
+void count_change(const Tensor& t) {
+    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 void* ptr(const Tensor& t) { return t.data_ptr(); }
 void* ptr(const Maybe& t) { return t ? t->data_ptr() : nullptr; }
 template <class T> T* ptr_as(const Tensor& t) { return static_cast<T*>(t.data_ptr()); }
@@ -246,6 +251,7 @@ std::tuple<Tensor, Tensor, Maybe> scan_backward(const Tensor& d_hidden, const Ma
                                 ptr_as<float>(b), ptr_as<float>(dl), o.steps, o.rows, o.width, ptr(*dc), dc->stride(0), dc->stride(1), ptr(*dz), dz->stride(0), dz->stride(1),
                                 ptr_as<float>(ds), ptr(work), bytes_of(work), stream_of(o.c)),
           "acx_scan_backward");
+    count_change(*dc), count_change(*dz);
     return {*dc, *dz, ds};
 }
 
@@ -360,6 +366,7 @@ std::tuple<Tensor, Maybe, Maybe, Maybe, Maybe, Maybe> block_backward(const Maybe
         check(api.acx_block_backward(rx.p, rx.stride, ry.p, ry.stride, rg.p, rg.stride, rn.p, rn.stride, ru.p, ru.stride, code, ptr_as<float>(o.w), ptr_as<float>(o.s), ptr_as<float>(o.n),
                                      ptr_as<float>(st), o.rows, o.width, ptr(dx), ptr(dy), rdg.p, rdg.stride, ptr_as<float>(weights), ptr(work), bytes_of(work), stream_of(o.x)),
               "acx_block_backward");
+        if (dg) count_change(*dg);
     }
     Maybe dw, ds, dn;
     if (o.y) dw = weights.select(0, 0);
@@ -524,6 +531,7 @@ std::tuple<Tensor, Maybe, Tensor> recurrent_step(const Tensor& x_, const Tensor&
         check(api.acx_block_step(ptr(x), x.stride(0), ptr(projected), projected.stride(0), code_of(x.scalar_type()), ptr_as<uint8_t>(reset), ptr_as<float>(state), ptr_as<float>(w), ptr_as<float>(s),
                                  ptr_as<float>(n), (float)eps, rows, width, ptr_as<float>(next), ptr(out), ptr(u), stream_of(x)),
               "acx_block_step");
+    if (next_state) count_change(next);
     return {out, u, next};
 }
 

@@ -518,3 +518,27 @@ def test_the_states_of_a_scan_do_not_replace_each_other_in_place():
         assert call(N * D) == _acx.OK
         torch.cuda.synchronize()
         assert torch.equal(both[N * D:].view(N, D), want)
+
+
+def test_writing_into_a_callers_tensor_is_noticed_by_autograd():
+    """what another function kept of a tensor that a result is then written into is not what it was: its gradient is refused, as after torch's own in-place functions"""
+    import torch
+
+    from ac_solver.agents.block_norm import block_output_backward, block_output_forward
+    from ac_solver.agents.recurrence import gated_scan_backward, gated_scan_forward, recurrent_step
+
+    c, z, r, s, dh, dl = inputs(6, 3, 8, "float32", 2)
+    w, k = torch.ones(8, device="cuda"), torch.ones(8, device="cuda", requires_grad=True)
+    _, _, bounds = gated_scan_forward(c, z, r, s)
+    _, _, stats = block_output_forward(c, z, dh, w, w, w)
+    p = torch.cat((c, z, dh), dim=-1)[0]
+    memory, a, b, g = s.clone(), torch.zeros_like(c), torch.zeros_like(c), torch.zeros_like(c)
+    for target, write in ((memory, lambda: recurrent_step(c[0], p, memory, w, next_state=memory)), (a, lambda: gated_scan_backward(dh, dl, c, z, r, bounds, out=(a, b))),
+                          (b, lambda: gated_scan_backward(dh, dl, c, z, r, bounds, out=(a, b))), (g, lambda: block_output_backward(c, c, c, z, dh, w, w, w, stats, d_gate_out=g))):
+        out = (target * k).sum()
+        write()
+        with pytest.raises(RuntimeError, match="inplace"):
+            out.backward()
+    with torch.inference_mode():  # (tensors that count no changes)
+        state = s.clone()
+        recurrent_step(c[0], p, state, w, next_state=state)
