@@ -32,6 +32,9 @@ def weight_grad8(d_out, q, exponent):
     return ops.weight_grad8(d_out, q, exponent)
 
 
+MAX_SIDE, MAX_WEIGHTS = 1 << 16, 1 << 29  # of weight_grad8
+
+
 class _Linear8(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias):
@@ -52,8 +55,8 @@ class _Linear8(torch.autograd.Function):
 
 def linear8(x, weight, bias=None):
     """torch.nn.functional.linear with float32 parameters [outputs, inputs], [outputs], computed in the type of x; what it keeps for the
-    backward pass is x in 8 bits (pack8), and the gradient of the weight is taken from that (weight_grad8).  The gradient of x is the
-    library's and knows nothing of the 8 bits."""
+    backward pass is x in 8 bits (pack8), and the gradient of the weight is taken from that (weight_grad8, whose sizes are the limit of a
+    layer that wants one).  The gradient of x is the library's and knows nothing of the 8 bits."""
     if not isinstance(weight, torch.Tensor) or weight.dtype != torch.float32 or weight.dim() != 2:
         raise TypeError("weight has to be a float32 matrix")
     if bias is not None and (not isinstance(bias, torch.Tensor) or bias.dtype != torch.float32 or bias.shape != weight.shape[:1]):
@@ -62,6 +65,9 @@ def linear8(x, weight, bias=None):
         raise TypeError("x has to be a float32, bfloat16 or float16 tensor")
     if x.shape[-1:] != weight.shape[1:]:
         raise ValueError(f"x has the shape {tuple(x.shape)}, the weight {tuple(weight.shape)}")
+    outputs, inputs = weight.shape
+    if torch.is_grad_enabled() and (weight.requires_grad or (bias is not None and bias.requires_grad)) and (outputs > MAX_SIDE or inputs > MAX_SIDE or outputs * inputs > MAX_WEIGHTS):
+        raise ValueError(f"the gradient of a layer of up to {MAX_SIDE} outputs and inputs and {MAX_WEIGHTS} weights is handled, not of {outputs} x {inputs}")
     if not x.is_cuda:
         raise ValueError(f"the activations have to live on a GPU, not on {x.device}: there is no CPU path")
     return _Linear8.apply(x, weight, bias)

@@ -286,3 +286,17 @@ def test_the_binding_is_built_again_for_another_torch(tmp_path):
         os.environ["PATH"] = path
     assert all(s.returncode == 0 for s in said), [s.stderr for s in said]
     assert ["acx_torch.cpp" in s.stdout for s in said] == [True, False, True, False, True, False]
+
+
+def test_a_layer_whose_gradient_is_out_of_reach_is_refused_before_it_is_used():
+    from ac_solver.agents.activation8 import linear8
+
+    for outputs, inputs in (((1 << 16) + 1, 1), (1, (1 << 16) + 1)):
+        w, x, b = torch.zeros(outputs, inputs), torch.zeros(2, inputs), torch.zeros(outputs)
+        for weight, bias in ((w.clone().requires_grad_(), None), (w, b.clone().requires_grad_())):
+            with pytest.raises(ValueError, match="65536 outputs and inputs"):
+                linear8(x, weight, bias)
+            with torch.no_grad(), pytest.raises(ValueError, match="GPU"):  # no gradient is wanted: only the place is wrong
+                linear8(x, weight, bias)
+        with pytest.raises(ValueError, match="GPU"):
+            linear8(x.requires_grad_(), w, b)
