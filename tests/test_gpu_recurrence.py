@@ -542,3 +542,24 @@ def test_writing_into_a_callers_tensor_is_noticed_by_autograd():
     with torch.inference_mode():  # (tensors that count no changes)
         state = s.clone()
         recurrent_step(c[0], p, state, w, next_state=state)
+
+
+VARIANTS = {  # (steps, rows, features): how plan_of cuts them
+    "16 waves, 5 tiles, the last one ragged": (1046, 19, 846),
+    "16 waves, 3 tiles": (523, 19, 846),
+    "two channels a lane, 4 waves, 4 tiles, an odd width": (201, 399, 151),
+    "two channels a lane, 4 waves, 2 tiles, an even width": (128, 399, 150),
+    "two channels a lane, 4 waves, rows of three lanes": (90, 9000, 5),
+    "two channels a lane, one wave, an odd width": (37, 1030, 257),
+    "two channels a lane, one wave, rows of two lanes": (20, 66000, 3),
+    "one channel a lane, one wave, rows of one lane": (10, 9000, 1),
+    "one channel a lane, chunks, rows of 7 lanes": (5003, 9, 7),
+    "one channel a lane, 8 waves, 3 tiles, no chunks": (300, 40000, 1),
+}
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("variant", list(VARIANTS))
+def test_every_way_of_cutting_the_work(variant, dtype):
+    check(*VARIANTS[variant], dtype, seed=3)
+    check(*VARIANTS[variant], dtype, seed=4, layout="slices", state=False)
