@@ -144,8 +144,8 @@ class checkpoint8(torch.autograd.graph.saved_tensors_hooks):
         super().__init__(self._keep, self._restore)
 
     def __enter__(self):
+        super().__enter__()
         _inside.depth = getattr(_inside, "depth", 0) + 1
-        return super().__enter__()
 
     def __exit__(self, *exc):
         _inside.depth -= 1

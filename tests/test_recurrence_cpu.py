@@ -300,3 +300,18 @@ def test_a_layer_whose_gradient_is_out_of_reach_is_refused_before_it_is_used():
                 linear8(x, weight, bias)
         with pytest.raises(ValueError, match="GPU"):
             linear8(x.requires_grad_(), w, b)
+
+
+def test_a_checkpoint8_block_that_could_not_be_entered_leaves_nothing_behind():
+    """where saved-tensor hooks are forbidden: outside the block nothing is packed (recurrent_block asks `packing`)"""
+    from ac_solver.agents import activation8 as A
+
+    with torch.autograd.graph.disable_saved_tensors_hooks("not here"), pytest.raises(RuntimeError, match="not here"):
+        with A.checkpoint8():
+            pass
+    assert not A.packing()
+    with A.checkpoint8():
+        with A.checkpoint8():
+            assert A.packing()
+        assert A.packing()
+    assert not A.packing()
