@@ -44,19 +44,20 @@ class _Linear8(torch.autograd.Function):
         return out
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, d_out):
         q, exponent, weight = ctx.saved_tensors
         need_x, need_w, need_b = ctx.needs_input_grad
-        dx = d_out @ weight.to(d_out.dtype) if need_x else None
-        dw, db = weight_grad8(d_out, q, exponent) if need_w or need_b else (None, None)
-        return dx, dw if need_w else None, db if need_b else None
+        with torch.no_grad():
+            dx = d_out @ weight.to(d_out.dtype) if need_x else None
+            dw, db = weight_grad8(d_out, q, exponent) if need_w or need_b else (None, None)
+        grads = dx, dw if need_w else None, db if need_b else None
+        return ops.once(grads, d_out) if torch.is_grad_enabled() else grads
 
 
 def linear8(x, weight, bias=None):
     """torch.nn.functional.linear with float32 parameters [outputs, inputs], [outputs], computed in the type of x; what it keeps for the
     backward pass is x in 8 bits (pack8), and the gradient of the weight is taken from that (weight_grad8, whose sizes are the limit of a
-    layer that wants one).  The gradient of x is the library's and knows nothing of the 8 bits."""
+    layer that wants one).  The gradient of x is the library's and knows nothing of the 8 bits.  Differentiable once."""
     if not isinstance(weight, torch.Tensor) or weight.dtype != torch.float32 or weight.dim() != 2:
         raise TypeError("weight has to be a float32 matrix")
     if bias is not None and (not isinstance(bias, torch.Tensor) or bias.dtype != torch.float32 or bias.shape != weight.shape[:1]):

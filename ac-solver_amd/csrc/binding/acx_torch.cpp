@@ -183,17 +183,23 @@ bool wants_grad(std::initializer_list<const Maybe*> ts) {
         if (*t && (*t)->requires_grad()) return true;
     return false;
 }
-// the gradients of a backward pass that is itself recorded (create_graph): differentiating them again raises
-variable_list once(variable_list grads) {
+// The gradients of a backward pass that is itself recorded (create_graph), from those of the outputs: differentiating them again raises.  They hang on every operand
+// of the forward pass (the edges of the node that runs), whether it was kept or not, so that no way from them to an operand leaves a term out.
+variable_list once(variable_list grads, const variable_list& from) {
     if (!at::GradMode::is_enabled()) return grads;
-    variable_list defined, out = grads;
+    torch::autograd::edge_list edges;
+    if (const auto node = torch::autograd::get_current_node())
+        for (const auto& e : node->next_edges())
+            if (e.is_valid()) edges.push_back(e);
+    for (const auto& t : from)
+        if (t.defined() && t.requires_grad()) edges.push_back(torch::autograd::impl::gradient_edge(t));
+    const auto error = std::make_shared<torch::autograd::Error>("the gradients of this operator cannot be differentiated again", std::move(edges));
     for (auto& g : grads)
-        if (g.defined()) defined.push_back(g.detach().requires_grad_(true));
-    auto wrapped = (*std::make_shared<torch::autograd::DelayedError>("the gradients of this operator cannot be differentiated again", defined.size()))(std::move(defined));
-    size_t k = 0;
-    for (auto& g : out)
-        if (g.defined()) g = wrapped[k++];
-    return out;
+        if (g.defined()) {
+            g = g.detach();
+            torch::autograd::create_gradient_edge(g, error);
+        }
+    return grads;
 }
 Maybe opt(const Tensor& t) { return t.defined() ? Maybe(t) : std::nullopt; }
 Tensor orundef(const Maybe& t) { return t ? *t : Tensor(); }
@@ -273,7 +279,7 @@ struct GatedScan : torch::autograd::Function<GatedScan> {
             auto [dc, dz, ds] = scan_backward(d_hidden, opt(g[1]), saved[0], saved[1], opt(saved[2]), saved[3], ctx->saved_data["state"].toBool());
             out = {dc, dz, Tensor(), orundef(ds)};
         }
-        return once(std::move(out));
+        return once(std::move(out), g);
     }
 };
 
@@ -401,7 +407,7 @@ struct BlockOutput : torch::autograd::Function<BlockOutput> {
             for (int i = 3; i < 6; i++)
                 if (s[i].defined() && !out[i].defined()) out[i] = at::zeros(s[i].sizes(), s[i].options());
         }
-        return once(std::move(out));
+        return once(std::move(out), g);
     }
 };
 
@@ -496,7 +502,7 @@ struct RecurrentBlock : torch::autograd::Function<RecurrentBlock> {
                                                    third(d_projected, 1));
             out = {dx, d_projected, Tensor(), orundef(d_state), orundef(dw), orundef(ds), orundef(dn), Tensor(), Tensor()};
         }
-        return once(std::move(out));
+        return once(std::move(out), g);
     }
 };
 
@@ -641,6 +647,14 @@ PYBIND11_MODULE(acx_torch, m) {
         const at::NoGradGuard no_grad;
         auto [a, b, c] = recurrent_step(xt, pt, stt, wt, sct, nt, rt, nst, eps);
         return py::make_tuple(wrap(a), wrap(b), ns.is_none() ? wrap(c) : py::reinterpret_borrow<py::object>(ns));
+    });
+    m.def("once", [](const py::sequence& grads, H from) {  // (of a backward pass in Python: a tuple of tensors and None)
+        variable_list g;
+        for (H t : grads) g.push_back(orundef(maybe(t, "a gradient")));
+        g = once(std::move(g), {tensor(from, "d_out")});
+        py::tuple out(g.size());
+        for (size_t k = 0; k < g.size(); k++) out[k] = wrap(opt(g[k]));
+        return out;
     });
     m.def("pack8", [](H x) {
         const Tensor xt = tensor(x, "x");

@@ -563,3 +563,38 @@ VARIANTS = {  # (steps, rows, features): how plan_of cuts them
 def test_every_way_of_cutting_the_work(variant, dtype):
     check(*VARIANTS[variant], dtype, seed=3)
     check(*VARIANTS[variant], dtype, seed=4, layout="slices", state=False)
+
+
+def test_second_derivatives_are_refused_wherever_they_are_asked_for():
+    """gradients that were taken with create_graph hang on all operands, also on those that the gradient itself was not kept for: a sum of a loss and a penalty on its
+    gradient, a Hessian, or a penalty alone with operands that may be unused all raise, none leaves its second-order term out; what does not depend on
+    the gradient is not in the way"""
+    import torch
+
+    from ac_solver.agents.activation8 import linear8
+    from ac_solver.agents.block_norm import block_input, block_output
+    from ac_solver.agents.recurrence import gated_scan, recurrent_block
+
+    c, z, r, s, dh, dl = inputs(6, 2, 8, "float32", 2)
+    w, p, m = torch.rand(8, device="cuda"), torch.cat((c, z, dh), dim=-1), torch.randn(3, 8, device="cuda")
+    calls = ((lambda c, z, s: gated_scan(c, z, r, s), (c, z, s)), (lambda x, y, g, w, s, v: block_output(x, y, g, w, s, v), (c, z, dh, w, w + 1, w + 2)), (lambda x, w: (block_input(x, w),), (c, w)),
+             (lambda x, p, s, w, a, v: recurrent_block(x, p, s, w, a, v), (c, p, s, w, w + 1, w + 2)), (lambda x, m, b: (linear8(x, m, b),), (c, m, torch.ones(3, device="cuda"))))
+    for f, operands in calls:
+        for k in range(len(operands)):
+            leaves = [t.clone().requires_grad_() for t in operands]
+            other = torch.ones((), device="cuda", requires_grad=True)
+            outs = f(*leaves)
+            loss = sum(o.square().sum() for o in outs) * other
+            first = torch.autograd.grad(loss, leaves, create_graph=True)
+            penalty = first[k].square().sum()
+            assert all(g.requires_grad for g in first)
+            for total, unused in ((penalty, True), (penalty + sum(t.square().sum() for t in leaves), False)):
+                for leaf in leaves:
+                    with pytest.raises(RuntimeError, match="again"):
+                        torch.autograd.grad(total, [leaf], retain_graph=True, allow_unused=unused)
+            with pytest.raises(RuntimeError, match="again"):
+                (penalty + sum(t.square().sum() for t in leaves)).backward(retain_graph=True)
+            apart = torch.ones((), device="cuda", requires_grad=True)
+            assert float(torch.autograd.grad(penalty.detach() + 2 * apart, apart)[0]) == 2
+    with pytest.raises(RuntimeError, match="again"):
+        torch.autograd.functional.hessian(lambda t: gated_scan(t, z)[0].square().sum(), c)
