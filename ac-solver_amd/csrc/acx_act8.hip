@@ -321,9 +321,10 @@ template <class E, int TO, int TI, int NT, int PART> __device__ __forceinline__ 
 #pragma unroll
                         for (int v = 0; v < VI; v++)
                             if (i0 + g * VI + v < p.I) q[r] |= (uint32_t)(uint8_t)p.q[m * p.I + i0 + g * VI + v] << (8 * v);
-                        edge |= at_edge(e[r]);
                     }
                 }
+#pragma unroll
+                for (int r = 0; r < 8; r++) edge |= at_edge(e[r]);  // (behind all the loads, which wait for each other otherwise)
                 write_b(set + kP * kChunks * TO, chunk, g, q, e, __any(edge));
             }
         }
