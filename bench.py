@@ -764,6 +764,19 @@ def launch_ranks(n, argv, child=None, env=None, grace_s=20.0):
     return 0
 
 
+def result_line(out):
+    """The one line that a run prints.  The headline's own numbers as they are; the secondary measurements to six digits, and no blanks: with all of them in full the
+    line had 20 250 characters, and whoever keeps the last 20 000 of a run's output has no line that parses."""
+    def short(v):
+        if isinstance(v, float):
+            return float(f"{v:.6g}")
+        if isinstance(v, dict):
+            return {k: short(x) for k, x in v.items()}
+        return [short(x) for x in v] if isinstance(v, (list, tuple)) else v
+
+    return json.dumps({k: short(v) if isinstance(v, (dict, list, tuple)) else v for k, v in out.items()}, separators=(",", ":"))
+
+
 def main():
     ap = argparse.ArgumentParser()
     ap.add_argument("--gpus", type=int, default=None, help="ranks (one process per GPU).  Under a launcher (WORLD_SIZE set) it must agree with it; "
@@ -1031,7 +1044,7 @@ def main():
             if rank == 0:
                 got = dict(partial)
                 got["error"] = f"secondary measurements did not finish within {SEARCH_TIMEOUT_S} s (finished stages: {sorted(partial)})"
-                print(json.dumps(headline(extras_box[0], got)), flush=True)
+                print(result_line(headline(extras_box[0], got)), flush=True)
             # exit code: 0 when the sharded search itself was measured (the line is usable and says what is missing), else failure
             os._exit(0 if "nodes_per_s" in partial.get("bfs_sharded", {}) else 3)
 
@@ -1067,7 +1080,7 @@ def main():
             if not args.no_search:
                 out["cpu_baseline"].update(cpu_search_baseline(10**6 if CPU_SCALE == 1.0 else 10**4))
             out["cpu_baseline"]["python_numpy"] = cpu_python_baseline(states, budget_s=4.0 * CPU_SCALE)
-        print(json.dumps(out), flush=True)
+        print(result_line(out), flush=True)
 
 
 if __name__ == "__main__":

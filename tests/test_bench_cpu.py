@@ -141,3 +141,30 @@ def test_bench_refuses_a_gpus_flag_that_contradicts_the_launcher():
     env = dict(os.environ, WORLD_SIZE="2", RANK="0", LOCAL_RANK="0")
     r = subprocess.run([sys.executable, bench.__file__, "--gpus", "4"], env=env, capture_output=True, text=True, timeout=120)
     assert r.returncode != 0 and "WORLD_SIZE=2" in r.stderr and r.stdout.strip() == ""
+
+
+def test_the_result_line_is_short_and_keeps_the_headline():
+    """a full run's line (the one in profiles/, 20 251 characters as it was printed) in the form it is printed in: one line, the headline's numbers exact, the secondary
+    ones to six digits, well below 20 000 characters"""
+    import json
+    import os
+
+    import bench
+
+    with open(os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "profiles", "r6_bench_line.json")) as f:
+        full = json.load(f)
+    assert len(json.dumps(full)) > 20000
+    line = bench.result_line(full)
+    got = json.loads(line)
+    assert "\n" not in line and len(line) < 18500 and list(got) == list(full)
+    for k, v in full.items():
+        assert isinstance(v, (dict, list)) or got[k] == v
+
+    def close(a, b):
+        if isinstance(a, dict):
+            return a.keys() == b.keys() and all(close(a[k], b[k]) for k in a)
+        if isinstance(a, list):
+            return len(a) == len(b) and all(close(x, y) for x, y in zip(a, b))
+        return abs(a - b) <= 5e-6 * abs(a) if isinstance(a, float) else a == b
+
+    assert close(full, got)
