@@ -10,9 +10,10 @@
 // the accuracy of a float32 product, at one to three times the matrix work of a bf16 one and 1 byte instead of 4 read per x.
 // A block with an infinity or a NaN is marked with the exponent byte 255 and restores to NaN: it is not hidden.  Finite values restore to finite ones: where rounding up left
 // the type, to its largest.
-// Measured: 1 Mi x 256 f32 packed in 0.273 ms and restored in 0.273 ms (4.95 TB/s).  Weight gradient of 1 Mi rows, 768 x 256: dy bf16 0.53 ms (4.5 TB/s,
-// memory), dy f32 1.19 ms: 1.24 PFLOP of bf16 products at 1.04 PFLOP/s, where the chip's clock drops to 1.5 GHz under the matrix units' load
-// (a library's bf16 product of 8192^3: 1.16 PFLOP/s).  65537 x 256 x 72 bf16 20 + 5 us: five steps a workgroup, their latency and the join.
+// Measured: 1 Mi x 256 f32 packed in 0.275 ms and restored in 0.275 ms (4.9 TB/s).  Weight gradient of 1 Mi rows, 768 x 256: dy bf16 0.52 to 0.54 ms (4.6 TB/s of
+// what it moves: three tiles of outputs read q), f16 0.83 to 0.86, f32 1.19 to 1.27 by the card: 1.24 TFLOP of bf16 products at 1.04 to 0.98 PFLOP/s, where the chip's clock drops to
+// 1.5 GHz under the matrix units' load (a library's bf16 product of 8192^3: 1.16 PFLOP/s).  65537 x 256 x 72 bf16 20 + 5 us: five steps a workgroup,
+// their latency and the join.  Between the tiles the padding is staged and multiplied, too: 65 x 129 f32 0.36 ms, 0.09 by its bytes.
 #include <type_traits>
 
 #include "acx_elem.h"
@@ -114,7 +115,8 @@ template <class E, int V, bool STREAM> __global__ void __launch_bounds__(256) k_
 // bring them (column c of a vector of V stands at (c % V) TO / V + c / V): a wave's stores and its operand loads are both contiguous, and
 // the order is undone when dW is written (a lane's products then are neighbours in a row of dW: whole vectors are stored).
 // LDS holds two sets of rows and registers a third that is on its way from memory: a step multiplies one set and writes the next.  The two
-// waves of a SIMD take these halves in opposite order, so one's conversions (vector pipe) run under the other's products (matrix pipe).
+// waves of a SIMD take these halves in opposite order, so one's conversions (vector pipe) run under the other's products (matrix pipe).  (Workgroups of
+// 8 waves; the tile of 64 outputs has 4, one a SIMD, and does the halves one after the other.)
 typedef __bf16 frag __attribute__((ext_vector_type(8)));
 typedef float acc16 __attribute__((ext_vector_type(16)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));

@@ -310,9 +310,10 @@ template <class E, class F> static void with_shape(int64_t D, F&& fn) {
         else fn(integral_constant<int, 4>{}, integral_constant<int, 1024>{}, (int)(D + 255) / 256 * 64);
     }
 }
-// About as many workgroups as stay resident (what is gained by more is less than their partial sums cost), the same number for each of the 256
-// compute units: 819 of 320 lanes on 49016 x 1104 f32, the backward pass takes 592 us and 484 with 768, because 51 of them start
-// when the others end.
+// Workgroups of 1024 lanes a compute unit: as many as stay resident where the backward pass has up to 128 registers (float32 rows, but for those of a whole
+// wave), two rounds of them for 16-bit rows, whose backward pass has 168 to 206; what is gained by more is less than their partial sums cost.
+// The same number for each of the 256 compute units: 819 of 320 lanes on 49016 x 1104 f32, the backward pass takes 592 us and 484 with 768,
+// because 51 of them start when the others end.
 static int64_t workgroups(int64_t M, int lr, int threads, int lanes = 1024) {
     const int rows = lr > 64 ? 1 : 256 / lr;
     const int64_t n = (M + rows - 1) / rows, most = lanes / threads * 256;
