@@ -1,6 +1,7 @@
 """Activations kept in 8 bits for the backward pass, and the weight gradient that reads them as they are: `acx_act8_pack` / `_unpack` /
 `_weight_grad` (csrc/acx_act8.hip).  Opt-in (`--checkpoint-8bit` of ac_solver.agents.ppo); the reference keeps float32 activations
 (ac_solver/agents/ppo_agent.py:11-109, agents/training.py:273-330)."""
+import re
 import threading
 
 import torch
@@ -115,9 +116,9 @@ def packing():
     return getattr(_inside, "depth", 0) > 0
 
 
-# nodes of autograd that hand a tensor on with the same values, up to a rounding to another type (their names without the number behind them)
-_SAME_VALUES = frozenset(n + "Backward" for n in ("Alias AsStrided Clone Diagonal Expand Movedim Permute ReshapeAlias Select Slice Split SplitWithSizes Squeeze T ToCopy Transpose Unbind "
-                                                  "Unfold UnsafeSplit UnsafeView Unsqueeze View").split())
+# nodes of autograd that hand a tensor on with the same values, up to a rounding to another type (torch's own have a number behind their names)
+_SAME_VALUES = re.compile("(Alias|AsStrided|Clone|Diagonal|Expand|Movedim|Permute|ReshapeAlias|Select|Slice|Split|SplitWithSizes|Squeeze|T|ToCopy|Transpose|Unbind|Unfold|UnsafeSplit|UnsafeView|"
+                          "Unsqueeze|View)Backward[0-9]+")
 
 
 def _is_leaf(t):
@@ -127,7 +128,7 @@ def _is_leaf(t):
     if t.grad_fn is None or (t._base is not None and t._base.is_leaf and t._base.requires_grad):
         return True
     node = t.grad_fn
-    while node.name().rstrip("0123456789") in _SAME_VALUES:
+    while _SAME_VALUES.fullmatch(node.name()):
         node = node.next_functions[0][0]
         if node is None:
             return True

@@ -315,3 +315,29 @@ def test_a_checkpoint8_block_that_could_not_be_entered_leaves_nothing_behind():
             assert A.packing()
         assert A.packing()
     assert not A.packing()
+
+
+def test_what_counts_as_a_leaf_in_another_form():
+    """views and copies of a leaf, and nothing that has been computed: not behind a view or a copy either, nor a function that happens to be named like one of torch's"""
+    from ac_solver.agents.activation8 import _is_leaf
+
+    class View(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, x):
+            return x * 2
+
+        @staticmethod
+        def backward(ctx, g):
+            return g * 2
+
+    w = torch.randn(8, 8, requires_grad=True)
+    buffer, changed, part = torch.zeros(8, 8), w.clone(), w.clone()
+    buffer[0] = w[0] * 2
+    changed.mul_(2)
+    part[0] *= 2
+    for t in (w, w.detach(), w.t(), w.view(4, 16)[None].expand(2, 4, 16), w.chunk(2)[1], w.mT, w.unbind(0)[1], w.clone(), w.bfloat16(), w.bfloat16().t(), w.t().bfloat16(), w.double().float()[1:],
+              w.t().reshape(-1), buffer.detach()):
+        assert _is_leaf(t)
+    for t in (w * 1, (w * 1).t(), (w * 1).bfloat16(), w.bfloat16().exp().t(), torch.cat([w, w]), w[torch.tensor([1, 2])], buffer, buffer.t(), changed, changed.t(), part, part.t(), View.apply(w),
+              View.apply(w).t()):
+        assert not _is_leaf(t)
